@@ -274,6 +274,68 @@ LINREC_API int linrec_b200_bwd_dim(const void* dy, const void* c, const void* y,
                                    const linrec_opts* opts, void* workspace, size_t workspace_bytes,
                                    void* stream);
 
+/* ---- gated recurrence on channels-last tensors -----------------------------------------------------------
+ *     h[t] = a[t] * h[t-1] + b[t] * u[t],   y[t] = h[t] rounded to the storage type, state in fp32
+ * along the rows of (nrows, nchan) tensors whose rows have their own strides, with s the logistic function:
+ *   forget form (input_gate and decay NULL)   a = s(forget), b = s(-forget), u = x
+ *   decay form                                 log a = -decay_scale * softplus(decay) * s(forget),
+ *                                              b = sqrt(1 - a^2), u = s(input_gate) * x
+ * Sequences: with cu_seqlens, nseq + 1 non-decreasing DEVICE offsets (int32, or int64 with cu_is_64); rows
+ * that no sequence holds give zeros in y and in the gradients.  Without, nseq sequences of `seqlen` rows
+ * each (nrows = nseq * seqlen).  `reverse` scans every sequence from its last row to its first.
+ * States are (nseq, nchan) fp32, contiguous; NULL initial_state means zeros.  The final states of sequences
+ * without rows are not written, nor are their initial states' gradients.
+ * Results (y, dx, dforget, dinput_gate) have rows at stride nchan.  Backward pass: the checkpoints that the
+ * forward pass left (linrec_b200_gated_checkpoint_rows rows of nchan floats), and for the decay form
+ * linrec_b200_gated_scratch_size bytes of scratch.  LINREC_DTYPE_F32, _BF16 and _F16.  The workspace is one
+ * of those of the other entry points (zeroed once), linrec_b200_gated_workspace_size bytes; it serves
+ * either pass.  Option: waitBudgetMs.  No counterpart in the reference, whose operators take finished
+ * coefficients. */
+typedef struct linrec_gated_args {
+    const void* x;
+    const void* forget;
+    const void* input_gate;      /* decay form, else NULL */
+    int64_t x_stride, forget_stride, input_gate_stride;   /* elements between rows */
+    const float* decay;          /* decay form: nchan values, else NULL */
+    float decay_scale;
+    int dtype;
+    int reverse;
+    int cu_is_64;
+    const void* cu_seqlens;      /* or NULL */
+    int64_t nseq, seqlen, nrows, nchan;
+    const float* initial_state;  /* or NULL */
+    float* checkpoints;          /* forward: or NULL; backward: required */
+    void* y;                     /* forward */
+    float* final_state;          /* forward, or NULL */
+    const void* dy;              /* backward, as are all below */
+    int64_t dy_stride;
+    const float* d_final_state;  /* or NULL */
+    void* dx;
+    void* dforget;
+    void* dinput_gate;           /* decay form */
+    float* ddecay;               /* decay form: nchan values */
+    float* d_initial_state;      /* or NULL */
+    void* scratch;               /* decay form */
+    size_t scratch_bytes;
+} linrec_gated_args;
+LINREC_API size_t linrec_b200_gated_workspace_size(const linrec_gated_args* args);
+LINREC_API size_t linrec_b200_gated_scratch_size(const linrec_gated_args* args);
+LINREC_API int64_t linrec_b200_gated_checkpoint_rows(const linrec_gated_args* args);
+LINREC_API int linrec_b200_gated_fwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+LINREC_API int linrec_b200_gated_bwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* One token of each sequence: row r of x, forget(, input_gate) advances row slots[r] of `state` (nslots rows
+ * of nchan floats, state_stride apart, updated in place) and gives row r of y.  Without slots row r advances
+ * state row r (nrows <= nslots).  A slot outside [0, nslots) marks a padding row: its y is zero and no state
+ * changes.  Rows that name the same slot are consecutive tokens of one sequence, in row order. */
+LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const void* input_gate, int64_t x_stride,
+                                      int64_t forget_stride, int64_t input_gate_stride, const float* decay,
+                                      float decay_scale, void* y, float* state, int64_t state_stride, int64_t nslots,
+                                      const void* slots, int slots_are_64, int64_t nrows, int64_t nchan, int dtype,
+                                      void* stream);
+
 /* Number of kernels this library has launched in this process (all threads). */
 LINREC_API uint64_t linrec_b200_launch_count(void);
 
@@ -285,7 +347,8 @@ LINREC_API const char* linrec_b200_last_cuda_error(void);
 /* Text for a status code. */
 LINREC_API const char* linrec_b200_strerror(int code);
 
-/* Library version, e.g. 200 for 0.2.0 (0.2.0 changed the fix-up entry points: they take the operands x / dy). */
+/* Library version, e.g. 200 for 0.2.0 (0.2.0 changed the fix-up entry points: they take the operands x / dy;
+ * 0.3.0 added the gated recurrence and the group norm). */
 LINREC_API int linrec_b200_version(void);
 
 #ifdef __cplusplus

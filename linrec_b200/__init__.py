@@ -22,8 +22,10 @@ from .ops import (  # noqa: F401
 )
 
 from .general import linrec_general  # noqa: E402,F401
+from .gated import linrec_gated, linrec_gated_step  # noqa: E402,F401
 
 linrec = linrec_pipe
 
 __version__ = "0.2.0"
-__all__ = ["linrec", "linrec_ref", "linrec_tile", "linrec_pipe", "linrec_general", "check_status"]
+__all__ = ["linrec", "linrec_ref", "linrec_tile", "linrec_pipe", "linrec_general", "linrec_gated", "linrec_gated_step",
+           "check_status"]

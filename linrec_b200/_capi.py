@@ -34,6 +34,20 @@ class LinrecOpts(ctypes.Structure):
                 ("values", ctypes.POINTER(ctypes.c_int))]
 
 
+class GatedArgs(ctypes.Structure):
+    """linrec_gated_args of the header, field for field; zeroed by ctypes (null pointers)."""
+    _fields_ = [("x", ctypes.c_void_p), ("forget", ctypes.c_void_p), ("input_gate", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("forget_stride", ctypes.c_int64), ("input_gate_stride", ctypes.c_int64),
+                ("decay", ctypes.c_void_p), ("decay_scale", ctypes.c_float), ("dtype", ctypes.c_int),
+                ("reverse", ctypes.c_int), ("cu_is_64", ctypes.c_int), ("cu_seqlens", ctypes.c_void_p),
+                ("nseq", ctypes.c_int64), ("seqlen", ctypes.c_int64), ("nrows", ctypes.c_int64), ("nchan", ctypes.c_int64),
+                ("initial_state", ctypes.c_void_p), ("checkpoints", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("final_state", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64),
+                ("d_final_state", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dforget", ctypes.c_void_p),
+                ("dinput_gate", ctypes.c_void_p), ("ddecay", ctypes.c_void_p), ("d_initial_state", ctypes.c_void_p),
+                ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
+
+
 def _load() -> ctypes.CDLL:
     path = _build.LIB_PATH
     try:
@@ -90,6 +104,15 @@ def _load() -> ctypes.CDLL:
     lib.linrec_b200_fwd_static.restype = i32
     lib.linrec_b200_static_workspace.argtypes = [pp, ctypes.POINTER(sz)]
     lib.linrec_b200_static_workspace.restype = i32
+    pg = ctypes.POINTER(GatedArgs)
+    for name, res in (("workspace_size", sz), ("scratch_size", sz), ("checkpoint_rows", i64)):
+        fn = getattr(lib, "linrec_b200_gated_" + name)
+        fn.argtypes, fn.restype = [pg], res
+    for name in ("fwd", "bwd"):
+        fn = getattr(lib, "linrec_b200_gated_" + name)
+        fn.argtypes, fn.restype = [pg, po, vp, sz, vp], i32
+    lib.linrec_b200_gated_step.argtypes = [vp, vp, vp, i64, i64, i64, vp, ctypes.c_float, vp, vp, i64, i64, vp, i32, i64, i64, i32, vp]
+    lib.linrec_b200_gated_step.restype = i32
     lib.linrec_b200_launch_count.argtypes = []
     lib.linrec_b200_launch_count.restype = ctypes.c_uint64
     lib.linrec_b200_last_cuda_error.argtypes = []

@@ -69,10 +69,10 @@ def _all_deps():
 
 
 def _translation_units():
-    """capi.cu (host logic, the small kernels) and the variants_*.cu files the kernel variants are spread
-    over so that they compile side by side."""
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC)
-                  if f.endswith(".cu") and (f == "capi.cu" or f.startswith("variants_")))
+    """capi.cu (host logic, the small kernels), the variants_*.cu files the kernel variants are spread
+    over so that they compile side by side, and the operators around the scan (gated.cu, norm.cu): every
+    .cu file but the standalone harness."""
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cu") and f != "linrec_cli.cu")
 
 
 class _BuildLock:

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "../../include/linrec_b200.h"
+#include "host.h"
 #include "variants.h"
 #include "shard_kernels.cuh"
 
@@ -171,11 +172,7 @@ const std::vector<GenericVariant>& word_variants()
 }
 
 // ---- per-device facts and per-kernel launch facts ------------------------------------------------
-struct DeviceInfo {
-    int sm_count = 0;
-    int clock_khz = 0;
-    int max_smem_optin = 0;
-};
+using linrec_host::DeviceInfo;
 
 std::mutex g_mutex;
 std::unordered_map<int, DeviceInfo> g_devices;
@@ -279,10 +276,7 @@ int occupancy(const void* fn, int threads, size_t smem, int& out)
 }
 
 // ---- tensor maps ---------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                   CUtensorMapFloatOOBfill);
+using linrec_host::EncodeTiledFn;
 
 EncodeTiledFn encode_tiled_fn()
 {
@@ -1155,6 +1149,15 @@ int static_scratch_address(void** out)
 }
 }  // namespace
 
+// What the other host files use of this one (host.h).
+namespace linrec_host {
+int device_facts(DeviceInfo& out) { return ::device_info(out); }
+int occupancy(const void* fn, int threads, size_t smem, int& out) { return ::occupancy(fn, threads, smem, out); }
+EncodeTiledFn encode_tiled_fn() { return ::encode_tiled_fn(); }
+void note_cuda_error(const char* where, const char* what) { ::note_cuda_error(where, what); }
+int launch_result(const char* where) { return ::launch_result(where); }
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+}  // namespace linrec_host
 
 // =================================================================================================
 //  C ABI

@@ -1,0 +1,206 @@
+// Host side of the gated recurrence (include/linrec_b200.h): argument checks, how the sequences are laid
+// on scan axes, launches.
+#include "gated_kernels.cuh"
+#include "host.h"
+
+#include <cstring>
+
+namespace {
+
+using linrec::GatedParams;
+using linrec::GatedStepParams;
+using linrec::kGatedChannels;
+using linrec::kGatedCheckpoint;
+using linrec::kGatedThreads;
+using linrec_host::DeviceInfo;
+
+bool known_dtype(int dtype)
+{
+    return dtype == LINREC_DTYPE_F32 || dtype == LINREC_DTYPE_BF16 || dtype == LINREC_DTYPE_F16;
+}
+
+struct Axes {
+    int nb;            // scan axes side by side
+    int64_t nrows;     // rows per axis
+};
+
+// A batch of equal lengths gets one axis per entry, whose tiles depend on nothing but their own sequence,
+// unless the entries are so short that the last tile of each would be mostly empty; those, and packed
+// sequences, share one axis.  128 positions: the longest tile of any type, so that the choice (which the
+// checkpoints depend on) is the same in both passes.
+Axes axes_of(const linrec_gated_args& a)
+{
+    if (!a.cu_seqlens && a.nseq > 1 && (a.seqlen >= 512 || a.seqlen % 128 == 0)) return Axes{(int)a.nseq, a.seqlen};
+    return Axes{1, a.nrows};
+}
+
+int check(const linrec_gated_args* a)
+{
+    if (!a || a->nseq < 0 || a->nrows < 0 || a->nchan < 0 || (!a->cu_seqlens && a->seqlen < 0)) return LINREC_ERR_INVALID_ARG;
+    if (!known_dtype(a->dtype)) return LINREC_ERR_NOT_IMPLEMENTED;
+    if (!a->decay != !a->input_gate) return LINREC_ERR_INVALID_ARG;
+    if (a->nseq >= 0x7fffffffLL || a->nrows >= 0x40000000LL || a->nchan >= 0x40000000LL) return LINREC_ERR_INVALID_ARG;
+    if (!a->cu_seqlens && (a->seqlen > a->nrows || a->nseq * a->seqlen != a->nrows)) return LINREC_ERR_INVALID_ARG;
+    const int64_t rows = (a->nrows + 63) / 64, chans = (a->nchan + 63) / 64;
+    if ((rows + a->nseq) * chans >= 0x7f000000LL) return LINREC_ERR_INVALID_ARG;   // tickets are 32-bit
+    return LINREC_OK;
+}
+
+int run_length(int dtype, bool bwd) { return bwd || dtype == LINREC_DTYPE_F32 ? 64 : 128; }
+
+int parse(const linrec_opts* o, int& wait_ms)
+{
+    wait_ms = 2000;
+    if (!o || o->n_opts == 0) return LINREC_OK;
+    if (o->n_opts < 0 || !o->names || !o->values) return LINREC_ERR_INVALID_ARG;
+    for (int i = 0; i < o->n_opts; ++i) {
+        if (!o->names[i]) return LINREC_ERR_INVALID_ARG;
+        if (strcmp(o->names[i], "waitBudgetMs")) return LINREC_ERR_NOT_IMPLEMENTED;
+        wait_ms = o->values[i];
+    }
+    return LINREC_OK;
+}
+
+using Fn = void (*)(const GatedParams);
+template <typename ST>
+Fn pick(bool bwd, bool decay)
+{
+    if (bwd) return decay ? linrec::gated_bwd_kernel<ST, true> : linrec::gated_bwd_kernel<ST, false>;
+    return decay ? linrec::gated_fwd_kernel<ST, true> : linrec::gated_fwd_kernel<ST, false>;
+}
+
+int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream_)
+{
+    int rc = check(args);
+    if (rc != LINREC_OK) return rc;
+    const linrec_gated_args& a = *args;
+    const bool decay = a.decay != nullptr;
+    int wait_ms;
+    rc = parse(opts, wait_ms);
+    if (rc != LINREC_OK) return rc;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (a.nchan == 0) return LINREC_OK;
+    if (a.nrows == 0) {
+        if (bwd && decay && a.ddecay && cudaMemsetAsync(a.ddecay, 0, (size_t)a.nchan * 4, stream) != cudaSuccess) {
+            linrec_host::note_cuda_error("cudaMemsetAsync", cudaGetErrorString(cudaGetLastError()));
+            return LINREC_ERR_CUDA;
+        }
+        return LINREC_OK;
+    }
+    if (!a.x || !a.forget || a.x_stride < a.nchan || a.forget_stride < a.nchan) return LINREC_ERR_INVALID_ARG;
+    if (decay && a.input_gate_stride < a.nchan) return LINREC_ERR_INVALID_ARG;
+    if (!bwd && !a.y) return LINREC_ERR_INVALID_ARG;
+    if (bwd && (!a.dy || a.dy_stride < a.nchan || !a.dx || !a.dforget || !a.checkpoints)) return LINREC_ERR_INVALID_ARG;
+    if (bwd && decay && (!a.dinput_gate || !a.ddecay || !a.scratch || a.scratch_bytes < linrec_b200_gated_scratch_size(args)))
+        return LINREC_ERR_INVALID_ARG;
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < linrec_b200_gated_workspace_size(args))
+        return LINREC_ERR_WORKSPACE;
+    DeviceInfo dev;
+    rc = linrec_host::device_facts(dev);
+    if (rc != LINREC_OK) return rc;
+
+    const Axes ax = axes_of(a);
+    GatedParams p{};
+    p.x = a.x; p.f = a.forget; p.ig = a.input_gate; p.dy = a.dy;
+    p.sx = a.x_stride; p.sf = a.forget_stride; p.si = a.input_gate_stride; p.sdy = a.dy_stride;
+    p.y = a.y; p.dx = a.dx; p.df = a.dforget; p.di = a.dinput_gate;
+    p.decay = a.decay; p.scale = a.decay_scale;
+    p.h0 = a.initial_state; p.hT = a.final_state; p.dhT = a.d_final_state; p.dh0 = a.d_initial_state;
+    p.ckpt = a.checkpoints;
+    p.dlam = static_cast<float*>(a.scratch);
+    p.cu = a.cu_seqlens; p.cu64 = a.cu_is_64; p.nseq = (int)a.nseq; p.seqlen = a.seqlen;
+    p.nrows = ax.nrows; p.nb = ax.nb;
+    p.D = (int)a.nchan; p.dtiles = linrec_host::ceil_div_i(a.nchan, kGatedChannels); p.units = p.dtiles * p.nb;
+    p.nk = linrec_host::ceil_div_i(ax.nrows, run_length(a.dtype, bwd));
+    p.nck = linrec_host::ceil_div_i(ax.nrows, kGatedCheckpoint);
+    p.ntickets = (long long)p.nk * p.units;
+    p.reverse = a.reverse != 0;
+    p.header = static_cast<uint32_t*>(workspace);
+    p.desc = reinterpret_cast<linrec::TileDesc*>(static_cast<char*>(workspace) + linrec::kHeaderBytes);
+    p.wait_budget = (long long)wait_ms * (long long)dev.clock_khz;
+
+    const Fn fn = a.dtype == LINREC_DTYPE_F32 ? pick<float>(bwd, decay)
+                : a.dtype == LINREC_DTYPE_BF16 ? pick<__nv_bfloat16>(bwd, decay) : pick<__half>(bwd, decay);
+    int occ = 0;
+    rc = linrec_host::occupancy(reinterpret_cast<const void*>(fn), kGatedThreads, 0, occ);
+    if (rc != LINREC_OK) return rc;
+    long long grid = (long long)dev.sm_count * occ;
+    if (grid > p.ntickets) grid = p.ntickets;
+    rc = linrec_host::launch("gated recurrence", fn, dim3((unsigned)grid), kGatedThreads, 0, stream, p);
+    if (rc != LINREC_OK || !bwd || !decay) return rc;
+    return linrec_host::launch("decay gradient", linrec::gated_decay_grad_kernel, dim3((unsigned)linrec_host::ceil_div_i(a.nchan, 32)), 256, 0,
+                               stream, (const float*)p.dlam, (long long)p.nk * p.nb, p.D, p.decay, a.ddecay);
+}
+
+template <typename ST>
+int launch_step(const GatedStepParams& p, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)p.rows, (unsigned)linrec_host::ceil_div_i(p.D, 256));
+    return linrec_host::launch("gated step", p.decay ? linrec::gated_step_kernel<ST, true> : linrec::gated_step_kernel<ST, false>, grid,
+                               128, 0, stream, p);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t linrec_b200_gated_workspace_size(const linrec_gated_args* args)
+{
+    size_t n = linrec::kHeaderBytes;
+    if (check(args) == LINREC_OK) {
+        const Axes ax = axes_of(*args);
+        const size_t tiles = (size_t)((ax.nrows + 63) / 64) * ax.nb * (size_t)((args->nchan + kGatedChannels - 1) / kGatedChannels);
+        n += tiles * kGatedChannels * sizeof(linrec::TileDesc);
+    }
+    return n;
+}
+
+size_t linrec_b200_gated_scratch_size(const linrec_gated_args* args)
+{
+    if (check(args) != LINREC_OK || !args->decay) return 0;
+    return (size_t)linrec_b200_gated_checkpoint_rows(args) * (size_t)args->nchan * sizeof(float);
+}
+
+int64_t linrec_b200_gated_checkpoint_rows(const linrec_gated_args* args)
+{
+    if (check(args) != LINREC_OK) return 0;
+    const Axes ax = axes_of(*args);
+    return (ax.nrows + kGatedCheckpoint - 1) / kGatedCheckpoint * ax.nb;
+}
+
+int linrec_b200_gated_fwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return launch_gated(false, args, opts, workspace, workspace_bytes, stream);
+}
+
+int linrec_b200_gated_bwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream)
+{
+    return launch_gated(true, args, opts, workspace, workspace_bytes, stream);
+}
+
+int linrec_b200_gated_step(const void* x, const void* forget, const void* input_gate, int64_t x_stride, int64_t forget_stride,
+                           int64_t input_gate_stride, const float* decay, float decay_scale, void* y, float* state,
+                           int64_t state_stride, int64_t nslots, const void* slots, int slots_are_64, int64_t nrows, int64_t nchan,
+                           int dtype, void* stream)
+{
+    if (!known_dtype(dtype)) return LINREC_ERR_NOT_IMPLEMENTED;
+    if (nrows < 0 || nchan < 0 || nslots < 0 || nrows >= 0x7fffffffLL || nslots >= 0x7fffffffLL || nchan > 256LL * 65535)
+        return LINREC_ERR_INVALID_ARG;
+    if (!decay != !input_gate) return LINREC_ERR_INVALID_ARG;
+    if (nrows == 0 || nchan == 0) return LINREC_OK;
+    if (!x || !forget || !y || (!state && nslots > 0) || x_stride < nchan || forget_stride < nchan || state_stride < nchan ||
+        (decay && input_gate_stride < nchan) || (!slots && nrows > nslots))
+        return LINREC_ERR_INVALID_ARG;
+    DeviceInfo dev;
+    const int rc = linrec_host::device_facts(dev);
+    if (rc != LINREC_OK) return rc;
+    GatedStepParams p{};
+    p.x = x; p.f = forget; p.ig = input_gate; p.sx = x_stride; p.sf = forget_stride; p.si = input_gate_stride;
+    p.y = y; p.decay = decay; p.scale = decay_scale; p.state = state; p.sstate = state_stride;
+    p.slots = slots; p.slots64 = slots_are_64; p.rows = (int)nrows; p.nslots = (int)nslots; p.D = (int)nchan;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == LINREC_DTYPE_F32 ? launch_step<float>(p, s)
+         : dtype == LINREC_DTYPE_BF16 ? launch_step<__nv_bfloat16>(p, s) : launch_step<__half>(p, s);
+}
+
+}  // extern "C"

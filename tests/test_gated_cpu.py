@@ -1,0 +1,91 @@
+"""Refusals of the gated recurrence and its step that need no GPU: every check runs before a device is
+touched, and tensors outside a GPU are refused like everywhere in the package."""
+import ctypes
+
+import pytest
+import torch
+
+import linrec_b200 as lb
+from linrec_b200 import _capi
+
+X = torch.zeros(2, 5, 8)
+P = torch.zeros(10, 8)
+
+
+@pytest.mark.parametrize("why,call", [
+    ("sequence and a channel", lambda: lb.linrec_gated(torch.zeros(8), torch.zeros(8))),
+    ("not supported", lambda: lb.linrec_gated(X.double(), X.double())),
+    ("not supported", lambda: lb.linrec_gated(X.long(), X.long())),
+    ("forget must have the sizes", lambda: lb.linrec_gated(X, X[:, :4])),
+    ("forget must have the dtype", lambda: lb.linrec_gated(X, X.bfloat16())),
+    ("input_gate must have the sizes", lambda: lb.linrec_gated(X, X, input_gate=X[:1], decay=torch.zeros(8))),
+    ("come together", lambda: lb.linrec_gated(X, X, input_gate=X)),
+    ("come together", lambda: lb.linrec_gated(X, X, decay=torch.zeros(8))),
+    ("one value per channel", lambda: lb.linrec_gated(X, X, input_gate=X, decay=torch.zeros(1))),
+    ("floating-point", lambda: lb.linrec_gated(X, X, input_gate=X, decay=torch.zeros(8, dtype=torch.int32))),
+    ("decay_scale", lambda: lb.linrec_gated(X, X, input_gate=X, decay=torch.zeros(8), decay_scale=0.0)),
+    ("decay_scale", lambda: lb.linrec_gated(X, X, input_gate=X, decay=torch.zeros(8), decay_scale=float("nan"))),
+    ("decay_scale", lambda: lb.linrec_gated(X, X, input_gate=X, decay=torch.zeros(8), decay_scale=float("inf"))),
+    ("one row of channels per sequence", lambda: lb.linrec_gated(X, X, initial_state=torch.zeros(8))),
+    ("one row of channels per sequence", lambda: lb.linrec_gated(P, P, initial_state=torch.zeros(3, 8), cu_seqlens=torch.zeros(3, dtype=torch.int32))),
+    ("floating-point", lambda: lb.linrec_gated(X, X, initial_state=torch.zeros(2, 8, dtype=torch.int64))),
+    ("int32 or int64", lambda: lb.linrec_gated(P, P, cu_seqlens=torch.zeros(3))),
+    ("one dimension", lambda: lb.linrec_gated(P, P, cu_seqlens=torch.zeros(3, 1, dtype=torch.int32))),
+    ("one offset more", lambda: lb.linrec_gated(P, P, cu_seqlens=torch.zeros(0, dtype=torch.int32))),
+    ("two dimensions", lambda: lb.linrec_gated(X, X, cu_seqlens=torch.zeros(3, dtype=torch.int32))),
+    ("CUDA tensors", lambda: lb.linrec_gated(X, X)),
+    ("CUDA tensors", lambda: lb.linrec_gated(P, P, cu_seqlens=torch.zeros(3, dtype=torch.int32))),
+    ("two dimensions", lambda: lb.linrec_gated_step(X, X, P)),
+    ("one row of channels per slot", lambda: lb.linrec_gated_step(P, P, torch.zeros(10, 7))),
+    ("state must be float32", lambda: lb.linrec_gated_step(P, P, P.bfloat16())),
+    ("must not overlap", lambda: lb.linrec_gated_step(P, P, torch.zeros(1, 8).expand(10, 8))),
+    ("must not overlap", lambda: lb.linrec_gated_step(P, P, torch.zeros(8, 10).t())),
+    ("one row per row", lambda: lb.linrec_gated_step(P, P, torch.zeros(9, 8))),
+    ("int32 or int64", lambda: lb.linrec_gated_step(P, P, P, slots=torch.zeros(10))),
+    ("one state row per row", lambda: lb.linrec_gated_step(P, P, P, slots=torch.zeros(9, dtype=torch.int32))),
+    ("come together", lambda: lb.linrec_gated_step(P, P, P, decay=torch.zeros(8))),
+    ("CUDA tensors", lambda: lb.linrec_gated_step(P, P, P)),
+])
+def test_refusals(why, call):
+    with pytest.raises(RuntimeError, match=why):
+        call()
+
+
+def _args(**kw):
+    a = _capi.GatedArgs()
+    base = {"nseq": 2, "seqlen": 5, "nrows": 10, "nchan": 8, "x": 16, "forget": 16, "x_stride": 8, "forget_stride": 8, "y": 16}
+    for k, v in {**base, **kw}.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("code,kw", [
+    (_capi.ERR_INVALID_ARG, {"nrows": -1}),
+    (_capi.ERR_INVALID_ARG, {"nrows": 11}),
+    (_capi.ERR_INVALID_ARG, {"nseq": 3}),
+    (_capi.ERR_INVALID_ARG, {"x_stride": 7}),
+    (_capi.ERR_INVALID_ARG, {"x": None}),
+    (_capi.ERR_INVALID_ARG, {"y": None}),
+    (_capi.ERR_INVALID_ARG, {"decay": 16}),
+    (_capi.ERR_INVALID_ARG, {"nrows": 1 << 40, "seqlen": 1 << 39}),
+    (_capi.ERR_NOT_IMPLEMENTED, {"dtype": _capi.DTYPE_F64}),
+    (_capi.ERR_NOT_IMPLEMENTED, {"dtype": 17}),
+    (_capi.ERR_WORKSPACE, {}),
+])
+def test_c_entry_refuses(code, kw):
+    a = _args(**kw)
+    assert _capi.lib.linrec_b200_gated_fwd(ctypes.byref(a), None, None, 0, None) == code
+
+
+def test_c_entry_options_and_sizes():
+    a = _args()
+    opts, keep = _capi.make_opts({"kStages": 2})
+    assert _capi.lib.linrec_b200_gated_fwd(ctypes.byref(a), opts, None, 0, None) == _capi.ERR_NOT_IMPLEMENTED
+    assert _capi.lib.linrec_b200_gated_fwd(None, None, None, 0, None) == _capi.ERR_INVALID_ARG
+    assert _capi.lib.linrec_b200_gated_bwd(ctypes.byref(a), None, None, 0, None) == _capi.ERR_INVALID_ARG
+    # no rows or channels: nothing to do, whatever the pointers are
+    assert _capi.lib.linrec_b200_gated_fwd(ctypes.byref(_args(nrows=0, seqlen=0, x=None)), None, None, 0, None) == _capi.OK
+    assert _capi.lib.linrec_b200_gated_checkpoint_rows(ctypes.byref(a)) == 1
+    assert _capi.lib.linrec_b200_gated_checkpoint_rows(ctypes.byref(_args(nseq=3, seqlen=600, nrows=1800))) == 30
+    assert _capi.lib.linrec_b200_gated_scratch_size(ctypes.byref(a)) == 0
+    assert _capi.lib.linrec_b200_gated_step(None, None, None, 8, 8, 8, None, 8.0, None, None, 8, 4, None, 0, 4, 8, 0, None) == _capi.ERR_INVALID_ARG

@@ -1,0 +1,451 @@
+"""Gated recurrence, its gradients and its one-token step on the GPU, against a sequential evaluation in 64
+bits (tests/gated_oracle.py, which also carries the error bound of a float32 evaluation).  Results in 16 bits
+may be off by half a step of their type on top of that."""
+import numpy as np
+import pytest
+import torch
+
+import gated_oracle as go
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = {"inputs": "dx", "forget": "dforget", "input_gate": "dinput", "decay": "ddecay", "initial_state": "dinitial"}
+
+
+def _lb():
+    import linrec_b200
+    return linrec_b200
+
+
+def _check(got, want, what):
+    value, bound = want
+    dt = got.dtype
+    g = got.detach().double().cpu().numpy().reshape(value.shape)
+    tol = bound + 1e-37
+    if dt != torch.float32:
+        # half a step of the type at the largest value the bound allows; subnormal steps of fp16
+        tol = tol + (np.abs(value) + bound) * torch.finfo(dt).eps / 2 + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2
+    bad = ~(np.abs(g - value) <= tol)
+    if bad.any():
+        at = np.unravel_index(np.argmax(np.where(bad, np.abs(g - value) / tol, 0)), bad.shape)
+        raise AssertionError(f"{what}: {bad.sum()} of {bad.size} outside, worst at {at}: {g[at]} for {value[at]} +- {tol[at]}")
+
+
+def _case(shape, decay, dtype, seed=0, states=True, nseq=None, spread=4.0):
+    g = torch.Generator().manual_seed(seed + 1)
+    D = shape[-1]
+    lead = shape[:-2] if nseq is None else (nseq,)
+    c = {"inputs": torch.randn(shape, generator=g), "forget": torch.rand(D, generator=g) * spread + torch.randn(shape, generator=g),
+         "dy": torch.randn(shape, generator=g)}
+    if decay:
+        c["input_gate"] = torch.randn(shape, generator=g)
+        c["decay"] = torch.rand(D, generator=g) * 5.0 - 5.0
+    if states:
+        c["initial_state"] = torch.randn(*lead, D, generator=g)
+        c["dfinal"] = torch.randn(*lead, D, generator=g)
+    for n in ("inputs", "forget", "input_gate", "dy"):
+        if n in c:
+            c[n] = c[n].to(dtype)
+    return c
+
+
+def _oracle(c, **kw):
+    n = {k: (v.double().numpy() if v is not None else None) for k, v in c.items()}
+    return go.evaluate(n["inputs"], n["forget"], n.get("input_gate"), n.get("decay"), h0=n.get("initial_state"), dy=n["dy"],
+                       dfinal=n.get("dfinal"), **kw)
+
+
+def _run(c, place=None, **kw):
+    """Forward and backward through the public entry point: dict of results."""
+    dev = {k: (place or (lambda _, t: t.to(DEV)))(k, v) for k, v in c.items()}
+    leaves = {k: dev[k].requires_grad_(True) for k in NAMES if k in dev}
+    y, final = _lb().linrec_gated(leaves["inputs"], leaves["forget"], return_state=True, **kw,
+                                  **{k: v for k, v in leaves.items() if k not in ("inputs", "forget")})
+    outs, grads = ([y, final], [dev["dy"], dev["dfinal"]]) if "dfinal" in dev else ([y], [dev["dy"]])
+    got = torch.autograd.grad(outs, list(leaves.values()), grads)
+    return {"y": y, "final": final, **{NAMES[k]: t for k, t in zip(leaves, got)}}
+
+
+def _compare(got, want):
+    for n, t in got.items():
+        _check(t, want[n], n)
+    _lb().check_status()
+
+
+SHAPES = [(1, 1, 1), (2, 1, 64), (1, 63, 65), (2, 64, 8), (3, 130, 72), (2, 512, 136), (1, 1000, 33), (5, 129, 64), (1, 4100, 16),
+          (33, 3, 66), (2, 3, 70, 40), (4, 384, 128), (70, 128)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_scan_and_gradients(shape, decay, dtype):
+    for reverse in (False, True):
+        for states in (False, True):
+            c = _case(shape, decay, dtype, seed=len(shape) + shape[-1], states=states)
+            _compare(_run(c, reverse=reverse), _oracle(c, reverse=reverse))
+
+
+LENGTHS = {"mixed": (0, [0, 1, 0, 5, 200, 0, 64, 1, 1, 0], 0), "gaps": (3, [130, 1, 128, 77], 19), "one": (0, [300], 0),
+           "singles": (0, [1] * 150, 2), "none": (0, [], 40), "empty": (5, [0, 0], 70), "long": (0, [3, 2500, 0, 700], 64)}
+
+
+@pytest.mark.parametrize("name", LENGTHS)
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_packed_sequences(name, decay, dtype):
+    front, lens, tail = LENGTHS[name]
+    offsets = [front]
+    for n in lens:
+        offsets.append(offsets[-1] + n)
+    for D, reverse, kind in ((72, False, torch.int32), (40, True, torch.int64), (67, False, torch.int64)):
+        c = _case((offsets[-1] + tail, D), decay, dtype, nseq=len(lens), seed=D)
+        # what lies outside the sequences must not matter
+        outside = torch.ones(offsets[-1] + tail, dtype=torch.bool)
+        outside[offsets[0]:offsets[-1]] = False
+        want = _oracle(c, offsets=offsets, reverse=reverse)
+        for i, n in enumerate(k for k in ("inputs", "forget", "input_gate", "dy") if k in c):
+            c[n] = c[n].clone()
+            c[n][outside] = [float("nan"), float("inf"), -float("inf"), float("nan")][i]
+        got = _run(c, cu_seqlens=torch.tensor(offsets, dtype=kind, device=DEV), reverse=reverse)
+        _compare(got, want)
+        for n in ("y", "dx", "dforget", "dinput"):
+            if n in got:
+                assert (got[n][outside.to(DEV)] == 0).all(), n
+
+
+def test_a_sequence_keeps_its_infinities():
+    """NaN and infinity in one sequence, its states included, leave the others' bits alone."""
+    offsets = [0, 100, 164, 230, 500]
+    for decay in (False, True):
+        for reverse in (False, True):
+            cu = torch.tensor(offsets, dtype=torch.int32, device=DEV)
+            c = _case((500, 66), decay, torch.float32, nseq=4)
+            clean = _run(c, cu_seqlens=cu, reverse=reverse)
+            for n in c:
+                if n in ("initial_state", "dfinal"):
+                    c[n] = c[n].clone()
+                    c[n][2] = float("nan")
+                elif n != "decay":
+                    c[n] = c[n].clone()
+                    c[n][180:200] = float("inf") if n == "forget" else float("nan")
+            dirty = _run(c, cu_seqlens=cu, reverse=reverse)
+            for n in clean:
+                if n == "ddecay":
+                    continue
+                keep = torch.ones(clean[n].shape[0], dtype=torch.bool, device=DEV)
+                if clean[n].shape[0] == 500:
+                    keep[164:230] = False
+                else:
+                    keep[2] = False
+                assert torch.equal(clean[n][keep], dirty[n][keep]), n
+                assert not torch.isfinite(dirty[n][~keep]).all(), n
+
+
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+def test_extreme_logits(decay):
+    """Open and shut gates: multipliers of exactly one and zero, input factors next to nothing."""
+    T, D = 150, 64
+    c = _case((1, T, D), decay, torch.float32)
+    c["forget"] = torch.tensor([-200.0, -100.0, -20.0, -1e-30, 0.0, 3.0, 17.0, 100.0, 200.0, float("inf"), -float("inf")])[
+        torch.randint(0, 11, (1, T, D), generator=torch.Generator().manual_seed(3))]
+    if decay:
+        c["decay"] = torch.linspace(-60.0, 12.0, D)
+        c["input_gate"] = 30.0 * c["input_gate"]
+    got = _run(c)
+    c["forget"] = c["forget"].clamp(-1e4, 1e4)
+    want = _oracle(c)
+    for n, t in got.items():
+        assert torch.isfinite(t).all(), n
+        # below 1.2e-38 values lose their bits; log a reaches the results through its root, 1.1e-19, times
+        # operands whose products stay below 1e4 here
+        _check(t, (want[n][0], want[n][1] + 2e-15), n)
+
+
+def test_differences():
+    """Gradients against central differences of the 64-bit evaluation."""
+    for decay in (False, True):
+        for reverse in (False, True):
+            offsets = [0, 4, 4, 9]
+            c = _case((9, 3), decay, torch.float32, nseq=3, spread=1.0)
+            got = _run(c, cu_seqlens=torch.tensor(offsets, dtype=torch.int32, device=DEV), reverse=reverse)
+
+            def loss(c):
+                r = _oracle(c, offsets=offsets, reverse=reverse)
+                return (r["y"][0] * c["dy"].numpy()).sum() + (r["final"][0] * c["dfinal"].numpy()).sum()
+
+            step = 1e-4
+            c = {k: v.double() for k, v in c.items()}
+            for k, n in NAMES.items():
+                if k not in c:
+                    continue
+                for at in np.ndindex(*c[k].shape):
+                    keep = c[k][at].item()
+                    c[k][at] = keep + step
+                    up = loss(c)
+                    c[k][at] = keep - step
+                    down = loss(c)
+                    c[k][at] = keep
+                    # third derivatives of this loss stay below 1e4: step^2/6 * 1e4 < 2e-5; float32 results of size < 100
+                    assert abs((up - down) / (2 * step) - got[n][at].item()) < 2e-5 + 1e-4 * abs(got[n][at].item()), (n, at)
+
+
+def test_slices_of_one_projection():
+    """Operands that are slices of a wider tensor, starting anywhere, and a gradient in another layout."""
+    for D, wide, starts in ((64, 256, (0, 64, 128)), (40, 137, (1, 45, 91)), (72, 300, (4, 80, 200)), (65, 260, (0, 65, 130))):
+        for dtype in (torch.float32, torch.bfloat16):
+            c = _case((3, 140, D), True, dtype, seed=D)
+            base = torch.full((3, 140, wide), float("nan"), dtype=dtype, device=DEV)
+            at = dict(zip(("inputs", "forget", "input_gate"), starts))
+
+            def place(k, t):
+                if k in at:
+                    v = base[..., at[k]:at[k] + D]
+                    v.copy_(t)
+                    return v.detach()
+                if k == "dy":
+                    return t.to(DEV).transpose(0, 1).contiguous().transpose(0, 1)
+                return t.to(DEV)
+
+            _compare(_run(c, place), _oracle(c))
+
+
+def test_rows_far_apart():
+    """Row offsets beyond 2^31 elements, in the operands and in the state cache."""
+    stride, D, T = (1 << 30) + 8, 64, 4
+    wide = torch.empty(stride * (T - 1) + D, dtype=torch.bfloat16, device=DEV)
+    c = _case((1, T, D), False, torch.bfloat16, states=False)
+
+    def place(k, t):
+        if k != "inputs":
+            return t.to(DEV)
+        v = wide.as_strided((1, T, D), (stride * T, stride, 1))
+        v.copy_(t)
+        return v
+
+    got = _run(c, place)
+    _compare(got, _oracle(c))
+    del got, wide
+    state = torch.empty(stride * 2 + D, dtype=torch.float32, device=DEV).as_strided((3, D), (stride, 1))
+    state.copy_(torch.ones(3, D))
+    x = torch.zeros(3, D, device=DEV)
+    y = _lb().linrec_gated_step(x, x, state)
+    assert (y == 0.5).all() and (state == 0.5).all()
+
+
+def test_states_chain_calls():
+    """A sequence scanned in pieces, state handed on, is the sequence scanned whole."""
+    lb = _lb()
+    for decay in (False, True):
+        c = {k: v.to(DEV) for k, v in _case((2, 700, 96), decay, torch.float32).items()}
+        kw = {"decay": c["decay"]} if decay else {}
+        whole, end = lb.linrec_gated(c["inputs"], c["forget"], input_gate=c.get("input_gate"), initial_state=c["initial_state"],
+                                     return_state=True, **kw)
+        h, parts = c["initial_state"], []
+        for lo, hi in ((0, 1), (1, 129), (129, 129), (129, 640), (640, 700)):
+            y, h = lb.linrec_gated(c["inputs"][:, lo:hi], c["forget"][:, lo:hi],
+                                   input_gate=c["input_gate"][:, lo:hi] if decay else None, initial_state=h, return_state=True, **kw)
+            parts.append(y)
+        # two float32 evaluations of one recurrence with multipliers below 0.9994: each within 1e-5 of the truth
+        # (bound of the oracle, checked above) at values up to 10
+        assert torch.allclose(torch.cat(parts, 1), whole, rtol=1e-4, atol=1e-4)
+        assert torch.allclose(h, end, rtol=1e-4, atol=1e-4)
+
+
+def test_same_bits_every_time():
+    c = _case((2, 1500, 200), True, torch.bfloat16)
+    one = _run(c)
+    for _ in range(3):
+        two = _run(c)
+        assert all(torch.equal(one[n], two[n]) for n in one)
+    # a few columns only: how far the look-back walks differs from run to run, the bits do not
+    c = _case((1, 20000, 64), True, torch.float32)
+    one = _run(c)
+    for _ in range(5):
+        two = _run(c)
+        assert all(torch.equal(one[n], two[n]) for n in one)
+    _lb().check_status()
+
+
+def test_many_tiles_in_flight():
+    """Few channels and many positions: every resident CTA waits in the look-back of one column."""
+    for T, D, dtype in ((20000, 64, torch.float32), (15001, 72, torch.bfloat16)):
+        for decay in (False, True):
+            c = _case((1, T, D), decay, dtype, spread=8.0)
+            _compare(_run(c), _oracle(c))
+
+
+def test_captured_and_replayed():
+    """Forward and backward in CUDA graphs captured on one stream, replayed side by side on others, on new data."""
+    lb = _lb()
+    cases = [_case((2, 900, 128), True, torch.bfloat16, seed=s) for s in (1, 2)]
+    graphs = []
+    stream = torch.cuda.Stream()
+    for c in cases:
+        dev = {k: v.to(DEV) for k, v in c.items()}
+        leaves = [dev[k].requires_grad_(True) for k in NAMES]
+        torch.cuda.synchronize()
+
+        def step():
+            y, final = lb.linrec_gated(leaves[0], leaves[1], input_gate=leaves[2], decay=leaves[3], initial_state=leaves[4], return_state=True)
+            return [y, final, *torch.autograd.grad([y, final], leaves, [dev["dy"], dev["dfinal"]])]
+
+        with torch.cuda.stream(stream):
+            step()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs = step()
+        graphs.append((graph, outs, dev, leaves))
+    fresh = [_case((2, 900, 128), True, torch.bfloat16, seed=s) for s in (3, 4)]
+    for (_, _, dev, _), c in zip(graphs, fresh):
+        for k, v in c.items():
+            dev[k].detach().copy_(v)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for (graph, _, _, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, outs, _, _), c in zip(graphs, fresh):
+        want = _oracle(c)
+        for n, t in zip(("y", "final", *NAMES.values()), outs):
+            _check(t, want[n], n)
+
+
+def test_side_streams():
+    lb = _lb()
+    c = _case((2, 600, 128), False, torch.float32)
+    want = _oracle(c)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            got.append(_run(c))
+    torch.cuda.synchronize()
+    for g in got:
+        _compare(g, want)
+
+
+def test_gradients_asked_for_in_part():
+    lb = _lb()
+    c = {k: v.to(DEV) for k, v in _case((2, 70, 64), True, torch.float32).items()}
+    full = _run({k: v.cpu() for k, v in c.items()})
+    for k, n in NAMES.items():
+        t = c[k].clone().requires_grad_(True)
+        kw = {m: c[m] for m in NAMES if m != k}
+        kw[k] = t
+        y, final = lb.linrec_gated(kw.pop("inputs"), kw.pop("forget"), return_state=True, **kw)
+        got, = torch.autograd.grad([y, final], [t], [c["dy"], c["dfinal"]])
+        assert torch.equal(got, full[n]), n
+    # gradient through the state alone
+    x = c["inputs"].clone().requires_grad_(True)
+    _, final = lb.linrec_gated(x, c["forget"], return_state=True)
+    got, = torch.autograd.grad(final, x, c["dfinal"])
+    want = go.evaluate(c["inputs"].double().cpu().numpy(), c["forget"].double().cpu().numpy(), dfinal=c["dfinal"].double().cpu().numpy())
+    _check(got, want["dx"], "dx")
+    # 16-bit parameters and states are cast, their gradients cast back
+    d, h = c["decay"].bfloat16().requires_grad_(True), c["initial_state"].bfloat16().requires_grad_(True)
+    y = lb.linrec_gated(c["inputs"], c["forget"], input_gate=c["input_gate"], decay=d, initial_state=h)
+    gd, gh = torch.autograd.grad(y, [d, h], c["dy"])
+    assert gd.dtype == gh.dtype == torch.bfloat16
+
+
+def test_no_rows():
+    lb = _lb()
+    h0 = torch.randn(2, 8, device=DEV, requires_grad=True)
+    x = torch.empty(2, 0, 8, device=DEV, requires_grad=True)
+    d = torch.randn(8, device=DEV, requires_grad=True)
+    y, h = lb.linrec_gated(x, x, input_gate=x, decay=d, initial_state=h0, return_state=True)
+    assert y.shape == (2, 0, 8) and torch.equal(h, h0)
+    gx, gd, gh = torch.autograd.grad(h, [x, d, h0], torch.ones_like(h))
+    assert gx.shape == x.shape and (gd == 0).all() and (gh == 1).all()
+    assert lb.linrec_gated(torch.empty(0, 5, 8, device=DEV), torch.empty(0, 5, 8, device=DEV)).shape == (0, 5, 8)
+    assert lb.linrec_gated_step(torch.empty(0, 8, device=DEV), torch.empty(0, 8, device=DEV), torch.empty(0, 8, device=DEV)).shape == (0, 8)
+
+
+# ---- one token ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows,D", [(1, 1), (3, 64), (7, 257), (33, 1000), (2, 2048), (130, 40)])
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_step(rows, D, decay, dtype):
+    lb = _lb()
+    c = _case((rows, 1, D), decay, dtype)
+    want = _oracle(c)
+    args = [c[k].to(DEV)[:, 0] for k in ("inputs", "forget")]
+    kw = {"input_gate": c["input_gate"].to(DEV)[:, 0], "decay": c["decay"].to(DEV)} if decay else {}
+    state = c["initial_state"].to(DEV)
+    y = lb.linrec_gated_step(*args, state, **kw)
+    _check(y, want["y"], "y")
+    _check(state, want["final"], "state")
+    # through slots of a larger, padded cache, 64-bit and 32-bit indexes, with padding rows
+    slots = torch.randperm(rows + 5, generator=torch.Generator().manual_seed(rows))[:rows]
+    for kind in (torch.int64, torch.int32):
+        cache = torch.full((rows + 5, D + 3), 7.0, device=DEV)
+        view = cache[:, 1:D + 1]
+        view[slots.to(DEV)] = c["initial_state"].to(DEV)
+        use = slots.to(kind).to(DEV).clone()
+        if rows > 2:
+            use[1], use[2] = -1, rows + 5
+        y = lb.linrec_gated_step(*args, view, slots=use, **kw)
+        live = torch.ones(rows, dtype=torch.bool)
+        if rows > 2:
+            live[1:3] = False
+            assert (y[1:3] == 0).all()
+            assert torch.equal(view[slots[1:3].to(DEV)], c["initial_state"].to(DEV)[1:3])
+        _check(y[live.to(DEV)], tuple(t[live.numpy()] for t in want["y"]), "y")
+        _check(view[slots.to(DEV)[live.to(DEV)]], tuple(t[live.numpy()] for t in want["final"]), "state")
+        untouched = torch.ones(rows + 5, dtype=torch.bool, device=DEV)
+        untouched[slots.to(DEV)] = False
+        assert (cache[untouched] == 7.0).all() and (cache[:, 0] == 7.0).all() and (cache[:, D + 1:] == 7.0).all()
+
+
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+def test_steps_are_a_scan(decay):
+    lb = _lb()
+    B, T, D = 3, 9, 200
+    c = _case((B, T, D), decay, torch.float32)
+    want = _oracle(c)
+    dev = {k: v.to(DEV) for k, v in c.items()}
+    kw = (lambda t: {"input_gate": dev["input_gate"][:, t], "decay": dev["decay"]}) if decay else (lambda t: {})
+    state = dev["initial_state"].clone()
+    ys = [lb.linrec_gated_step(dev["inputs"][:, t], dev["forget"][:, t], state, **kw(t)) for t in range(T)]
+    _check(torch.stack(ys, 1), want["y"], "y")
+    _check(state, want["final"], "state")
+    # the same tokens as rows of one call: rows that share a slot are one sequence, in row order
+    order = torch.randperm(B * T, generator=torch.Generator().manual_seed(5))
+    seq = (torch.arange(B * T) % B)[order]                     # which sequence each row belongs to
+    pos = torch.empty(B * T, dtype=torch.long)
+    for q in range(B):
+        pos[seq == q] = torch.arange(T)
+    rows = {k: dev[k][seq, pos] for k in ("inputs", "forget", "input_gate") if k in dev}
+    state = dev["initial_state"].clone()
+    kw = {"input_gate": rows["input_gate"], "decay": dev["decay"]} if decay else {}
+    y = lb.linrec_gated_step(rows["inputs"], rows["forget"], state, slots=seq.to(torch.int32).to(DEV), **kw)
+    _check(y, tuple(t[seq.numpy(), pos.numpy()] for t in want["y"]), "y")
+    _check(state, want["final"], "state")
+
+
+def test_step_replayed():
+    """A captured decode step advances its cache at every replay."""
+    lb = _lb()
+    c = _case((4, 6, 128), True, torch.bfloat16)
+    want = _oracle(c)
+    dev = {k: v.to(DEV) for k, v in c.items()}
+    x, f, i = (dev[k][:, 0].clone() for k in ("inputs", "forget", "input_gate"))
+    state = dev["initial_state"].clone()
+    keep = state.clone()
+    lb.linrec_gated_step(x, f, state, input_gate=i, decay=dev["decay"])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = lb.linrec_gated_step(x, f, state, input_gate=i, decay=dev["decay"])
+    state.copy_(keep)
+    for t in range(6):
+        for buf, k in ((x, "inputs"), (f, "forget"), (i, "input_gate")):
+            buf.copy_(dev[k][:, t])
+        graph.replay()
+        _check(y, tuple(v[:, t] for v in want["y"]), "y")
+    _check(state, want["final"], "state")
