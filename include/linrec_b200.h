@@ -336,6 +336,40 @@ LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const v
                                       const void* slots, int slots_are_64, int64_t nrows, int64_t nchan, int dtype,
                                       void* stream);
 
+/* ---- group norm on channels-last tensors, with an activation or an activated gate -------------------------
+ * x is (nsamples, positions, nchan), rows (one position of one sample) at their own stride.  A group is
+ * nchan / groups consecutive channels over all positions of a sample; mean and variance (biased) are fp32:
+ *   z = (x - mean) / sqrt(var + eps) * weight + bias;   y = act(z), or z * act(gate) where gate is given
+ * activation: 0 none, 1 v s(v), 2 s(v), with s the logistic function.  weight and bias: nchan floats, or NULL
+ * for ones and zeros.  stats: nsamples * groups pairs (mean, 1/sqrt(var + eps)), written by the forward pass
+ * if given, required by the backward pass.  Results have rows at stride nchan.  dweight and dbias may be
+ * NULL; otherwise the backward pass needs linrec_b200_group_norm_scratch_size bytes of scratch.  What follows the recurrence
+ * in a layer with heads: one position per sample, heads as groups.  No counterpart in the reference. */
+typedef struct linrec_group_norm_args {
+    const void* x;
+    const void* gate;            /* or NULL */
+    int64_t x_stride, gate_stride;
+    const float* weight;
+    const float* bias;
+    float eps;
+    int activation;
+    int dtype;
+    int64_t nsamples, positions, nchan, groups;
+    float* stats;
+    void* y;                     /* forward */
+    const void* dy;              /* backward, as are all below */
+    int64_t dy_stride;
+    void* dx;
+    void* dgate;
+    float* dweight;
+    float* dbias;
+    void* scratch;
+    size_t scratch_bytes;
+} linrec_group_norm_args;
+LINREC_API size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args);
+LINREC_API int linrec_b200_group_norm_fwd(const linrec_group_norm_args* args, void* stream);
+LINREC_API int linrec_b200_group_norm_bwd(const linrec_group_norm_args* args, void* stream);
+
 /* Number of kernels this library has launched in this process (all threads). */
 LINREC_API uint64_t linrec_b200_launch_count(void);
 

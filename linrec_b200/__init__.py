@@ -22,10 +22,11 @@ from .ops import (  # noqa: F401
 )
 
 from .general import linrec_general  # noqa: E402,F401
-from .gated import linrec_gated, linrec_gated_step  # noqa: E402,F401
+from .gated import linrec_gated, linrec_gated_norm, linrec_gated_norm_step, linrec_gated_step  # noqa: E402,F401
+from .norm import group_norm_act  # noqa: E402,F401
 
 linrec = linrec_pipe
 
 __version__ = "0.2.0"
 __all__ = ["linrec", "linrec_ref", "linrec_tile", "linrec_pipe", "linrec_general", "linrec_gated", "linrec_gated_step",
-           "check_status"]
+           "group_norm_act", "linrec_gated_norm", "linrec_gated_norm_step", "check_status"]

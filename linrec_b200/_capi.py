@@ -48,6 +48,16 @@ class GatedArgs(ctypes.Structure):
                 ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
 
 
+class GroupNormArgs(ctypes.Structure):
+    """linrec_group_norm_args of the header, field for field."""
+    _fields_ = [("x", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64),
+                ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("eps", ctypes.c_float), ("activation", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("nsamples", ctypes.c_int64), ("positions", ctypes.c_int64), ("nchan", ctypes.c_int64),
+                ("groups", ctypes.c_int64), ("stats", ctypes.c_void_p), ("y", ctypes.c_void_p), ("dy", ctypes.c_void_p),
+                ("dy_stride", ctypes.c_int64), ("dx", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("dweight", ctypes.c_void_p),
+                ("dbias", ctypes.c_void_p), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_size_t)]
+
+
 def _load() -> ctypes.CDLL:
     path = _build.LIB_PATH
     try:
@@ -113,6 +123,12 @@ def _load() -> ctypes.CDLL:
         fn.argtypes, fn.restype = [pg, po, vp, sz, vp], i32
     lib.linrec_b200_gated_step.argtypes = [vp, vp, vp, i64, i64, i64, vp, ctypes.c_float, vp, vp, i64, i64, vp, i32, i64, i64, i32, vp]
     lib.linrec_b200_gated_step.restype = i32
+    pn = ctypes.POINTER(GroupNormArgs)
+    lib.linrec_b200_group_norm_scratch_size.argtypes = [pn]
+    lib.linrec_b200_group_norm_scratch_size.restype = sz
+    for name in ("fwd", "bwd"):
+        fn = getattr(lib, "linrec_b200_group_norm_" + name)
+        fn.argtypes, fn.restype = [pn, vp], i32
     lib.linrec_b200_launch_count.argtypes = []
     lib.linrec_b200_launch_count.restype = ctypes.c_uint64
     lib.linrec_b200_last_cuda_error.argtypes = []

@@ -30,6 +30,7 @@
 // whose multiplier is the element's own, so one product P serves both directions.
 #pragma once
 #include "column_kernels.cuh"
+#include "elements.cuh"
 
 namespace linrec {
 
@@ -66,35 +67,6 @@ struct GatedParams {
 };
 
 // ---- gates ------------------------------------------------------------------------------------------
-// 1/d for d in [1, 2]: the hardware approximation and one Newton step.
-__device__ __forceinline__ float gated_rcp(float d)
-{
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    return fmaf(r, fmaf(-d, r, 1.0f), r);
-}
-__device__ __forceinline__ float gated_sqrt(float v)
-{
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-// s(v) and s(-v), both to full relative accuracy.
-__device__ __forceinline__ void logistic_pair(float v, float& p, float& n)
-{
-    const float e = expf(-fabsf(v));
-    const float r = gated_rcp(1.0f + e), s = e * r;
-    p = v >= 0.0f ? r : s;
-    n = v >= 0.0f ? s : r;
-}
-__device__ __forceinline__ float logistic(float v)
-{
-    float p, n;
-    logistic_pair(v, p, n);
-    return p;
-}
-__device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
-
 // sqrt(1 - exp(2 la)) for la <= 0: the Taylor series of 1 - exp(-z) where the difference would cancel.
 __device__ __forceinline__ float decay_input_factor(float la, float a)
 {
@@ -105,7 +77,7 @@ __device__ __forceinline__ float decay_input_factor(float la, float a)
     s = fmaf(z * s, -1.0f / 4.0f, 1.0f);
     s = fmaf(z * s, -1.0f / 3.0f, 1.0f);
     s = fmaf(z * s, -1.0f / 2.0f, 1.0f);
-    return gated_sqrt(z < 0.25f ? z * s : fmaf(-a, a, 1.0f));
+    return approx_sqrt(z < 0.25f ? z * s : fmaf(-a, a, 1.0f));
 }
 
 // ---- the pair operator with cuts ------------------------------------------------------------------------
@@ -175,53 +147,6 @@ __device__ __forceinline__ GatedRun gated_run(const GatedParams& p, int b, long 
     r.cut = r.start | ~r.valid;
     r.seq = q;
     return r;
-}
-
-// ---- loads and stores of a lane's two channels ----------------------------------------------------------
-template <typename ST>
-__device__ __forceinline__ float to_f32(ST v)
-{
-    return (float)v;
-}
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v)
-{
-    return __bfloat162float(v);
-}
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half v)
-{
-    return __half2float(v);
-}
-template <typename ST>
-__device__ __forceinline__ ST from_f32(float v)
-{
-    return (ST)v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v)
-{
-    return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v)
-{
-    return __float2half_rn(v);
-}
-
-template <typename ST>
-__device__ __forceinline__ void load_two(const void* base, long long offset, int have, float* v)
-{
-    const ST* q = static_cast<const ST*>(base) + offset;
-    v[0] = have > 0 ? to_f32<ST>(q[0]) : 0.0f;
-    v[1] = have > 1 ? to_f32<ST>(q[1]) : 0.0f;
-}
-template <typename ST>
-__device__ __forceinline__ void store_two(void* base, long long offset, int have, const float* v)
-{
-    ST* q = static_cast<ST*>(base) + offset;
-    if (have > 0) q[0] = from_f32<ST>(v[0]);
-    if (have > 1) q[1] = from_f32<ST>(v[1]);
 }
 
 // ---- linking a tile to its predecessor -----------------------------------------------------------------
@@ -626,7 +551,7 @@ __global__ void __launch_bounds__(kGatedThreads) gated_bwd_kernel(const GatedPar
 
 // Gradient of the decay parameter from the tiles' sums, in a fixed order: d L = s(L)/softplus(L) * sum.
 // One warp-wide column of 32 channels per CTA, eight warps along the tiles.
-__global__ void __launch_bounds__(256) gated_decay_grad_kernel(const float* part, long long tiles, int D, const float* decay, float* out)
+static __global__ void __launch_bounds__(256) gated_decay_grad_kernel(const float* part, long long tiles, int D, const float* decay, float* out)
 {
     __shared__ double sums[8][32];
     const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;

@@ -9,6 +9,8 @@ carried in and out in float32, a backward pass, and a form for single tokens on 
     y = linrec_gated(inputs, forget, cu_seqlens=offsets)                 # (rows, D), sequences end to end
     y = linrec_gated_step(inputs, forget, state, slots=slots)            # one token each, state in place
 
+    y = linrec_gated_norm(inputs, forget, gate, groups, weight, bias)    # recurrence, norm per head, gate
+
 (s is the logistic function.)  `linrec_general(x, c, dim=1)` scans the same layout with finished
 coefficients in the storage type; rounded to 16 bits a multiplier near one is off by more than its distance
 from one, and it takes no states and no packed sequences, which is what these operators are for.  The
@@ -24,26 +26,13 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .ops import _DTYPES, _on_device, _row_layout, _workspace
+from .norm import _as_rows, _check_cuda, _fail, _ptr, _STORAGE, group_norm_act
+from .ops import _DTYPES, _on_device, _workspace
 
-__all__ = ["linrec_gated", "linrec_gated_step"]
-
-_STORAGE = (torch.float32, torch.bfloat16, torch.float16)
+__all__ = ["linrec_gated", "linrec_gated_step", "linrec_gated_norm", "linrec_gated_norm_step"]
 
 
 # ---- arguments ---------------------------------------------------------------------------------------
-def _fail(what: str):
-    raise RuntimeError(f"linrec: {what}")
-
-
-def _check_cuda(*ts) -> None:
-    ts = [t for t in ts if t is not None]
-    if not all(t.is_cuda for t in ts):
-        _fail("tensors must be CUDA tensors (there is no CPU implementation)")
-    if any(t.device != ts[0].device for t in ts[1:]):
-        _fail("tensors must be on the same device")
-
-
 def _check_operands(inputs, forget, input_gate, decay, decay_scale) -> None:
     """What the scan and the step have in common."""
     if inputs.dtype not in _STORAGE:
@@ -73,27 +62,12 @@ def _check_index(name: str, t) -> None:
         _fail(f"{name} must have one dimension")
 
 
-def _as_rows(t: torch.Tensor):
-    """(`t` or a dense copy, elements between consecutive rows): the kernels take rows at one stride."""
-    if t.numel() == 0:
-        return t, t.size(-1)
-    layout = _row_layout(t) if t.size(-1) == 1 or t.stride(-1) == 1 else None
-    if layout is None:
-        t = t.contiguous()
-        return t, t.size(-1)
-    return t, layout[2]
-
-
 def _scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """The stream's workspace.  Inside a graph capture a fresh one that belongs to the graph: graphs that
     were captured on one stream may be replayed side by side on others."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return _workspace(device, stream, nbytes)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 # ---- the scan ----------------------------------------------------------------------------------------
@@ -290,3 +264,29 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
     _capi.raise_for(rc, "linrec_b200_gated_step")
     torch.autograd.graph.increment_version(state)
     return y
+
+
+# ---- with the norm behind it ---------------------------------------------------------------------------
+def linrec_gated_norm(inputs: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | None, groups: int,
+                      weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *, activation: str | None = "silu",
+                      eps: float = 1e-5, return_state: bool = False, **recurrence):
+    """The mixing of a gated recurrence layer with heads: `linrec_gated(inputs, forget, **recurrence)`, then
+    every position normalised head by head (`groups` heads of adjacent channels) and multiplied with the
+    activated gate, `group_norm_act(h, groups, weight, bias, gate=gate)`.  Differentiable once."""
+    r = linrec_gated(inputs, forget, return_state=return_state, **recurrence)
+    h, state = r if return_state else (r, None)
+    D = h.size(-1)
+    if gate is not None and gate.shape != inputs.shape:
+        _fail("gate must have the sizes of the inputs")
+    y = group_norm_act(h.reshape(-1, D) if D else h, groups, weight, bias, gate=None if gate is None else gate.reshape(-1, D) if D else gate,
+                       activation=activation, eps=eps).reshape(inputs.shape)
+    return (y, state) if return_state else y
+
+
+def linrec_gated_norm_step(inputs: torch.Tensor, forget: torch.Tensor, gate: torch.Tensor | None, state: torch.Tensor, groups: int,
+                           weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                           activation: str | None = "silu", eps: float = 1e-5, **recurrence) -> torch.Tensor:
+    """`linrec_gated_norm` for one token per row: `linrec_gated_step`, then the norm and the gate.  A padding
+    row's norm is that of zeros, act of the bias times the gate."""
+    h = linrec_gated_step(inputs, forget, state, **recurrence)
+    return group_norm_act(h, groups, weight, bias, gate=gate, activation=activation, eps=eps)

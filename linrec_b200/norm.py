@@ -1,0 +1,144 @@
+"""Group norm of channels-last tensors with an activation or an activated gate: what stands behind the gated
+recurrence in a layer with heads (`linrec_gated_norm`), where every position is a sample of its own and the
+heads are the groups, and the usual group norm of (samples, positions, channels) tensors.
+
+    y = group_norm_act(x, groups, weight, bias)                # act(norm(x) * weight + bias)
+    y = group_norm_act(x, groups, weight, bias, gate=g)        # (norm(x) * weight + bias) * act(g)
+
+Storage types float32, bfloat16 and float16; statistics, parameters and their gradients are float32.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+from .ops import _DTYPES, _on_device, _row_layout
+
+__all__ = ["group_norm_act"]
+
+_STORAGE = (torch.float32, torch.bfloat16, torch.float16)
+_ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
+
+
+def _fail(what: str):
+    raise RuntimeError(f"linrec: {what}")
+
+
+def _check_cuda(*ts) -> None:
+    ts = [t for t in ts if t is not None]
+    if not all(t.is_cuda for t in ts):
+        _fail("tensors must be CUDA tensors (there is no CPU implementation)")
+    if any(t.device != ts[0].device for t in ts[1:]):
+        _fail("tensors must be on the same device")
+
+
+def _as_rows(t: torch.Tensor):
+    """(`t` or a dense copy, elements between consecutive rows): the kernels take rows at one stride."""
+    if t.numel() == 0:
+        return t, t.size(-1)
+    layout = _row_layout(t) if t.size(-1) == 1 or t.stride(-1) == 1 else None
+    if layout is None:
+        t = t.contiguous()
+        return t, t.size(-1)
+    return t, layout[2]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _describe(x, gate, weight, bias, groups, act, eps, stats):
+    a = _capi.GroupNormArgs()
+    C = x.size(-1)
+    xr, a.x_stride = _as_rows(x)
+    gr = None
+    if gate is not None:
+        gr, a.gate_stride = _as_rows(gate)
+    a.x, a.gate, a.weight, a.bias, a.stats = xr.data_ptr(), _ptr(gr), _ptr(weight), _ptr(bias), _ptr(stats)
+    a.eps, a.activation, a.dtype = eps, act, _DTYPES[x.dtype]
+    a.nsamples, a.nchan, a.groups = x.size(0), C, groups
+    a.positions = x.numel() // (x.size(0) * C) if x.numel() else 0
+    return a, (xr, gr)
+
+
+def _call(entry, name, device, a) -> None:
+    with _on_device(device):
+        _capi.raise_for(entry(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream), name)
+
+
+def _forward(x, gate, weight, bias, groups, act, eps, want_stats):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(x.size(0) * groups * 2, dtype=torch.float32, device=x.device) if want_stats else None
+    if y.numel():
+        a, keep = _describe(x, gate, weight, bias, groups, act, eps, stats)
+        a.y = y.data_ptr()
+        _call(_capi.lib.linrec_b200_group_norm_fwd, "linrec_b200_group_norm_fwd", x.device, a)
+    return y, stats
+
+
+class _GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, weight, bias, groups, act, eps):
+        y, stats = _forward(x, gate, weight, bias, groups, act, eps, True)
+        ctx.save_for_backward(x, gate, weight, bias, stats)
+        ctx.args = (groups, act, eps)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, gate, weight, bias, stats = ctx.saved_tensors
+        dev = x.device
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dgate = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        make = torch.empty_like if x.numel() else torch.zeros_like
+        dw = make(weight) if weight is not None and ctx.needs_input_grad[2] else None
+        db = make(bias) if bias is not None and ctx.needs_input_grad[3] else None
+        if x.numel():
+            a, keep = _describe(x, gate, weight, bias, *ctx.args, stats)
+            dy, a.dy_stride = _as_rows(dy)
+            a.dy, a.dx, a.dgate, a.dweight, a.dbias = dy.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw), _ptr(db)
+            scratch = None
+            if dw is not None or db is not None:
+                scratch = torch.empty(_capi.lib.linrec_b200_group_norm_scratch_size(ctypes.byref(a)), dtype=torch.uint8, device=dev)
+                a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel()
+            _call(_capi.lib.linrec_b200_group_norm_bwd, "linrec_b200_group_norm_bwd", dev, a)
+        return dx, dgate, dw, db, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                   gate: torch.Tensor | None = None, activation: str | None = "silu", eps: float = 1e-5) -> torch.Tensor:
+    """Group norm of `x`, (samples, ..., channels): mean and (biased) variance over the dimensions between and
+    the channels of a group, `groups` groups of adjacent channels; then weight and bias per channel; then
+    the activation of the result, or the product with the activated gate where one is given.
+
+    For statistics of every position by itself give x as (positions, channels).
+    activation   "silu", "sigmoid" or None
+    weight, bias (channels,), ones and zeros by default; gate has the sizes and dtype of x
+
+    Differentiable once with respect to x, gate, weight and bias."""
+    if x.dim() < 2:
+        _fail("x needs a sample and a channel dimension")
+    if x.dtype not in _STORAGE:
+        _fail(f"dtype {x.dtype} is not supported (float32, bfloat16, float16)")
+    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or x.size(-1) % groups:
+        _fail("groups must divide the channels")
+    if activation not in _ACTIVATIONS:
+        _fail(f"activation {activation!r} is not one of {list(_ACTIVATIONS)}")
+    if not 0.0 < float(eps) < float("inf"):
+        _fail("eps must be positive and finite")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != x.shape[-1:] or not t.is_floating_point()):
+            _fail(f"{name} must have one floating-point value per channel")
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        _fail("gate must have the sizes and the dtype of x")
+    _check_cuda(x, gate, weight, bias)
+    weight = None if weight is None else weight.float().contiguous()
+    bias = None if bias is None else bias.float().contiguous()
+    args = (x, gate, weight, bias, groups, _ACTIVATIONS[activation], float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return _GroupNormFn.apply(*args)
+    return _forward(*args, False)[0]
