@@ -4,35 +4,55 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stdint.h>
 
 namespace linrec {
 
 // ---- logistic function ---------------------------------------------------------------------------------
-// 1/d for d in [1, 2]: the hardware approximation and one Newton step.
-__device__ __forceinline__ float newton_rcp(float d)
+__device__ __forceinline__ float approx_rcp(float d)
 {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    return fmaf(r, fmaf(-d, r, 1.0f), r);
+    return r;
 }
 __device__ __forceinline__ float approx_sqrt(float v)
 {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-// s(v) and s(-v), both to full relative accuracy.
+// exp(v) as a power of two.  The product v log2(e) is rounded, so the relative error is (4 + 1.3 |v|) 2^-24:
+// far below half a step of a 16-bit result, not good enough for 32-bit storage.
+__device__ __forceinline__ float fast_exp(float v)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.44269504f));
+    return r;
+}
+template <bool FAST>
+__device__ __forceinline__ float exp_of(float v)
+{
+    return FAST ? fast_exp(v) : expf(v);
+}
+// s(v) and s(-v) to full relative accuracy: the smaller one as a quotient, the larger as its distance from one
+// (a value next to one is then off by half its last place, whatever the reciprocal's error is).
+template <bool FAST>
 __device__ __forceinline__ void logistic_pair(float v, float& p, float& n)
 {
-    const float e = expf(-fabsf(v));
-    const float r = newton_rcp(1.0f + e), s = e * r;
-    p = v >= 0.0f ? r : s;
-    n = v >= 0.0f ? s : r;
+    const float e = exp_of<FAST>(-fabsf(v)), d = 1.0f + e;
+    float r = approx_rcp(d);
+    if (!FAST) r = fmaf(r, fmaf(-d, r, 1.0f), r);
+    const float s = e * r, l = 1.0f - s;
+    p = v >= 0.0f ? l : s;
+    n = v >= 0.0f ? s : l;
 }
+// s(v) alone; a value next to one may be off by two of its last places.
+template <bool FAST>
 __device__ __forceinline__ float logistic(float v)
 {
+    if (FAST) return approx_rcp(1.0f + fast_exp(-v));
     float p, n;
-    logistic_pair(v, p, n);
+    logistic_pair<false>(v, p, n);
     return p;
 }
 __device__ __forceinline__ float softplus(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
@@ -82,6 +102,51 @@ __device__ __forceinline__ void store_two(void* base, long long offset, int have
     ST* q = static_cast<ST*>(base) + offset;
     if (have > 0) q[0] = from_f32<ST>(v[0]);
     if (have > 1) q[1] = from_f32<ST>(v[1]);
+}
+
+// Two adjacent channels as one word of shared or global memory.
+template <typename ST>
+struct Two;
+template <>
+struct Two<float> {
+    using Word = float2;
+    __device__ static __forceinline__ void unpack(Word w, float* v) { v[0] = w.x, v[1] = w.y; }
+    __device__ static __forceinline__ Word pack(const float* v) { return make_float2(v[0], v[1]); }
+};
+template <>
+struct Two<__nv_bfloat16> {
+    using Word = uint32_t;
+    __device__ static __forceinline__ void unpack(Word w, float* v)
+    {
+        v[0] = __uint_as_float(w << 16);
+        v[1] = __uint_as_float(w & 0xffff0000u);
+    }
+    __device__ static __forceinline__ Word pack(const float* v)
+    {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+template <>
+struct Two<__half> {
+    using Word = uint32_t;
+    __device__ static __forceinline__ void unpack(Word w, float* v)
+    {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        v[0] = f.x, v[1] = f.y;
+    }
+    __device__ static __forceinline__ Word pack(const float* v)
+    {
+        const __half2 h = __floats2half2_rn(v[0], v[1]);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+};
+// `pair`: the two channels exist and lie at an address a whole word can be written to.
+template <typename ST>
+__device__ __forceinline__ void store_two(void* base, long long offset, int have, const float* v, bool pair)
+{
+    if (pair) *reinterpret_cast<typename Two<ST>::Word*>(static_cast<ST*>(base) + offset) = Two<ST>::pack(v);
+    else store_two<ST>(base, offset, have, v);
 }
 
 }  // namespace linrec

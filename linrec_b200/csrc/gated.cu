@@ -1,8 +1,9 @@
 // Host side of the gated recurrence (include/linrec_b200.h): argument checks, how the sequences are laid
 // on scan axes, launches.
-#include "gated_kernels.cuh"
+#include "gated_variants.h"
 #include "host.h"
 
+#include <cstdio>
 #include <cstring>
 
 namespace {
@@ -46,8 +47,6 @@ int check(const linrec_gated_args* a)
     return LINREC_OK;
 }
 
-int run_length(int dtype, bool bwd) { return bwd || dtype == LINREC_DTYPE_F32 ? 64 : 128; }
-
 int parse(const linrec_opts* o, int& wait_ms)
 {
     wait_ms = 2000;
@@ -61,12 +60,34 @@ int parse(const linrec_opts* o, int& wait_ms)
     return LINREC_OK;
 }
 
-using Fn = void (*)(const GatedParams);
-template <typename ST>
-Fn pick(bool bwd, bool decay)
+bool on_boundary(const void* p, int64_t stride, int size, int bytes)
 {
-    if (bwd) return decay ? linrec::gated_bwd_kernel<ST, true> : linrec::gated_bwd_kernel<ST, false>;
-    return decay ? linrec::gated_fwd_kernel<ST, true> : linrec::gated_fwd_kernel<ST, false>;
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0;
+}
+
+// Rank-3 view (channels, positions, axes) of rows at `stride`, no swizzle; box = one tile.  Positions outside
+// an axis and channels outside the rows read as zero.
+int make_map(CUtensorMap* map, const void* ptr, int64_t stride, const GatedParams& p, int rows, int dtype)
+{
+    linrec_host::EncodeTiledFn enc = linrec_host::encode_tiled_fn();
+    if (!enc) {
+        linrec_host::note_cuda_error("cudaGetDriverEntryPoint", "cuTensorMapEncodeTiled not found");
+        return LINREC_ERR_CUDA;
+    }
+    const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
+    const cuuint64_t dims[3] = {(cuuint64_t)p.D, (cuuint64_t)p.nrows, (cuuint64_t)p.nb};
+    const cuuint64_t strides[2] = {(cuuint64_t)(stride * size), (cuuint64_t)(stride * size * p.nrows)};
+    const cuuint32_t box[3] = {(cuuint32_t)kGatedChannels, (cuuint32_t)rows, 1u};
+    const cuuint32_t ones[3] = {1, 1, 1};
+    const CUresult r = enc(map, dtype == LINREC_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                           : dtype == LINREC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           3, const_cast<void*>(ptr), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return LINREC_OK;
+    char msg[64];
+    snprintf(msg, sizeof(msg), "driver error %d", (int)r);
+    linrec_host::note_cuda_error("cuTensorMapEncodeTiled", msg);
+    return LINREC_ERR_CUDA;
 }
 
 int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream_)
@@ -111,22 +132,45 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
     p.cu = a.cu_seqlens; p.cu64 = a.cu_is_64; p.nseq = (int)a.nseq; p.seqlen = a.seqlen;
     p.nrows = ax.nrows; p.nb = ax.nb;
     p.D = (int)a.nchan; p.dtiles = linrec_host::ceil_div_i(a.nchan, kGatedChannels); p.units = p.dtiles * p.nb;
-    p.nk = linrec_host::ceil_div_i(ax.nrows, run_length(a.dtype, bwd));
     p.nck = linrec_host::ceil_div_i(ax.nrows, kGatedCheckpoint);
-    p.ntickets = (long long)p.nk * p.units;
     p.reverse = a.reverse != 0;
     p.header = static_cast<uint32_t*>(workspace);
     p.desc = reinterpret_cast<linrec::TileDesc*>(static_cast<char*>(workspace) + linrec::kHeaderBytes);
     p.wait_budget = (long long)wait_ms * (long long)dev.clock_khz;
 
-    const Fn fn = a.dtype == LINREC_DTYPE_F32 ? pick<float>(bwd, decay)
-                : a.dtype == LINREC_DTYPE_BF16 ? pick<__nv_bfloat16>(bwd, decay) : pick<__half>(bwd, decay);
+    const int size = a.dtype == LINREC_DTYPE_F32 ? 4 : 2;
+    const void* in[4] = {a.x, a.forget, decay ? a.input_gate : a.x, bwd ? a.dy : a.x};
+    const int64_t stride[4] = {a.x_stride, a.forget_stride, decay ? a.input_gate_stride : a.x_stride, bwd ? a.dy_stride : a.x_stride};
+    const void* out[4] = {bwd ? a.dx : a.y, bwd ? a.dforget : a.y, bwd && decay ? a.dinput_gate : a.y, a.y};
+    p.pair = 1;
+    for (int i = 0; i < (bwd ? (decay ? 3 : 2) : 1); ++i) p.pair &= on_boundary(out[i], a.nchan, size, 2 * size);
+    int load = linrec::kLoadTma;
+    for (int i = 0; i < 4; ++i) {
+        if (!on_boundary(in[i], stride[i], size, 4)) load = linrec::kLoadAny;
+        else if (load == linrec::kLoadTma &&
+                 (!on_boundary(in[i], stride[i], size, 16) || !p.pair || (double)stride[i] * size * (double)ax.nrows >= 1e12))
+            load = linrec::kLoadWord;
+    }
+    const linrec_variants::GatedKernel kernel = a.dtype == LINREC_DTYPE_F32 ? linrec_variants::gated_kernel_f32(bwd, decay, load)
+                                              : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::gated_kernel_bf16(bwd, decay, load)
+                                                                             : linrec_variants::gated_kernel_f16(bwd, decay, load);
+    p.nk = linrec_host::ceil_div_i(ax.nrows, kernel.rows);
+    p.ntickets = (long long)p.nk * p.units;
+    linrec::GatedMaps maps{};
+    if (load == linrec::kLoadTma) {
+        CUtensorMap* to[4] = {&maps.x, &maps.f, &maps.i, &maps.dy};
+        for (int i = 0; i < 4; ++i) {
+            if ((i == 2 && !decay) || (i == 3 && !bwd)) continue;
+            rc = make_map(to[i], in[i], stride[i], p, kernel.rows, a.dtype);
+            if (rc != LINREC_OK) return rc;
+        }
+    }
     int occ = 0;
-    rc = linrec_host::occupancy(reinterpret_cast<const void*>(fn), kGatedThreads, 0, occ);
+    rc = linrec_host::occupancy(reinterpret_cast<const void*>(kernel.fn), kGatedThreads, (size_t)kernel.smem, occ);
     if (rc != LINREC_OK) return rc;
     long long grid = (long long)dev.sm_count * occ;
     if (grid > p.ntickets) grid = p.ntickets;
-    rc = linrec_host::launch("gated recurrence", fn, dim3((unsigned)grid), kGatedThreads, 0, stream, p);
+    rc = linrec_host::launch("gated recurrence", kernel.fn, dim3((unsigned)grid), kGatedThreads, (size_t)kernel.smem, stream, p, maps);
     if (rc != LINREC_OK || !bwd || !decay) return rc;
     return linrec_host::launch("decay gradient", linrec::gated_decay_grad_kernel, dim3((unsigned)linrec_host::ceil_div_i(a.nchan, 32)), 256, 0,
                                stream, (const float*)p.dlam, (long long)p.nk * p.nb, p.D, p.decay, a.ddecay);

@@ -32,6 +32,8 @@
 #include "column_kernels.cuh"
 #include "elements.cuh"
 
+#include <type_traits>
+
 namespace linrec {
 
 constexpr int kGatedWarps = 8;
@@ -64,20 +66,27 @@ struct GatedParams {
     uint32_t* header;
     TileDesc* desc;                     // [nk][units][64]
     long long wait_budget;
+    int pair;                           // results may be written two channels at a time
 };
 
 // ---- gates ------------------------------------------------------------------------------------------
-// sqrt(1 - exp(2 la)) for la <= 0: the Taylor series of 1 - exp(-z) where the difference would cancel.
-__device__ __forceinline__ float decay_input_factor(float la, float a)
+// a = exp(-y) and b^2 = 1 - a^2 = (1 - a)(1 + a) from y = -log a >= 0.  Below 1/4 the distance 1 - a comes from
+// its Taylor series (truncated at y^6/7! = 5e-8 relative) and a from it: an error of the multiplier is
+// kept for 1/(1 - a) positions, so next to one it has to be right to half its last place.  SMALL: y is known to be below 1/4.
+template <bool FAST, bool SMALL>
+__device__ __forceinline__ void decay_factors(float y, float& a, float& b2)
 {
-    const float z = -2.0f * la;
-    float s = fmaf(z, -1.0f / 7.0f, 1.0f);
-    s = fmaf(z * s, -1.0f / 6.0f, 1.0f);
-    s = fmaf(z * s, -1.0f / 5.0f, 1.0f);
-    s = fmaf(z * s, -1.0f / 4.0f, 1.0f);
-    s = fmaf(z * s, -1.0f / 3.0f, 1.0f);
-    s = fmaf(z * s, -1.0f / 2.0f, 1.0f);
-    return approx_sqrt(z < 0.25f ? z * s : fmaf(-a, a, 1.0f));
+    float s = fmaf(y, -1.0f / 720.0f, 1.0f / 120.0f);
+    s = fmaf(y, s, -1.0f / 24.0f);
+    s = fmaf(y, s, 1.0f / 6.0f);
+    s = fmaf(y, s, -0.5f);
+    float d = y * fmaf(y, s, 1.0f);
+    a = 1.0f - d;
+    if (!SMALL && !(y < 0.25f)) {
+        a = exp_of<FAST>(-y);
+        d = 1.0f - a;
+    }
+    b2 = d * (1.0f + a);
 }
 
 // ---- the pair operator with cuts ------------------------------------------------------------------------
@@ -236,81 +245,299 @@ __device__ __forceinline__ float gated_link(const GatedParams& p, TileDesc* d, u
     return in;
 }
 
-// ---- forward ------------------------------------------------------------------------------------------
-template <typename ST>
+// ---- the tile ---------------------------------------------------------------------------------------------
+// How operands reach shared memory, where every thread finds the words of its own two channels and K
+// positions:
+//   kLoadTma    one bulk-tensor copy per operand through a ring of stages, issued by the last warp as soon as a
+//               barrier of the tile shows a stage free (rows on 16-byte boundaries); a ninth warp for the
+//               copies would cost every thread a quarter of its registers
+//   kLoadWord   4-byte asynchronous copies, every thread its own words, one tile ahead (4-byte boundaries)
+//   kLoadAny    plain loads by the thread, stored to the same place (any alignment)
+constexpr int kLoadTma = 0, kLoadWord = 1, kLoadAny = 2;
+
+template <typename ST, bool DECAY, bool BWD>
 struct GatedTile {
-    static constexpr int kRunFwd = sizeof(ST) == 4 ? 8 : 16;      // positions per thread
-    static constexpr int kRunBwd = 8;
-    static constexpr int kRowsFwd = kRunFwd * kGatedWarps;
-    static constexpr int kRowsBwd = kRunBwd * kGatedWarps;
+    static constexpr bool kFast = sizeof(ST) == 2;                     // 16-bit results: fast exponentials will do
+    static constexpr int K = BWD || sizeof(ST) == 4 ? 8 : 16;          // positions per thread
+    static constexpr int R = K * kGatedWarps;                          // positions per tile
+    static constexpr int kArrays = (DECAY ? 3 : 2) + (BWD ? 1 : 0);    // x, f(, i)(, dy)
+    static constexpr int kArrayBytes = R * kGatedChannels * (int)sizeof(ST);
+    static constexpr int kStageBytes = kArrays * kArrayBytes;
+    // forward: a stage is free once the gates are in registers; backward: only when the next tile has begun
+    static constexpr int kStages = BWD && sizeof(ST) == 2 ? 3 : 2;
+    static constexpr int kDynSmem = kStages * kStageBytes + 128;
+    using Word = typename Two<ST>::Word;
 };
 
-template <typename ST, bool DECAY>
-__global__ void __launch_bounds__(kGatedThreads) gated_fwd_kernel(const GatedParams p)
+struct GatedMaps {
+    CUtensorMap x, f, i, dy;
+};
+
+struct GatedWhere {
+    int k;            // tile along the axis, in forward scan order
+    int g;            // the same in the order of this pass
+    int b, dt;        // axis, channel block
+};
+template <bool BWD>
+__device__ __forceinline__ GatedWhere gated_where(const GatedParams& p, uint32_t ticket)
 {
-    constexpr int K = GatedTile<ST>::kRunFwd, R = GatedTile<ST>::kRowsFwd;
-    __shared__ float4 runs[2][kGatedWarps][32];      // (Y, P) of both channels of every thread
-    __shared__ float entering[kGatedChannels];
-    __shared__ uint32_t next_ticket;
+    GatedWhere w;
+    w.g = (int)(ticket / (uint32_t)p.units);
+    const int unit = (int)(ticket - (uint32_t)w.g * (uint32_t)p.units);
+    w.b = unit / p.dtiles;
+    w.dt = unit - w.b * p.dtiles;
+    w.k = BWD ? p.nk - 1 - w.g : w.g;
+    return w;
+}
 
-    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    ptx::grid_dependency_wait();
-    const uint32_t epoch = read_epoch(p.header);
+// A thread's own words of one tile, by asynchronous 4-byte copies or plain loads.
+template <typename ST, bool DECAY, bool BWD, int LOAD>
+__device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhere& w, typename Two<ST>::Word* stage, int warp, int lane)
+{
+    using T = GatedTile<ST, DECAY, BWD>;
+    const void* src[4] = {p.x, p.f, DECAY ? p.ig : p.dy, p.dy};
+    const long long stride[4] = {p.sx, p.sf, DECAY ? p.si : p.sdy, p.sdy};
+    const int ch = w.dt * kGatedChannels + 2 * lane, have = p.D - ch;
+    const long long s0 = (long long)w.k * T::R + warp * T::K;
+    const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
+    const int step = p.reverse ? -1 : 1;
+#pragma unroll
+    for (int a = 0; a < T::kArrays; ++a) {
+        const ST* from = static_cast<const ST*>(src[a]) + ch;
+#pragma unroll
+        for (int j = 0; j < T::K; ++j) {
+            const int sl = warp * T::K + j, r = p.reverse ? T::R - 1 - sl : sl;
+            typename Two<ST>::Word* to = stage + (a * T::R + r) * 32 + lane;
+            const ST* at = from + (row0 + (long long)j * step) * stride[a];
+            const bool in = s0 + j < p.nrows;
+            if (LOAD == kLoadWord) {
+                if (sizeof(ST) == 4) {
+                    if (in && have > 0) ptx::cp_async_4(to, at);
+                    if (in && have > 1) ptx::cp_async_4(reinterpret_cast<char*>(to) + 4, at + 1);
+                } else if (in && have > 1) {
+                    ptx::cp_async_4(to, at);
+                } else if (in && have > 0) {   // the last channel of an odd number
+                    float v[2];
+                    load_two<ST>(at, 0, have, v);
+                    *to = Two<ST>::pack(v);
+                }
+            } else {
+                float v[2] = {0.0f, 0.0f};
+                if (in) load_two<ST>(at, 0, have, v);
+                *to = Two<ST>::pack(v);
+            }
+        }
+    }
+}
 
-    for (int it = 0;; ++it) {
-        if (tid == 0) next_ticket = atomicAdd(p.header, 1u);
-        __syncthreads();
-        const uint32_t ticket = next_ticket;
-        if ((long long)ticket >= p.ntickets) break;
-        const int k = (int)(ticket / (uint32_t)p.units);
-        const int unit = (int)(ticket - (uint32_t)k * (uint32_t)p.units);
-        const int b = unit / p.dtiles, dt = unit - b * p.dtiles;
-        const int ch = dt * kGatedChannels + 2 * lane;
-        const int have = p.D - ch;
-        const long long s0 = (long long)k * R + warp * K;
-        const GatedRun run = gated_run<K>(p, b, s0, lane);
-        TileDesc* desc = p.desc + ((long long)ticket * kGatedChannels + tid);
-        uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && k > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
-        const long long row0 = (long long)b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
-        const int step = p.reverse ? -1 : 1;
+// The last warp's side of the ring: tickets (drawn one ahead, so that the counter's latency is hidden), copies,
+// and the block's decay parameters, which the other warps find beside the operands.
+template <typename ST, bool DECAY, bool BWD>
+struct GatedRing {
+    using T = GatedTile<ST, DECAY, BWD>;
+    const GatedParams& p;
+    const GatedMaps& maps;
+    char* stages;
+    uint64_t* full;
+    uint32_t* tickets;
+    float (*rates)[kGatedChannels];
+    int lane;
+    uint32_t ahead, issued;
+    bool drained;
 
-        float nsp[2] = {0.0f, 0.0f};
+    __device__ __forceinline__ void draw()
+    {
+        if (lane == 0) ahead = atomicAdd(p.header, 1u);
+    }
+    __device__ __forceinline__ void refill()
+    {
+        if (drained) return;
+        const int s = (int)(issued % T::kStages);
+        const uint32_t ticket = __shfl_sync(0xffffffffu, ahead, 0);
+        if ((long long)ticket >= p.ntickets) {
+            drained = true;
+            if (lane == 0) {
+                tickets[s] = 0xffffffffu;
+                ptx::mbar_arrive(&full[s]);
+            }
+            return;
+        }
+        ++issued;
+        const GatedWhere w = gated_where<BWD>(p, ticket);
+        if (lane == 0) {
+            // (operands first: the barrier completes when the arrival below has come as well)
+            tickets[s] = ticket;
+            const int row = p.reverse ? (int)(p.nrows - (long long)(w.k + 1) * T::R) : w.k * T::R;
+            char* to = stages + s * T::kStageBytes;
+            if (DECAY) ptx::mbar_expect_tx(&full[s], (uint32_t)T::kStageBytes);
+            else ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
+            ptx::tma_load_3d(to, &maps.x, &full[s], w.dt * kGatedChannels, row, w.b);
+            ptx::tma_load_3d(to + T::kArrayBytes, &maps.f, &full[s], w.dt * kGatedChannels, row, w.b);
+            if (DECAY) ptx::tma_load_3d(to + 2 * T::kArrayBytes, &maps.i, &full[s], w.dt * kGatedChannels, row, w.b);
+            if (BWD) ptx::tma_load_3d(to + (T::kArrays - 1) * T::kArrayBytes, &maps.dy, &full[s], w.dt * kGatedChannels, row, w.b);
+        }
+        draw();
         if (DECAY) {
 #pragma unroll
-            for (int v = 0; v < 2; ++v)
-                if (v < have) nsp[v] = -p.scale * softplus(p.decay[ch + v]);
-        }
-        float a[K][2], u[K][2];
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            float xv[2] = {0.0f, 0.0f}, fv[2] = {0.0f, 0.0f}, iv[2] = {0.0f, 0.0f};
-            if (run.valid >> j & 1u) {
-                const long long row = row0 + (long long)j * step;
-                load_two<ST>(p.x, row * p.sx + ch, have, xv);
-                load_two<ST>(p.f, row * p.sf + ch, have, fv);
-                if (DECAY) load_two<ST>(p.ig, row * p.si + ch, have, iv);
-            }
-#pragma unroll
             for (int v = 0; v < 2; ++v) {
-                float g, n;
-                logistic_pair(fv[v], g, n);
-                if (DECAY) {
-                    const float la = nsp[v] * g;
-                    a[j][v] = expf(la);
-                    u[j][v] = decay_input_factor(la, a[j][v]) * (logistic(iv[v]) * xv[v]);
-                } else {
-                    a[j][v] = g;
-                    u[j][v] = n * xv[v];
+                const int ch = w.dt * kGatedChannels + v * 32 + lane;
+                rates[s][v * 32 + lane] = ch < p.D ? p.scale * softplus(p.decay[ch]) : 0.0f;
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&full[s]);
+        }
+    }
+};
+
+// What both passes have in common: the pipeline of tiles around `body`, which calls `refill` behind its first
+// barrier and returns false to stop (all threads alike).
+template <typename ST, bool DECAY, bool BWD, int LOAD, typename Body>
+__device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMaps& maps, Body body)
+{
+    using T = GatedTile<ST, DECAY, BWD>;
+    using Word = typename T::Word;
+    extern __shared__ char gated_smem[];
+    char* stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(gated_smem) + 127) & ~(uintptr_t)127);
+    __shared__ __align__(8) uint64_t full[T::kStages];
+    __shared__ uint32_t tickets[T::kStages];
+    __shared__ float rates[T::kStages][kGatedChannels];
+    __shared__ int abort_flag;
+    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (LOAD == kLoadTma) {
+        if (tid == 0) {
+#pragma unroll
+            for (int s = 0; s < T::kStages; ++s) {
+                ptx::mbar_init(&full[s], 1u);
+                tickets[s] = 0u;
+            }
+            abort_flag = 0;
+            ptx::fence_mbar_init();
+        }
+        __syncthreads();
+        ptx::grid_dependency_wait();
+        const uint32_t epoch = read_epoch(p.header);
+        GatedRing<ST, DECAY, BWD> ring{p, maps, stages, full, tickets, rates, lane, 0u, 0u, false};
+        const bool issuer = warp == kGatedWarps - 1;
+        if (issuer) {
+            ring.draw();
+            for (int s = 0; s < T::kStages - (BWD ? 1 : 0); ++s) ring.refill();
+        }
+        uint32_t it = 0;
+        bool gave_up = false;
+        for (;; ++it) {
+            const int s = (int)(it % T::kStages);
+            if (!ptx::mbar_wait_bounded(&full[s], (it / T::kStages) & 1u, p.wait_budget)) {
+                // keeps step with the other warps up to the next barrier, where all of them see the flag
+                *(volatile int*)&abort_flag = 1;
+                atomicOr(p.header + 1, kStatusCopyTimeout);
+            }
+            const uint32_t ticket = *(volatile uint32_t*)&tickets[s];
+            if (ticket == 0xffffffffu) break;
+            if (!body(gated_where<BWD>(p, ticket), ticket, it, epoch, reinterpret_cast<const Word*>(stages + s * T::kStageBytes), rates[s],
+                      [&] { if (issuer) ring.refill(); }, (volatile int*)&abort_flag)) {
+                gave_up = true;
+                break;
+            }
+        }
+        if (issuer) {
+            // no copy may land in this CTA's shared memory after it has left
+            if (gave_up)
+                for (uint32_t i = it; i < ring.issued; ++i) (void)ptx::mbar_wait_bounded(&full[i % T::kStages], (i / T::kStages) & 1u, p.wait_budget);
+            if (lane == 0) finish_launch(p.header, epoch);
+        }
+        return;
+    }
+    ptx::grid_dependency_wait();
+    const uint32_t epoch = read_epoch(p.header);
+    if (tid == 0) {
+        tickets[0] = atomicAdd(p.header, 1u);
+        abort_flag = 0;
+    }
+    __syncthreads();
+    uint32_t ticket = tickets[0];
+    if ((long long)ticket < p.ntickets) gated_fetch<ST, DECAY, BWD, LOAD>(p, gated_where<BWD>(p, ticket), reinterpret_cast<Word*>(stages), warp, lane);
+    ptx::cp_async_commit();
+    for (uint32_t it = 0; (long long)ticket < p.ntickets; ++it) {
+        if (tid == 0) tickets[(it + 1) & 1] = atomicAdd(p.header, 1u);
+        const GatedWhere w = gated_where<BWD>(p, ticket);
+        if (DECAY && tid < kGatedChannels) {
+            const int ch = w.dt * kGatedChannels + tid;
+            rates[it & 1][tid] = ch < p.D ? p.scale * softplus(p.decay[ch]) : 0.0f;
+        }
+        __syncthreads();
+        const uint32_t next = tickets[(it + 1) & 1];
+        if ((long long)next < p.ntickets)
+            gated_fetch<ST, DECAY, BWD, LOAD>(p, gated_where<BWD>(p, next), reinterpret_cast<Word*>(stages + ((it + 1) & 1) * T::kStageBytes), warp, lane);
+        ptx::cp_async_commit();
+        ptx::cp_async_wait_group<1>();
+        body(w, ticket, it, epoch, reinterpret_cast<const Word*>(stages + (it & 1) * T::kStageBytes), rates[it & 1], [] {}, (volatile int*)&abort_flag);
+        ticket = next;
+    }
+    if (tid == 0) finish_launch(p.header, epoch);
+}
+
+// ---- forward ------------------------------------------------------------------------------------------
+template <typename ST, bool DECAY, int LOAD>
+__global__ void __launch_bounds__(kGatedThreads, 2)
+    gated_fwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
+{
+    using T = GatedTile<ST, DECAY, false>;
+    constexpr int K = T::K, R = T::R;
+    __shared__ float4 runs[2][kGatedWarps][32];      // (Y, P) of both channels of every thread
+    __shared__ float entering[kGatedChannels];
+    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    gated_tiles<ST, DECAY, false, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t ticket, uint32_t it, uint32_t epoch,
+                                                     const typename T::Word* stage, const float* rates, auto refill, volatile int* abort_flag) {
+        const int ch = w.dt * kGatedChannels + 2 * lane;
+        const int have = p.D - ch;
+        const long long s0 = (long long)w.k * R + warp * K;
+        TileDesc* desc = p.desc + ((long long)ticket * kGatedChannels + tid);
+        uint4 seen = make_uint4(0u, 0u, 0u, 0u);
+        if (tid < kGatedChannels && w.g > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
+        const GatedRun run = gated_run<K>(p, w.b, s0, lane);
+        const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
+        const int wstep = p.reverse ? -32 : 32;
+
+        float a[K][2], u[K][2];
+        auto gates = [&](auto small) {
+            float rate[2] = {0.0f, 0.0f};
+            if (DECAY) rate[0] = rates[2 * lane], rate[1] = rates[2 * lane + 1];
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                float xv[2], fv[2], iv[2];
+                Two<ST>::unpack(words[j * wstep], xv);
+                Two<ST>::unpack(words[j * wstep + R * 32], fv);
+                if (DECAY) Two<ST>::unpack(words[j * wstep + 2 * R * 32], iv);
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (DECAY) {
+                        float b2;
+                        decay_factors<T::kFast, decltype(small)::value>(rate[v] * logistic<T::kFast>(fv[v]), a[j][v], b2);
+                        u[j][v] = approx_sqrt(b2) * (logistic<T::kFast>(iv[v]) * xv[v]);
+                    } else {
+                        float n;
+                        logistic_pair<T::kFast>(fv[v], a[j][v], n);
+                        u[j][v] = n * xv[v];
+                    }
                 }
             }
-            if (!(run.valid >> j & 1u)) u[j][0] = u[j][1] = 0.0f;
-            if (run.start >> j & 1u) {
-                const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                float hv[2] = {0.0f, 0.0f};
-                if (p.h0) load_two<float>(p.h0, (long long)q * p.D + ch, have, hv);
+        };
+        // a slow decay (rate below 1/4 in all of the warp's channels) never needs the exponential
+        if (DECAY && !__all_sync(0xffffffffu, rates[2 * lane] < 0.25f && rates[2 * lane + 1] < 0.25f)) gates(std::false_type{});
+        else gates(std::true_type{});
+        if (run.cut) {
 #pragma unroll
-                for (int v = 0; v < 2; ++v) u[j][v] = fmaf(a[j][v], hv[v], u[j][v]);
+            for (int j = 0; j < K; ++j) {
+                if (!(run.valid >> j & 1u)) u[j][0] = u[j][1] = 0.0f;
+                if (p.h0 && (run.start >> j & 1u)) {
+                    const int q = __shfl_sync(0xffffffffu, run.seq, j);
+                    float hv[2];
+                    load_two<float>(p.h0, (long long)q * p.D + ch, have, hv);
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) u[j][v] = fmaf(a[j][v], hv[v], u[j][v]);
+                }
             }
         }
         Pair agg[2] = {pair_identity(), pair_identity()};
@@ -326,142 +553,162 @@ __global__ void __launch_bounds__(kGatedThreads) gated_fwd_kernel(const GatedPar
         float4(*set)[32] = runs[it & 1];
         set[warp][lane] = make_float4(agg[0].y, agg[0].p, agg[1].y, agg[1].p);
         __syncthreads();
+        if (LOAD == kLoadTma && *abort_flag) return false;
+        refill();
 
         if (tid < kGatedChannels) {
             Pair total = pair_identity();
 #pragma unroll
             for (int i = 0; i < kGatedWarps; ++i) {
-                const float2 w = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1];
-                total = join(total, Pair{w.x, w.y});
+                const float2 r = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1];
+                total = join(total, Pair{r.x, r.y});
             }
-            entering[tid] = gated_link(p, desc, seen, k, total, epoch);
+            entering[tid] = gated_link(p, desc, seen, w.g, total, epoch);
         }
         Pair before[2] = {pair_identity(), pair_identity()};
         for (int i = 0; i < warp; ++i) {
-            const float4 w = set[i][lane];
-            before[0] = join(before[0], Pair{w.x, w.y});
-            before[1] = join(before[1], Pair{w.z, w.w});
+            const float4 r = set[i][lane];
+            before[0] = join(before[0], Pair{r.x, r.y});
+            before[1] = join(before[1], Pair{r.z, r.w});
         }
         __syncthreads();
         float h[2];
 #pragma unroll
         for (int v = 0; v < 2; ++v) h[v] = enter(entering[2 * lane + v], before[v]);
         if (p.ckpt && s0 % kGatedCheckpoint == 0 && s0 < p.nrows)
-            store_two<float>(p.ckpt, ((long long)b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h);
+            store_two<float>(p.ckpt, ((long long)w.b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h);
+        const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
+        const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
+        ST* y = static_cast<ST*>(p.y) + row0 * p.D + ch;
+        const long long ystep = p.reverse ? -(long long)p.D : p.D;
+        const int rows = (int)min((long long)K, p.nrows - s0);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            if (s0 + j >= p.nrows) break;
+            if (j >= rows) break;
 #pragma unroll
             for (int v = 0; v < 2; ++v) h[v] = (run.cut >> j & 1u) ? u[j][v] : fmaf(a[j][v], h[v], u[j][v]);
-            store_two<ST>(p.y, (row0 + (long long)j * step) * p.D + ch, have, h);
+            store_two<ST>(y, j * ystep, have, h, pair);
             if (p.hT && (run.end >> j & 1u)) {
                 const int q = __shfl_sync(0xffffffffu, run.seq, j);
                 store_two<float>(p.hT, (long long)q * p.D + ch, have, h);
             }
         }
-    }
-    if (tid == 0) finish_launch(p.header, epoch);
+        return true;
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-template <typename ST, bool DECAY>
-__global__ void __launch_bounds__(kGatedThreads) gated_bwd_kernel(const GatedParams p)
+// Between the two halves of a tile a thread keeps a, b, s(i) and the state in front of each of its elements;
+// x, dy and the logits stay in shared memory and what else is needed is evaluated again from them (two
+// exponentials cheaper than the registers: keeping everything leaves one CTA per SM).
+template <typename ST, bool DECAY, int LOAD>
+__global__ void __launch_bounds__(kGatedThreads, 2)
+    gated_bwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
 {
-    constexpr int K = GatedTile<ST>::kRunBwd, R = GatedTile<ST>::kRowsBwd;
+    using T = GatedTile<ST, DECAY, true>;
+    constexpr int K = T::K, R = T::R;
     static_assert(R == kGatedCheckpoint, "one checkpoint per tile");
+    constexpr int kDy = (T::kArrays - 1) * R * 32;
     __shared__ float4 runs[2][kGatedWarps][32];      // (Y, P) of both channels, forward direction
     __shared__ float2 back[2][kGatedWarps][32];      // Y of both channels, adjoint direction (same P)
     __shared__ float entering[kGatedChannels];
     __shared__ float2 dsum[kGatedWarps][32];
-    __shared__ uint32_t next_ticket;
-
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    ptx::grid_dependency_wait();
-    const uint32_t epoch = read_epoch(p.header);
 
-    for (int it = 0;; ++it) {
-        if (tid == 0) next_ticket = atomicAdd(p.header, 1u);
-        __syncthreads();
-        const uint32_t ticket = next_ticket;
-        if ((long long)ticket >= p.ntickets) break;
-        const int g = (int)(ticket / (uint32_t)p.units);      // tiles in adjoint order
-        const int unit = (int)(ticket - (uint32_t)g * (uint32_t)p.units);
-        const int k = p.nk - 1 - g;
-        const int b = unit / p.dtiles, dt = unit - b * p.dtiles;
-        const int ch = dt * kGatedChannels + 2 * lane;
+    gated_tiles<ST, DECAY, true, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t ticket, uint32_t it, uint32_t epoch,
+                                                    const typename T::Word* stage, const float* rates, auto refill, volatile int* abort_flag) {
+        const int ch = w.dt * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
-        const long long s0 = (long long)k * R + warp * K;
-        const GatedRun run = gated_run<K>(p, b, s0, lane);
+        const long long s0 = (long long)w.k * R + warp * K;
         TileDesc* desc = p.desc + ((long long)ticket * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && g > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
-        const long long row0 = (long long)b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
-        const int step = p.reverse ? -1 : 1;
-
-        float nsp[2] = {0.0f, 0.0f};
+        if (tid < kGatedChannels && w.g > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
         float h[2];
-        load_two<float>(p.ckpt, ((long long)b * p.nck + k) * p.D + ch, have, h);
-        if (DECAY) {
+        load_two<float>(p.ckpt, ((long long)w.b * p.nck + w.k) * p.D + ch, have, h);
+        const GatedRun run = gated_run<K>(p, w.b, s0, lane);
+        const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
+        const int wstep = p.reverse ? -32 : 32;
+        float rate[2] = {0.0f, 0.0f};
+        if (DECAY) rate[0] = rates[2 * lane], rate[1] = rates[2 * lane + 1];
+
+        // add: b u, later the state in front of the element
+        float a[K][2], bb[K][2], gi[K][2], add[K][2];
+        auto gates = [&](auto small) {
 #pragma unroll
-            for (int v = 0; v < 2; ++v)
-                if (v < have) nsp[v] = -p.scale * softplus(p.decay[ch + v]);
+            for (int j = 0; j < K; ++j) {
+                float xv[2], fv[2], iv[2];
+                Two<ST>::unpack(words[j * wstep], xv);
+                Two<ST>::unpack(words[j * wstep + R * 32], fv);
+                if (DECAY) Two<ST>::unpack(words[j * wstep + 2 * R * 32], iv);
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    if (DECAY) {
+                        float b2;
+                        decay_factors<T::kFast, decltype(small)::value>(rate[v] * logistic<T::kFast>(fv[v]), a[j][v], b2);
+                        bb[j][v] = approx_sqrt(b2);
+                        gi[j][v] = logistic<T::kFast>(iv[v]);
+                        add[j][v] = bb[j][v] * (gi[j][v] * xv[v]);
+                    } else {
+                        logistic_pair<T::kFast>(fv[v], a[j][v], bb[j][v]);
+                        add[j][v] = bb[j][v] * xv[v];
+                    }
+                }
+            }
+        };
+        if (DECAY && !__all_sync(0xffffffffu, rate[0] < 0.25f && rate[1] < 0.25f)) gates(std::false_type{});
+        else gates(std::true_type{});
+        // initial states and final gradients of sequences that start or end in this run
+        auto state_of = [&](const float* states, uint32_t mask, int j, float* v) {
+            v[0] = v[1] = 0.0f;
+            if (states && (mask >> j & 1u)) {
+                const int q = __shfl_sync(0xffffffffu, run.seq, j);
+                load_two<float>(states, (long long)q * p.D + ch, have, v);
+            }
+        };
+        auto gradient = [&](int j, float* v) {
+            Two<ST>::unpack(words[j * wstep + kDy], v);
+            if (p.dhT && (run.end >> j & 1u)) {
+                float e[2];
+                state_of(p.dhT, run.end, j, e);
+                v[0] += e[0];
+                v[1] += e[1];
+            }
+        };
+        if (~run.valid & ((1u << K) - 1u)) {
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (!(run.valid >> j & 1u)) {
+                    a[j][0] = a[j][1] = bb[j][0] = bb[j][1] = add[j][0] = add[j][1] = 0.0f;
+                    if (DECAY) gi[j][0] = gi[j][1] = 0.0f;
+                }
         }
-        float a[K][2], bb[K][2], x[K][2], dyv[K][2], sn[K][2], gi[K][2], la[K][2], hs[K][2];
         Pair agg[2] = {pair_identity(), pair_identity()};
 #pragma unroll
         for (int j = 0; j < K; ++j) {
-            float fv[2] = {0.0f, 0.0f}, iv[2] = {0.0f, 0.0f};
-            x[j][0] = x[j][1] = dyv[j][0] = dyv[j][1] = hs[j][0] = hs[j][1] = 0.0f;
-            const bool ok = run.valid >> j & 1u;
-            if (ok) {
-                const long long row = row0 + (long long)j * step;
-                load_two<ST>(p.x, row * p.sx + ch, have, x[j]);
-                load_two<ST>(p.f, row * p.sf + ch, have, fv);
-                if (DECAY) load_two<ST>(p.ig, row * p.si + ch, have, iv);
-                load_two<ST>(p.dy, row * p.sdy + ch, have, dyv[j]);
-                if (p.dhT && (run.end >> j & 1u)) {
-                    const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                    float e[2] = {0.0f, 0.0f};
-                    load_two<float>(p.dhT, (long long)q * p.D + ch, have, e);
-                    dyv[j][0] += e[0];
-                    dyv[j][1] += e[1];
-                }
-                if (p.h0 && (run.start >> j & 1u)) {
-                    const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                    load_two<float>(p.h0, (long long)q * p.D + ch, have, hs[j]);
-                }
-            }
+            const bool cut = run.cut >> j & 1u;
+            float start[2] = {0.0f, 0.0f};
+            if (cut) state_of(p.h0, run.start, j, start);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                float s;
-                logistic_pair(fv[v], s, sn[j][v]);
-                float uv = x[j][v];
-                if (DECAY) {
-                    la[j][v] = nsp[v] * s;
-                    a[j][v] = expf(la[j][v]);
-                    bb[j][v] = decay_input_factor(la[j][v], a[j][v]);
-                    gi[j][v] = logistic(iv[v]);
-                    uv *= gi[j][v];
-                } else {
-                    a[j][v] = s;
-                    bb[j][v] = sn[j][v];
-                }
-                if (!ok) a[j][v] = bb[j][v] = 0.0f;
-                const bool cut = run.cut >> j & 1u;
-                agg[v].y = fmaf(a[j][v], cut ? hs[j][v] : agg[v].y, bb[j][v] * uv);
+                agg[v].y = fmaf(a[j][v], cut ? start[v] : agg[v].y, add[j][v]);
                 agg[v].p = cut ? kCut : agg[v].p * a[j][v];
             }
         }
-        float qv[2] = {0.0f, 0.0f};
+        float q[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int j = K - 1; j >= 0; --j)
+        for (int j = K - 1; j >= 0; --j) {
+            float dy[2];
+            gradient(j, dy);
 #pragma unroll
-            for (int v = 0; v < 2; ++v) qv[v] = (run.cut >> j & 1u) ? 0.0f : a[j][v] * (dyv[j][v] + qv[v]);
+            for (int v = 0; v < 2; ++v) q[v] = (run.cut >> j & 1u) ? 0.0f : a[j][v] * (dy[v] + q[v]);
+        }
         float4(*set)[32] = runs[it & 1];
         float2(*bset)[32] = back[it & 1];
         set[warp][lane] = make_float4(agg[0].y, agg[0].p, agg[1].y, agg[1].p);
-        bset[warp][lane] = make_float2(qv[0], qv[1]);
+        bset[warp][lane] = make_float2(q[0], q[1]);
         __syncthreads();
+        if (LOAD == kLoadTma && *abort_flag) return false;
+        refill();
 
         if (tid < kGatedChannels) {
             Pair total = pair_identity();
@@ -471,64 +718,72 @@ __global__ void __launch_bounds__(kGatedThreads) gated_bwd_kernel(const GatedPar
                 const float Y = reinterpret_cast<const float*>(&bset[i][tid >> 1])[tid & 1];
                 total = join(total, Pair{Y, P});
             }
-            entering[tid] = gated_link(p, desc, seen, g, total, epoch);
+            entering[tid] = gated_link(p, desc, seen, w.g, total, epoch);
         }
         // the state that enters this run, from the checkpoint
         for (int i = 0; i < warp; ++i) {
-            const float4 w = set[i][lane];
-            h[0] = enter(h[0], Pair{w.x, w.y});
-            h[1] = enter(h[1], Pair{w.z, w.w});
+            const float4 r = set[i][lane];
+            h[0] = enter(h[0], Pair{r.x, r.y});
+            h[1] = enter(h[1], Pair{r.z, r.w});
         }
         Pair after[2] = {pair_identity(), pair_identity()};
         for (int i = kGatedWarps - 1; i > warp; --i) {
-            const float4 w = set[i][lane];
+            const float4 r = set[i][lane];
             const float2 y = bset[i][lane];
-            after[0] = join(after[0], Pair{y.x, w.y});
-            after[1] = join(after[1], Pair{y.y, w.w});
+            after[0] = join(after[0], Pair{y.x, r.y});
+            after[1] = join(after[1], Pair{y.y, r.w});
         }
 #pragma unroll
-        for (int j = 0; j < K; ++j)
+        for (int j = 0; j < K; ++j) {
+            if (run.cut >> j & 1u) state_of(p.h0, run.start, j, h);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                const float before = (run.cut >> j & 1u) ? hs[j][v] : h[v];
-                hs[j][v] = before;
-                float uv = x[j][v];
-                if (DECAY) uv *= gi[j][v];
-                h[v] = fmaf(a[j][v], before, bb[j][v] * uv);
+                const float before = h[v];
+                h[v] = fmaf(a[j][v], before, add[j][v]);
+                add[j][v] = before;
             }
+        }
         __syncthreads();
-        float q[2], dl[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < 2; ++v) q[v] = enter(entering[2 * lane + v], after[v]);
+        float dl[2] = {0.0f, 0.0f};
+        const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
+        const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
+        const long long at0 = row0 * p.D + ch, astep = p.reverse ? -(long long)p.D : p.D;
 #pragma unroll
         for (int j = K - 1; j >= 0; --j) {
             const bool cut = run.cut >> j & 1u, ok = run.valid >> j & 1u;
-            float odx[2], odf[2], odi[2], oq[2];
+            float xv[2], fv[2], dy[2], odx[2], odf[2], odi[2], oq[2];
+            Two<ST>::unpack(words[j * wstep], xv);
+            gradient(j, dy);
+            if (DECAY) Two<ST>::unpack(words[j * wstep + R * 32], fv);
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                const float w = dyv[j][v] + q[v];
-                oq[v] = a[j][v] * w;
+                const float grad = dy[v] + q[v], b = bb[j][v], hp = add[j][v];
+                oq[v] = a[j][v] * grad;
                 q[v] = cut ? 0.0f : oq[v];
+                const float wb = grad * b;
                 if (DECAY) {
-                    const float u = gi[j][v] * x[j][v];
-                    const float aa = a[j][v], slope = bb[j][v] > 0.0f ? __fdividef(aa * aa, bb[j][v]) : 0.0f;
-                    const float dla = w * fmaf(aa, hs[j][v], -u * slope);
-                    const float t = dla * la[j][v];
-                    dl[v] += ok ? t : 0.0f;
-                    odx[v] = w * bb[j][v] * gi[j][v];
-                    odi[v] = w * bb[j][v] * (u * (1.0f - gi[j][v]));
-                    odf[v] = t * sn[j][v];
+                    float s, n;
+                    logistic_pair<T::kFast>(fv[v], s, n);
+                    const float u = gi[j][v] * xv[v];
+                    const float slope = b > 0.0f ? a[j][v] * approx_rcp(b) : 0.0f;
+                    // d(log a) * log a, with log a = -rate s
+                    const float t = oq[v] * fmaf(-u, slope, hp) * (-rate[v] * s);
+                    if (ok) dl[v] += t;
+                    odx[v] = wb * gi[j][v];
+                    odi[v] = wb * (u * (1.0f - gi[j][v]));
+                    odf[v] = t * n;
                 } else {
-                    odx[v] = w * bb[j][v];
-                    odf[v] = oq[v] * bb[j][v] * (hs[j][v] - x[j][v]);
+                    odx[v] = wb;
+                    odf[v] = oq[v] * b * (hp - xv[v]);
                 }
             }
             if (s0 + j < p.nrows) {
-                const long long at = (row0 + (long long)j * step) * p.D + ch;
                 if (!ok) odx[0] = odx[1] = odf[0] = odf[1] = odi[0] = odi[1] = 0.0f;
-                store_two<ST>(p.dx, at, have, odx);
-                store_two<ST>(p.df, at, have, odf);
-                if (DECAY) store_two<ST>(p.di, at, have, odi);
+                store_two<ST>(p.dx, at0 + j * astep, have, odx, pair);
+                store_two<ST>(p.df, at0 + j * astep, have, odf, pair);
+                if (DECAY) store_two<ST>(p.di, at0 + j * astep, have, odi, pair);
                 if (p.dh0 && (run.start >> j & 1u)) {
                     const int n = __shfl_sync(0xffffffffu, run.seq, j);
                     store_two<float>(p.dh0, (long long)n * p.D + ch, have, oq);
@@ -538,15 +793,15 @@ __global__ void __launch_bounds__(kGatedThreads) gated_bwd_kernel(const GatedPar
         if (DECAY) {
             dsum[warp][lane] = make_float2(dl[0], dl[1]);
             __syncthreads();
-            if (tid < kGatedChannels && dt * kGatedChannels + tid < p.D) {
+            if (tid < kGatedChannels && w.dt * kGatedChannels + tid < p.D) {
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kGatedWarps; ++i) s += reinterpret_cast<const float*>(&dsum[i][tid >> 1])[tid & 1];
-                p.dlam[((long long)b * p.nk + k) * p.D + dt * kGatedChannels + tid] = s;
+                p.dlam[((long long)w.b * p.nk + w.k) * p.D + w.dt * kGatedChannels + tid] = s;
             }
         }
-    }
-    if (tid == 0) finish_launch(p.header, epoch);
+        return true;
+    });
 }
 
 // Gradient of the decay parameter from the tiles' sums, in a fixed order: d L = s(L)/softplus(L) * sum.
@@ -565,7 +820,7 @@ static __global__ void __launch_bounds__(256) gated_decay_grad_kernel(const floa
     if (warp == 0 && ch < D) {
         for (int i = 1; i < 8; ++i) s += sums[i][lane];
         const float L = decay[ch], sp = softplus(L);
-        out[ch] = (float)s * (sp > 0.0f ? logistic(L) / sp : 1.0f);
+        out[ch] = (float)s * (sp > 0.0f ? logistic<false>(L) / sp : 1.0f);
     }
 }
 
@@ -595,6 +850,7 @@ __device__ __forceinline__ long long step_slot(const GatedStepParams& p, int r)
 template <typename ST, bool DECAY>
 __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p)
 {
+    constexpr bool kFast = sizeof(ST) == 2;
     __shared__ int nearest;
     const int tid = (int)threadIdx.x;
     const int ch = ((int)blockIdx.y * 128 + tid) * 2;
@@ -614,12 +870,12 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p
     if (__syncthreads_or(earlier)) return;
     const bool chain = __syncthreads_or(later);
 
-    float h[2] = {0.0f, 0.0f}, nsp[2] = {0.0f, 0.0f};
+    float h[2] = {0.0f, 0.0f}, rate[2] = {0.0f, 0.0f};
     load_two<float>(p.state, slot * p.sstate + ch, have, h);
     if (DECAY) {
 #pragma unroll
         for (int v = 0; v < 2; ++v)
-            if (v < have) nsp[v] = -p.scale * softplus(p.decay[ch + v]);
+            if (v < have) rate[v] = p.scale * softplus(p.decay[ch + v]);
     }
     while (true) {
         float xv[2], fv[2], iv[2];
@@ -628,12 +884,13 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p
         if (DECAY) load_two<ST>(p.ig, (long long)row * p.si + ch, have, iv);
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
-            float s, n;
-            logistic_pair(fv[v], s, n);
             if (DECAY) {
-                const float la = nsp[v] * s, a = expf(la);
-                h[v] = fmaf(a, h[v], decay_input_factor(la, a) * (logistic(iv[v]) * xv[v]));
+                float a, b2;
+                decay_factors<kFast, false>(rate[v] * logistic<kFast>(fv[v]), a, b2);
+                h[v] = fmaf(a, h[v], approx_sqrt(b2) * (logistic<kFast>(iv[v]) * xv[v]));
             } else {
+                float s, n;
+                logistic_pair<kFast>(fv[v], s, n);
                 h[v] = fmaf(s, h[v], n * xv[v]);
             }
         }

@@ -28,6 +28,7 @@ struct NormParams {
 };
 
 // act(v) and its derivative.
+template <bool FAST>
 __device__ __forceinline__ void activate(int act, float v, float& value, float& slope)
 {
     if (act == kActNone) {
@@ -36,7 +37,7 @@ __device__ __forceinline__ void activate(int act, float v, float& value, float& 
         return;
     }
     float p, n;
-    logistic_pair(v, p, n);
+    logistic_pair<FAST>(v, p, n);
     if (act == kActSilu) {
         value = v * p;
         slope = p * fmaf(v, n, 1.0f);
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(256) norm_fwd_kernel(const NormParams p)
         at(i, row, ch);
         const float z = fmaf((to_f32<ST>(x[row * p.sx + ch]) - mean) * inv, p.w ? p.w[ch] : 1.0f, p.b ? p.b[ch] : 0.0f);
         float v, slope;
-        activate(p.act, gate ? to_f32<ST>(gate[row * p.sg + ch]) : z, v, slope);
+        activate<sizeof(ST) == 2>(p.act, gate ? to_f32<ST>(gate[row * p.sg + ch]) : z, v, slope);
         static_cast<ST*>(p.y)[row * p.C + ch] = from_f32<ST>(gate ? z * v : v);
     }
 }
@@ -109,11 +110,11 @@ __device__ __forceinline__ void norm_element(const NormParams& p, float2 st, lon
     const float dy = to_f32<ST>(static_cast<const ST*>(p.dy)[row * p.sdy + ch]);
     float v, slope;
     if (p.gate) {
-        activate(p.act, to_f32<ST>(static_cast<const ST*>(p.gate)[row * p.sg + ch]), v, slope);
+        activate<sizeof(ST) == 2>(p.act, to_f32<ST>(static_cast<const ST*>(p.gate)[row * p.sg + ch]), v, slope);
         dz = dy * v;
         dgate = dy * z * slope;
     } else {
-        activate(p.act, z, v, slope);
+        activate<sizeof(ST) == 2>(p.act, z, v, slope);
         dz = dy * slope;
         dgate = 0.0f;
     }

@@ -4,7 +4,8 @@ u = 2^-24.  A sum of n terms taken by threads and a tree is off by at most (32 +
 absolute terms: no thread adds more than n/64 of them one after the other, and the trees and shared-memory
 passes above it add fewer than 32.  A variance may be formed from sums of squares about any element of the
 same channel, so its error counts the squares of the largest distance from the channel's mean.  Logistic
-values are within 6u, slopes of activations below 1.1, second slopes below 0.5.
+values are within 6u, for 16-bit operands within (8 + 1.3 |v|) u, which 16u and 20u below cover for |v| < 6 and
+half a step of the result's type by far beyond; slopes of activations are below 1.1, second slopes below 0.5.
 """
 import numpy as np
 
