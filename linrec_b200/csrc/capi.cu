@@ -249,7 +249,7 @@ int occupancy(const void* fn, int threads, size_t smem, int& out)
     std::lock_guard<std::mutex> lock(g_mutex);
     auto it = g_occupancy.find(key);
     if (it == g_occupancy.end()) {
-        if (smem > 48 * 1024) {
+        if (smem > 32 * 1024) {   // (static shared memory counts towards the 48 KB as well)
             const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
             if (e != cudaSuccess) {
                 cudaGetLastError();

@@ -12,7 +12,6 @@ using linrec::GatedParams;
 using linrec::GatedStepParams;
 using linrec::kGatedChannels;
 using linrec::kGatedCheckpoint;
-using linrec::kGatedThreads;
 using linrec_host::DeviceInfo;
 
 bool known_dtype(int dtype)
@@ -42,7 +41,7 @@ int check(const linrec_gated_args* a)
     if (!a->decay != !a->input_gate) return LINREC_ERR_INVALID_ARG;
     if (a->nseq >= 0x7fffffffLL || a->nrows >= 0x40000000LL || a->nchan >= 0x40000000LL) return LINREC_ERR_INVALID_ARG;
     if (!a->cu_seqlens && (a->seqlen > a->nrows || a->nseq * a->seqlen != a->nrows)) return LINREC_ERR_INVALID_ARG;
-    const int64_t rows = (a->nrows + 63) / 64, chans = (a->nchan + 63) / 64;
+    const int64_t rows = a->nrows / kGatedCheckpoint + 1, chans = (a->nchan + 63) / 64;
     if ((rows + a->nseq) * chans >= 0x7f000000LL) return LINREC_ERR_INVALID_ARG;   // tickets are 32-bit
     return LINREC_OK;
 }
@@ -88,6 +87,16 @@ int make_map(CUtensorMap* map, const void* ptr, int64_t stride, const GatedParam
     snprintf(msg, sizeof(msg), "driver error %d", (int)r);
     linrec_host::note_cuda_error("cuTensorMapEncodeTiled", msg);
     return LINREC_ERR_CUDA;
+}
+
+// How many consecutive tiles of a column one CTA takes.  Jobs of four tiles where there are about as many
+// columns as CTAs at least (a job waits for its predecessor, handed out `units` jobs earlier: (8, 4096, 4096)
+// forward, 512 columns on 444 CTAs, 306 us as single tiles, 247 in fours, 259 in eights); fewer columns are
+// single tiles linked by decoupled look-back ((1, 32768, 2048), 32 columns: 240 us, 530 in fours).
+int tiles_per_job(long long units, int nk, long long slots)
+{
+    const int want = 7 * units >= 6 * slots ? 4 : 1;
+    return want < nk ? want : nk;
 }
 
 int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream_)
@@ -151,11 +160,19 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
                  (!on_boundary(in[i], stride[i], size, 16) || !p.pair || (double)stride[i] * size * (double)ax.nrows >= 1e12))
             load = linrec::kLoadWord;
     }
-    const linrec_variants::GatedKernel kernel = a.dtype == LINREC_DTYPE_F32 ? linrec_variants::gated_kernel_f32(bwd, decay, load)
-                                              : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::gated_kernel_bf16(bwd, decay, load)
-                                                                             : linrec_variants::gated_kernel_f16(bwd, decay, load);
+    // as many columns as the small CTAs of an SM-filling grid, or fewer, larger ones
+    const int shape = p.units < (bwd ? 2 : 3) * dev.sm_count;
+    const linrec_variants::GatedKernel kernel = a.dtype == LINREC_DTYPE_F32 ? linrec_variants::gated_kernel_f32(bwd, decay, load, shape)
+                                              : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::gated_kernel_bf16(bwd, decay, load, shape)
+                                                                             : linrec_variants::gated_kernel_f16(bwd, decay, load, shape);
     p.nk = linrec_host::ceil_div_i(ax.nrows, kernel.rows);
-    p.ntickets = (long long)p.nk * p.units;
+    int occ = 0;
+    rc = linrec_host::occupancy(reinterpret_cast<const void*>(kernel.fn), kernel.threads, (size_t)kernel.smem, occ);
+    if (rc != LINREC_OK) return rc;
+    const long long slots = (long long)dev.sm_count * occ;
+    p.tiles_per_job = tiles_per_job(p.units, p.nk, slots);
+    p.jobs = linrec_host::ceil_div_i(p.nk, p.tiles_per_job);
+    p.ntickets = (long long)p.jobs * p.units;
     linrec::GatedMaps maps{};
     if (load == linrec::kLoadTma) {
         CUtensorMap* to[4] = {&maps.x, &maps.f, &maps.i, &maps.dy};
@@ -165,15 +182,12 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
             if (rc != LINREC_OK) return rc;
         }
     }
-    int occ = 0;
-    rc = linrec_host::occupancy(reinterpret_cast<const void*>(kernel.fn), kGatedThreads, (size_t)kernel.smem, occ);
-    if (rc != LINREC_OK) return rc;
-    long long grid = (long long)dev.sm_count * occ;
+    long long grid = slots;
     if (grid > p.ntickets) grid = p.ntickets;
-    rc = linrec_host::launch("gated recurrence", kernel.fn, dim3((unsigned)grid), kGatedThreads, (size_t)kernel.smem, stream, p, maps);
+    rc = linrec_host::launch("gated recurrence", kernel.fn, dim3((unsigned)grid), kernel.threads, (size_t)kernel.smem, stream, p, maps);
     if (rc != LINREC_OK || !bwd || !decay) return rc;
     return linrec_host::launch("decay gradient", linrec::gated_decay_grad_kernel, dim3((unsigned)linrec_host::ceil_div_i(a.nchan, 32)), 256, 0,
-                               stream, (const float*)p.dlam, (long long)p.nk * p.nb, p.D, p.decay, a.ddecay);
+                               stream, (const float*)p.dlam, (long long)p.jobs * p.nb, p.D, p.decay, a.ddecay);
 }
 
 template <typename ST>
@@ -193,7 +207,7 @@ size_t linrec_b200_gated_workspace_size(const linrec_gated_args* args)
     size_t n = linrec::kHeaderBytes;
     if (check(args) == LINREC_OK) {
         const Axes ax = axes_of(*args);
-        const size_t tiles = (size_t)((ax.nrows + 63) / 64) * ax.nb * (size_t)((args->nchan + kGatedChannels - 1) / kGatedChannels);
+        const size_t tiles = (size_t)((ax.nrows + kGatedCheckpoint - 1) / kGatedCheckpoint) * ax.nb * (size_t)((args->nchan + kGatedChannels - 1) / kGatedChannels);
         n += tiles * kGatedChannels * sizeof(linrec::TileDesc);
     }
     return n;

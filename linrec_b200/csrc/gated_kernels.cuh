@@ -36,10 +36,8 @@
 
 namespace linrec {
 
-constexpr int kGatedWarps = 8;
 constexpr int kGatedChannels = 64;      // channels per tile: 32 lanes x 2
 constexpr int kGatedCheckpoint = 64;    // positions between two checkpoints
-constexpr int kGatedThreads = kGatedWarps * 32;
 
 struct GatedParams {
     const void *x, *f, *ig, *dy;        // (rows, D) with the row strides below; ig: decay form only; dy: backward only
@@ -52,7 +50,7 @@ struct GatedParams {
     const float* dhT;                   // [nseq][D] or null (backward)
     float* dh0;                         // [nseq][D] or null (backward)
     float* ckpt;                        // [nb * nck][D]: state that enters positions 0, 64, 128, ...; null: not wanted
-    float* dlam;                        // [nb * nk][D]: sums of d(log a) log a over a tile (backward, decay form)
+    float* dlam;                        // [nb * jobs][D]: sums of d(log a) log a over a job (backward, decay form)
     const void* cu;                     // nseq + 1 offsets, or null: sequences of `seqlen` rows
     int cu64;
     int nseq;
@@ -61,10 +59,11 @@ struct GatedParams {
     int nb;                             // axes (batch entries scanned side by side)
     int D, dtiles, units;               // units = nb * dtiles
     int nk, nck;                        // tiles, checkpoints per axis
-    long long ntickets;                 // nk * units
+    int tiles_per_job, jobs;            // a ticket is a job: consecutive tiles of one column; jobs per column
+    long long ntickets;                 // jobs * units
     int reverse;
     uint32_t* header;
-    TileDesc* desc;                     // [nk][units][64]
+    TileDesc* desc;                     // [jobs][units][64]
     long long wait_budget;
     int pair;                           // results may be written two channels at a time
 };
@@ -87,6 +86,29 @@ __device__ __forceinline__ void decay_factors(float y, float& a, float& b2)
         d = 1.0f - a;
     }
     b2 = d * (1.0f + a);
+}
+
+// The same for two channels.
+template <bool FAST, bool SMALL>
+__device__ __forceinline__ void decay_factors2(F2 y, F2& a, F2& b)
+{
+    if (SMALL) {
+        F2 s = f2_fma(y, f2(-1.0f / 720.0f), f2(1.0f / 120.0f));
+        s = f2_fma(y, s, f2(-1.0f / 24.0f));
+        s = f2_fma(y, s, f2(1.0f / 6.0f));
+        s = f2_fma(y, s, f2(-0.5f));
+        const F2 d = f2_mul(y, f2_fma(y, s, f2(1.0f)));
+        a = f2_fma(d, f2(-1.0f), f2(1.0f));
+        const float2 b2 = f2_get(f2_fma(d, a, d));
+        b = f2(approx_sqrt(b2.x), approx_sqrt(b2.y));
+    } else {
+        const float2 w = f2_get(y);
+        float a0, a1, b0, b1;
+        decay_factors<FAST, false>(w.x, a0, b0);
+        decay_factors<FAST, false>(w.y, a1, b1);
+        a = f2(a0, a1);
+        b = f2(approx_sqrt(b0), approx_sqrt(b1));
+    }
 }
 
 // ---- the pair operator with cuts ------------------------------------------------------------------------
@@ -153,9 +175,34 @@ __device__ __forceinline__ GatedRun gated_run(const GatedParams& p, int b, long 
     r.start = __ballot_sync(0xffffffffu, st);
     r.end = __ballot_sync(0xffffffffu, en);
     r.valid = __ballot_sync(0xffffffffu, ok);
-    r.cut = r.start | ~r.valid;
+    r.cut = (r.start | ~r.valid) & ((1u << K) - 1u);
     r.seq = q;
     return r;
+}
+
+// ---- tiles and jobs ------------------------------------------------------------------------------------
+// One tile: `k` along the axis in forward scan order (< 0: no more tiles), its job in the order of this pass,
+// axis, channel block; `first` and `last` of its job.
+struct GatedWhere {
+    int k, job, b, dt;
+    static constexpr int kFirst = 1 << 30, kLast = 1 << 29;
+    __device__ __forceinline__ int block() const { return dt & (kLast - 1); }
+    __device__ __forceinline__ bool first() const { return dt & kFirst; }
+    __device__ __forceinline__ bool last() const { return dt & kLast; }
+};
+template <bool BWD>
+__device__ __forceinline__ GatedWhere gated_where(const GatedParams& p, uint32_t ticket, int t)
+{
+    GatedWhere w;
+    w.job = (int)(ticket / (uint32_t)p.units);
+    const int unit = (int)(ticket - (uint32_t)w.job * (uint32_t)p.units);
+    const int g = w.job * p.tiles_per_job + t;
+    w.b = unit / p.dtiles;
+    w.dt = unit - w.b * p.dtiles;
+    if (t == 0) w.dt |= GatedWhere::kFirst;
+    if (t + 1 == p.tiles_per_job || g + 1 == p.nk) w.dt |= GatedWhere::kLast;
+    w.k = BWD ? p.nk - 1 - g : g;
+    return w;
 }
 
 // ---- linking a tile to its predecessor -----------------------------------------------------------------
@@ -221,83 +268,94 @@ __device__ __forceinline__ float gated_lookback(const TileDesc* d, long long str
     return v;
 }
 
-// Run by 64 threads, one channel each: returns the value that enters the tile and publishes the one that
-// leaves it.  `k` counts tiles along the axis in the direction of the scan; `d` is this tile's descriptor.
-__device__ __forceinline__ float gated_link(const GatedParams& p, TileDesc* d, uint4 seen, int k, Pair total, uint32_t epoch)
+// Run by 64 threads, one channel each, in the first tile of a job: returns the value that enters it.  `d` is
+// the job's descriptor, `seen` what its predecessor's held a while ago.  Jobs of one tile publish their total
+// before they look back (decoupled look-back); a longer job, of which the first tile says nothing about the
+// whole, waits for its predecessor, which was handed out `units` tickets earlier.
+__device__ __forceinline__ float gated_link(const GatedParams& p, TileDesc* d, uint4 seen, int job, Pair total, uint32_t epoch, bool& published)
 {
+    published = false;
+    if (job == 0) return 0.0f;
+    if (seen.z == 2u && seen.w == (uint32_t)(job - 1)) return __uint_as_float(seen.x);
     const long long stride = (long long)p.units * kGatedChannels;
-    const bool more = k + 1 < p.nk;
-    float in = 0.0f;
-    bool done = false;
-    if (k > 0) {
-        if (seen.z == 2u && seen.w == (uint32_t)(k - 1)) {
-            in = __uint_as_float(seen.x);
-        } else {
-            // a total that forgets what enters (a sequence starts in the tile) is final already
-            if (more) {
-                done = is_cut(total.p);
-                col_publish(d, total.y, total.p, done ? 2u : 1u, epoch, (uint32_t)k);
-            }
-            in = gated_lookback(d - stride, stride, k, epoch, p.wait_budget, p.header + 1);
-        }
+    if (p.tiles_per_job > 1) {
+        seen.z = 0u;
+        return gated_await(d - stride, job - 1, seen, epoch, p.wait_budget, p.header + 1) ? __uint_as_float(seen.x) : 0.0f;
     }
-    if (more && !done) col_publish(d, enter(in, total), 0.0f, 2u, epoch, (uint32_t)k);
-    return in;
+    if (job + 1 < p.jobs) {
+        // a total that forgets what enters (a sequence starts in the tile) is final already
+        published = is_cut(total.p);
+        col_publish(d, total.y, total.p, published ? 2u : 1u, epoch, (uint32_t)job);
+    }
+    return gated_lookback(d - stride, stride, job, epoch, p.wait_budget, p.header + 1);
+}
+
+// The 64 threads' part of every tile: what enters it (beside `now`, where the first tile of a job finds it only
+// behind the next barrier) and what leaves it, for the next tile and the next job.
+__device__ __forceinline__ void gated_carry(const GatedParams& p, const GatedWhere& w, TileDesc* d, uint4 seen, Pair total, uint32_t epoch,
+                                            float* now, float* then)
+{
+    float in;
+    bool published = false;
+    if (w.first()) *now = in = gated_link(p, d, seen, w.job, total, epoch, published);
+    else in = *now;
+    const float out = enter(in, total);
+    *then = out;
+    if (w.last() && !published && w.job + 1 < p.jobs) col_publish(d, out, 0.0f, 2u, epoch, (uint32_t)w.job);
 }
 
 // ---- the tile ---------------------------------------------------------------------------------------------
 // How operands reach shared memory, where every thread finds the words of its own two channels and K
 // positions:
-//   kLoadTma    one bulk-tensor copy per operand through a ring of stages, issued by the last warp as soon as a
-//               barrier of the tile shows a stage free (rows on 16-byte boundaries); a ninth warp for the
-//               copies would cost every thread a quarter of its registers
+//   kLoadTma    one bulk-tensor copy per operand through a ring of stages, issued by a warp of its own (rows on
+//               16-byte boundaries)
 //   kLoadWord   4-byte asynchronous copies, every thread its own words, one tile ahead (4-byte boundaries)
 //   kLoadAny    plain loads by the thread, stored to the same place (any alignment)
 constexpr int kLoadTma = 0, kLoadWord = 1, kLoadAny = 2;
 
-template <typename ST, bool DECAY, bool BWD>
+// Two shapes of a CTA.  SHAPE 0: four warps, several CTAs per SM, whose phases (gates, which the special
+// function unit bounds, and the exchange between warps, which latency bounds) overlap each other's.  SHAPE 1:
+// eight warps and longer tiles, one CTA per SM: half as many tiles wait for one another along a column, which
+// counts when there are few columns, and it is the shape that fits 32-bit operands.
+// Measured, forward / backward us, 16-bit decay form: (8, 4096, 4096), 512 columns: 247 / 614 and 292 / 689;
+// (1, 32768, 2048), 32 columns: 269 / 735 and 240 / 598.
+template <typename ST, bool DECAY, bool BWD, int SHAPE>
 struct GatedTile {
     static constexpr bool kFast = sizeof(ST) == 2;                     // 16-bit results: fast exponentials will do
-    static constexpr int K = BWD || sizeof(ST) == 4 ? 8 : 16;          // positions per thread
-    static constexpr int R = K * kGatedWarps;                          // positions per tile
+    static constexpr int W = SHAPE ? 8 : 4;                            // warps
+    static constexpr int K = SHAPE && BWD ? 8 : 16;                    // positions per thread
+    static constexpr int R = K * W;                                    // positions per tile
+    static constexpr int kCtas = SHAPE ? 1 : BWD ? 2 : 3;              // per SM, for the register budget
+    static_assert(R % kGatedCheckpoint == 0, "workspaces hold descriptors for tiles of that many positions, the shortest");
     static constexpr int kArrays = (DECAY ? 3 : 2) + (BWD ? 1 : 0);    // x, f(, i)(, dy)
     static constexpr int kArrayBytes = R * kGatedChannels * (int)sizeof(ST);
     static constexpr int kStageBytes = kArrays * kArrayBytes;
     // forward: a stage is free once the gates are in registers; backward: only when the next tile has begun
-    static constexpr int kStages = BWD && sizeof(ST) == 2 ? 3 : 2;
-    static constexpr int kDynSmem = kStages * kStageBytes + 128;
+    static constexpr int kStages = SHAPE && BWD ? 3 : 2;
+    static constexpr int kDynSmem = kStages * kStageBytes;
     using Word = typename Two<ST>::Word;
+    static constexpr int threads(int load) { return (W + (load == kLoadTma ? 1 : 0)) * 32; }
 };
+
+// A barrier of the warps that own positions.
+template <int W>
+__device__ __forceinline__ void gated_sync()
+{
+    asm volatile("bar.sync 1, %0;" ::"n"(W * 32) : "memory");
+}
 
 struct GatedMaps {
     CUtensorMap x, f, i, dy;
 };
 
-struct GatedWhere {
-    int k;            // tile along the axis, in forward scan order
-    int g;            // the same in the order of this pass
-    int b, dt;        // axis, channel block
-};
-template <bool BWD>
-__device__ __forceinline__ GatedWhere gated_where(const GatedParams& p, uint32_t ticket)
-{
-    GatedWhere w;
-    w.g = (int)(ticket / (uint32_t)p.units);
-    const int unit = (int)(ticket - (uint32_t)w.g * (uint32_t)p.units);
-    w.b = unit / p.dtiles;
-    w.dt = unit - w.b * p.dtiles;
-    w.k = BWD ? p.nk - 1 - w.g : w.g;
-    return w;
-}
-
 // A thread's own words of one tile, by asynchronous 4-byte copies or plain loads.
-template <typename ST, bool DECAY, bool BWD, int LOAD>
+template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD>
 __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhere& w, typename Two<ST>::Word* stage, int warp, int lane)
 {
-    using T = GatedTile<ST, DECAY, BWD>;
+    using T = GatedTile<ST, DECAY, BWD, SHAPE>;
     const void* src[4] = {p.x, p.f, DECAY ? p.ig : p.dy, p.dy};
     const long long stride[4] = {p.sx, p.sf, DECAY ? p.si : p.sdy, p.sdy};
-    const int ch = w.dt * kGatedChannels + 2 * lane, have = p.D - ch;
+    const int ch = w.block() * kGatedChannels + 2 * lane, have = p.D - ch;
     const long long s0 = (long long)w.k * T::R + warp * T::K;
     const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
     const int step = p.reverse ? -1 : 1;
@@ -330,77 +388,86 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
     }
 }
 
-// The last warp's side of the ring: tickets (drawn one ahead, so that the counter's latency is hidden), copies,
-// and the block's decay parameters, which the other warps find beside the operands.
-template <typename ST, bool DECAY, bool BWD>
-struct GatedRing {
-    using T = GatedTile<ST, DECAY, BWD>;
-    const GatedParams& p;
-    const GatedMaps& maps;
-    char* stages;
-    uint64_t* full;
-    uint32_t* tickets;
-    float (*rates)[kGatedChannels];
-    int lane;
-    uint32_t ahead, issued;
-    bool drained;
-
-    __device__ __forceinline__ void draw()
-    {
-        if (lane == 0) ahead = atomicAdd(p.header, 1u);
-    }
-    __device__ __forceinline__ void refill()
-    {
-        if (drained) return;
-        const int s = (int)(issued % T::kStages);
-        const uint32_t ticket = __shfl_sync(0xffffffffu, ahead, 0);
-        if ((long long)ticket >= p.ntickets) {
-            drained = true;
-            if (lane == 0) {
-                tickets[s] = 0xffffffffu;
-                ptx::mbar_arrive(&full[s]);
-            }
-            return;
+// The warp behind the others: draws tickets (one ahead, so that the counter's latency is hidden), issues the
+// copies, and evaluates the block's decay parameters, which the other warps find beside the operands.
+template <typename ST, bool DECAY, bool BWD, int SHAPE>
+__device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedMaps& maps, char* stages, uint64_t* full, uint64_t* empty,
+                                              GatedWhere* items, float (*rates)[kGatedChannels], volatile int* abort_flag, uint32_t epoch)
+{
+    using T = GatedTile<ST, DECAY, BWD, SHAPE>;
+    const int lane = (int)threadIdx.x & 31;
+    uint32_t ahead = 0, j = 0, ticket = 0;
+    if (lane == 0) ahead = atomicAdd(p.header, 1u);
+    bool gave_up = false, more = true;
+    float rate[2] = {0.0f, 0.0f};
+    GatedWhere w;
+    w.dt = GatedWhere::kLast;
+    for (int t = 0;; ++j, ++t) {
+        const int s = (int)(j % T::kStages);
+        if (w.last()) {
+            t = 0;
+            ticket = __shfl_sync(0xffffffffu, ahead, 0);
+            more = (long long)ticket < p.ntickets;
+            if (more && lane == 0) ahead = atomicAdd(p.header, 1u);
         }
-        ++issued;
-        const GatedWhere w = gated_where<BWD>(p, ticket);
-        if (lane == 0) {
-            // (operands first: the barrier completes when the arrival below has come as well)
-            tickets[s] = ticket;
-            const int row = p.reverse ? (int)(p.nrows - (long long)(w.k + 1) * T::R) : w.k * T::R;
-            char* to = stages + s * T::kStageBytes;
-            if (DECAY) ptx::mbar_expect_tx(&full[s], (uint32_t)T::kStageBytes);
-            else ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
-            ptx::tma_load_3d(to, &maps.x, &full[s], w.dt * kGatedChannels, row, w.b);
-            ptx::tma_load_3d(to + T::kArrayBytes, &maps.f, &full[s], w.dt * kGatedChannels, row, w.b);
-            if (DECAY) ptx::tma_load_3d(to + 2 * T::kArrayBytes, &maps.i, &full[s], w.dt * kGatedChannels, row, w.b);
-            if (BWD) ptx::tma_load_3d(to + (T::kArrays - 1) * T::kArrayBytes, &maps.dy, &full[s], w.dt * kGatedChannels, row, w.b);
-        }
-        draw();
-        if (DECAY) {
+        w = gated_where<BWD>(p, ticket, t);
+        const int block = w.block() * kGatedChannels;
+        if (DECAY && more && w.first()) {
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-                const int ch = w.dt * kGatedChannels + v * 32 + lane;
-                rates[s][v * 32 + lane] = ch < p.D ? p.scale * softplus(p.decay[ch]) : 0.0f;
+                const int ch = block + v * 32 + lane;
+                rate[v] = ch < p.D ? p.scale * softplus(__ldg(p.decay + ch)) : 0.0f;
             }
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&full[s]);
         }
+        if (j >= (uint32_t)T::kStages && !ptx::mbar_wait_bounded(&empty[s], ((j / T::kStages) - 1u) & 1u, p.wait_budget)) gave_up = true;
+        gave_up = __any_sync(0xffffffffu, gave_up || *abort_flag);
+        if (gave_up) break;
+        if (DECAY) {
+            rates[s][lane] = rate[0];
+            rates[s][32 + lane] = rate[1];
+            __syncwarp();
+        }
+        if (lane == 0) {
+            items[s] = more ? w : GatedWhere{-1, 0, 0, 0};
+            if (more) {
+                const int row = p.reverse ? (int)(p.nrows - (long long)(w.k + 1) * T::R) : w.k * T::R;
+                char* to = stages + s * T::kStageBytes;
+                ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
+                ptx::tma_load_3d(to, &maps.x, &full[s], block, row, w.b);
+                ptx::tma_load_3d(to + T::kArrayBytes, &maps.f, &full[s], block, row, w.b);
+                if (DECAY) ptx::tma_load_3d(to + 2 * T::kArrayBytes, &maps.i, &full[s], block, row, w.b);
+                if (BWD) ptx::tma_load_3d(to + (T::kArrays - 1) * T::kArrayBytes, &maps.dy, &full[s], block, row, w.b);
+            } else {
+                ptx::mbar_arrive(&full[s]);
+            }
+        }
+        if (!more) break;
     }
-};
+    if (gave_up) {
+        *abort_flag = 1;
+        if (lane == 0) atomicOr(p.header + 1, kStatusCopyTimeout);
+        // no copy may land in this CTA's shared memory after it has left
+        for (uint32_t i = j > (uint32_t)T::kStages ? j - T::kStages : 0u; i < j; ++i)
+            (void)ptx::mbar_wait_bounded(&full[i % T::kStages], (i / T::kStages) & 1u, p.wait_budget);
+    }
+    if (lane == 0) finish_launch(p.header, epoch);
+}
 
-// What both passes have in common: the pipeline of tiles around `body`, which calls `refill` behind its first
-// barrier and returns false to stop (all threads alike).
-template <typename ST, bool DECAY, bool BWD, int LOAD, typename Body>
+// What both passes have in common: the pipeline of tiles around `body`, which calls `next` behind its first
+// barrier (where a stage is free: forward its own, backward the one of the tile before) and returns false to
+// stop (all threads alike).
+template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD, typename Body>
 __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMaps& maps, Body body)
 {
-    using T = GatedTile<ST, DECAY, BWD>;
+    using T = GatedTile<ST, DECAY, BWD, SHAPE>;
     using Word = typename T::Word;
-    extern __shared__ char gated_smem[];
-    char* stages = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(gated_smem) + 127) & ~(uintptr_t)127);
-    __shared__ __align__(8) uint64_t full[T::kStages];
-    __shared__ uint32_t tickets[T::kStages];
-    __shared__ float rates[T::kStages][kGatedChannels];
+    // (used as it is: rounding the address up would hide from the compiler that it is shared memory)
+    extern __shared__ __align__(128) char gated_smem[];
+    char* const stages = gated_smem;
+    __shared__ __align__(8) uint64_t full[T::kStages], empty[T::kStages];
+    __shared__ uint32_t tickets[2];
+    __shared__ __align__(16) GatedWhere items[T::kStages];
+    __shared__ __align__(8) float rates[T::kStages][kGatedChannels];
     __shared__ int abort_flag;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -409,7 +476,8 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
 #pragma unroll
             for (int s = 0; s < T::kStages; ++s) {
                 ptx::mbar_init(&full[s], 1u);
-                tickets[s] = 0u;
+                ptx::mbar_init(&empty[s], 1u);
+                items[s] = GatedWhere{0, 0, 0, 0};
             }
             abort_flag = 0;
             ptx::fence_mbar_init();
@@ -417,34 +485,26 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
         __syncthreads();
         ptx::grid_dependency_wait();
         const uint32_t epoch = read_epoch(p.header);
-        GatedRing<ST, DECAY, BWD> ring{p, maps, stages, full, tickets, rates, lane, 0u, 0u, false};
-        const bool issuer = warp == kGatedWarps - 1;
-        if (issuer) {
-            ring.draw();
-            for (int s = 0; s < T::kStages - (BWD ? 1 : 0); ++s) ring.refill();
+        if (warp == T::W) {
+            gated_produce<ST, DECAY, BWD, SHAPE>(p, maps, stages, full, empty, items, rates, &abort_flag, epoch);
+            return;
         }
-        uint32_t it = 0;
-        bool gave_up = false;
-        for (;; ++it) {
+        for (uint32_t it = 0;; ++it) {
             const int s = (int)(it % T::kStages);
             if (!ptx::mbar_wait_bounded(&full[s], (it / T::kStages) & 1u, p.wait_budget)) {
                 // keeps step with the other warps up to the next barrier, where all of them see the flag
                 *(volatile int*)&abort_flag = 1;
                 atomicOr(p.header + 1, kStatusCopyTimeout);
             }
-            const uint32_t ticket = *(volatile uint32_t*)&tickets[s];
-            if (ticket == 0xffffffffu) break;
-            if (!body(gated_where<BWD>(p, ticket), ticket, it, epoch, reinterpret_cast<const Word*>(stages + s * T::kStageBytes), rates[s],
-                      [&] { if (issuer) ring.refill(); }, (volatile int*)&abort_flag)) {
-                gave_up = true;
-                break;
-            }
-        }
-        if (issuer) {
-            // no copy may land in this CTA's shared memory after it has left
-            if (gave_up)
-                for (uint32_t i = it; i < ring.issued; ++i) (void)ptx::mbar_wait_bounded(&full[i % T::kStages], (i / T::kStages) & 1u, p.wait_budget);
-            if (lane == 0) finish_launch(p.header, epoch);
+            const int4 item = *reinterpret_cast<const int4*>(&items[s]);
+            if (item.x < 0) break;
+            const bool on = body(GatedWhere{item.x, item.y, item.z, item.w}, it, epoch, reinterpret_cast<const Word*>(stages + s * T::kStageBytes), rates[s],
+                                 [&] {
+                                     const uint32_t done = BWD ? it - 1u : it;
+                                     if (tid == 0 && (!BWD || it > 0)) ptx::mbar_arrive(&empty[done % T::kStages]);
+                                 },
+                                 (volatile int*)&abort_flag);
+            if (!on) break;
         }
         return;
     }
@@ -456,141 +516,154 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
     }
     __syncthreads();
     uint32_t ticket = tickets[0];
-    if ((long long)ticket < p.ntickets) gated_fetch<ST, DECAY, BWD, LOAD>(p, gated_where<BWD>(p, ticket), reinterpret_cast<Word*>(stages), warp, lane);
+    int t = 0;
+    GatedWhere w = gated_where<BWD>(p, ticket, 0);
+    bool more = (long long)ticket < p.ntickets;
+    if (more) gated_fetch<ST, DECAY, BWD, SHAPE, LOAD>(p, w, reinterpret_cast<Word*>(stages), warp, lane);
     ptx::cp_async_commit();
-    for (uint32_t it = 0; (long long)ticket < p.ntickets; ++it) {
-        if (tid == 0) tickets[(it + 1) & 1] = atomicAdd(p.header, 1u);
-        const GatedWhere w = gated_where<BWD>(p, ticket);
+    for (uint32_t it = 0; more; ++it) {
+        if (tid == 0 && w.last()) tickets[(it + 1) & 1] = atomicAdd(p.header, 1u);
         if (DECAY && tid < kGatedChannels) {
-            const int ch = w.dt * kGatedChannels + tid;
+            const int ch = w.block() * kGatedChannels + tid;
             rates[it & 1][tid] = ch < p.D ? p.scale * softplus(p.decay[ch]) : 0.0f;
         }
         __syncthreads();
-        const uint32_t next = tickets[(it + 1) & 1];
-        if ((long long)next < p.ntickets)
-            gated_fetch<ST, DECAY, BWD, LOAD>(p, gated_where<BWD>(p, next), reinterpret_cast<Word*>(stages + ((it + 1) & 1) * T::kStageBytes), warp, lane);
+        ++t;
+        if (w.last()) {
+            t = 0;
+            ticket = tickets[(it + 1) & 1];
+            more = (long long)ticket < p.ntickets;
+        }
+        const GatedWhere next = gated_where<BWD>(p, ticket, t);
+        if (more) gated_fetch<ST, DECAY, BWD, SHAPE, LOAD>(p, next, reinterpret_cast<Word*>(stages + ((it + 1) & 1) * T::kStageBytes), warp, lane);
         ptx::cp_async_commit();
         ptx::cp_async_wait_group<1>();
-        body(w, ticket, it, epoch, reinterpret_cast<const Word*>(stages + (it & 1) * T::kStageBytes), rates[it & 1], [] {}, (volatile int*)&abort_flag);
-        ticket = next;
+        body(w, it, epoch, reinterpret_cast<const Word*>(stages + (it & 1) * T::kStageBytes), rates[it & 1], [] {}, (volatile int*)&abort_flag);
+        w = next;
     }
     if (tid == 0) finish_launch(p.header, epoch);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
-template <typename ST, bool DECAY, int LOAD>
-__global__ void __launch_bounds__(kGatedThreads, 2)
+template <typename ST, bool DECAY, int SHAPE, int LOAD>
+__global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LOAD), GatedTile<ST, DECAY, false, SHAPE>::kCtas)
     gated_fwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
 {
-    using T = GatedTile<ST, DECAY, false>;
+    using T = GatedTile<ST, DECAY, false, SHAPE>;
     constexpr int K = T::K, R = T::R;
-    __shared__ float4 runs[2][kGatedWarps][32];      // (Y, P) of both channels of every thread
-    __shared__ float entering[kGatedChannels];
+    __shared__ float4 runs[2][T::W][32];      // (Y, P) of both channels of every thread
+    __shared__ __align__(8) float entering[2][kGatedChannels];      // tiles take turns
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    gated_tiles<ST, DECAY, false, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t ticket, uint32_t it, uint32_t epoch,
-                                                     const typename T::Word* stage, const float* rates, auto refill, volatile int* abort_flag) {
-        const int ch = w.dt * kGatedChannels + 2 * lane;
+    gated_tiles<ST, DECAY, false, SHAPE, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
+                                                     const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
+        const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
-        TileDesc* desc = p.desc + ((long long)ticket * kGatedChannels + tid);
+        TileDesc* desc = p.desc + (((long long)w.job * p.units + w.b * p.dtiles + w.block()) * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && w.g > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
+        if (tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
         const GatedRun run = gated_run<K>(p, w.b, s0, lane);
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
 
-        float a[K][2], u[K][2];
+        F2 a[K], u[K];
         auto gates = [&](auto small) {
-            float rate[2] = {0.0f, 0.0f};
-            if (DECAY) rate[0] = rates[2 * lane], rate[1] = rates[2 * lane + 1];
+            F2 rate = f2(0.0f);
+            if (DECAY) rate = f2(rates[2 * lane], rates[2 * lane + 1]);
+            const typename T::Word* at = words;
 #pragma unroll
-            for (int j = 0; j < K; ++j) {
-                float xv[2], fv[2], iv[2];
-                Two<ST>::unpack(words[j * wstep], xv);
-                Two<ST>::unpack(words[j * wstep + R * 32], fv);
-                if (DECAY) Two<ST>::unpack(words[j * wstep + 2 * R * 32], iv);
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    if (DECAY) {
-                        float b2;
-                        decay_factors<T::kFast, decltype(small)::value>(rate[v] * logistic<T::kFast>(fv[v]), a[j][v], b2);
-                        u[j][v] = approx_sqrt(b2) * (logistic<T::kFast>(iv[v]) * xv[v]);
-                    } else {
-                        float n;
-                        logistic_pair<T::kFast>(fv[v], a[j][v], n);
-                        u[j][v] = n * xv[v];
-                    }
+            for (int j = 0; j < K; ++j, at += wstep) {
+                const F2 xv = Two<ST>::get(at[0]), fv = Two<ST>::get(at[R * 32]);
+                if (DECAY) {
+                    F2 b;
+                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], b);
+                    u[j] = f2_mul(b, f2_mul(logistic2<T::kFast>(Two<ST>::get(at[2 * R * 32])), xv));
+                } else {
+                    F2 n;
+                    logistic_pair2<T::kFast>(fv, a[j], n);
+                    u[j] = f2_mul(n, xv);
                 }
             }
         };
         // a slow decay (rate below 1/4 in all of the warp's channels) never needs the exponential
         if (DECAY && !__all_sync(0xffffffffu, rates[2 * lane] < 0.25f && rates[2 * lane + 1] < 0.25f)) gates(std::false_type{});
         else gates(std::true_type{});
+        // a run in which sequences start, or rows belong to none, takes a path of its own: it selects where
+        // the common one multiplies
+        F2 Y = f2(0.0f), P = f2(1.0f);
         if (run.cut) {
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                if (!(run.valid >> j & 1u)) u[j][0] = u[j][1] = 0.0f;
-                if (p.h0 && (run.start >> j & 1u)) {
-                    const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                    float hv[2];
-                    load_two<float>(p.h0, (long long)q * p.D + ch, have, hv);
-#pragma unroll
-                    for (int v = 0; v < 2; ++v) u[j][v] = fmaf(a[j][v], hv[v], u[j][v]);
-                }
+                if (!(run.valid >> j & 1u)) u[j] = f2(0.0f);
+                if (p.h0 && (run.start >> j & 1u)) u[j] = f2_fma(a[j], load_state(p.h0, (long long)__shfl_sync(0xffffffffu, run.seq, j) * p.D + ch, have), u[j]);
+                const bool cut = run.cut >> j & 1u;
+                Y = cut ? u[j] : f2_fma(a[j], Y, u[j]);
+                P = cut ? f2(kCut) : f2_mul(P, a[j]);
             }
-        }
-        Pair agg[2] = {pair_identity(), pair_identity()};
+        } else {
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const bool cut = run.cut >> j & 1u;
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                agg[v].y = cut ? u[j][v] : fmaf(a[j][v], agg[v].y, u[j][v]);
-                agg[v].p = cut ? kCut : agg[v].p * a[j][v];
+            for (int j = 0; j < K; ++j) {
+                Y = f2_fma(a[j], Y, u[j]);
+                P = f2_mul(P, a[j]);
             }
         }
         float4(*set)[32] = runs[it & 1];
-        set[warp][lane] = make_float4(agg[0].y, agg[0].p, agg[1].y, agg[1].p);
-        __syncthreads();
+        const float2 y2 = f2_get(Y), p2 = f2_get(P);
+        set[warp][lane] = make_float4(y2.x, p2.x, y2.y, p2.y);
+        gated_sync<T::W>();
         if (LOAD == kLoadTma && *abort_flag) return false;
-        refill();
+        next();
 
         if (tid < kGatedChannels) {
             Pair total = pair_identity();
 #pragma unroll
-            for (int i = 0; i < kGatedWarps; ++i) {
+            for (int i = 0; i < T::W; ++i) {
                 const float2 r = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1];
                 total = join(total, Pair{r.x, r.y});
             }
-            entering[tid] = gated_link(p, desc, seen, w.g, total, epoch);
+            gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
         }
         Pair before[2] = {pair_identity(), pair_identity()};
-        for (int i = 0; i < warp; ++i) {
-            const float4 r = set[i][lane];
-            before[0] = join(before[0], Pair{r.x, r.y});
-            before[1] = join(before[1], Pair{r.z, r.w});
-        }
-        __syncthreads();
-        float h[2];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) h[v] = enter(entering[2 * lane + v], before[v]);
+        for (int i = 0; i < T::W - 1; ++i) {
+            const float4 r = set[i][lane];
+            if (i < warp) {
+                before[0] = join(before[0], Pair{r.x, r.y});
+                before[1] = join(before[1], Pair{r.z, r.w});
+            }
+        }
+        if (w.first()) gated_sync<T::W>();
+        const float* in = entering[it & 1];
+        F2 h = f2(enter(in[2 * lane], before[0]), enter(in[2 * lane + 1], before[1]));
         if (p.ckpt && s0 % kGatedCheckpoint == 0 && s0 < p.nrows)
-            store_two<float>(p.ckpt, ((long long)w.b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h);
+            store_two<float>(p.ckpt, ((long long)w.b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h, false);
         const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
         const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
         ST* y = static_cast<ST*>(p.y) + row0 * p.D + ch;
         const long long ystep = p.reverse ? -(long long)p.D : p.D;
-        const int rows = (int)min((long long)K, p.nrows - s0);
+        if (run.cut | run.end) {
+            const int rows = (int)min((long long)K, p.nrows - s0);
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (j >= rows) break;
+            for (int j = 0; j < K; ++j) {
+                if (j >= rows) break;
+                h = (run.cut >> j & 1u) ? u[j] : f2_fma(a[j], h, u[j]);
+                store_two<ST>(y + j * ystep, 0, have, h, pair);
+                if (p.hT && (run.end >> j & 1u)) store_two<float>(p.hT, (long long)__shfl_sync(0xffffffffu, run.seq, j) * p.D + ch, have, h, false);
+            }
+        } else if (pair) {
 #pragma unroll
-            for (int v = 0; v < 2; ++v) h[v] = (run.cut >> j & 1u) ? u[j][v] : fmaf(a[j][v], h[v], u[j][v]);
-            store_two<ST>(y, j * ystep, have, h, pair);
-            if (p.hT && (run.end >> j & 1u)) {
-                const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                store_two<float>(p.hT, (long long)q * p.D + ch, have, h);
+            for (int j = 0; j < K; ++j) {
+                h = f2_fma(a[j], h, u[j]);
+                *reinterpret_cast<typename T::Word*>(y) = Two<ST>::put(h);
+                y += ystep;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                h = f2_fma(a[j], h, u[j]);
+                store_two<ST>(y, 0, have, h, false);
+                y += ystep;
             }
         }
         return true;
@@ -598,206 +671,204 @@ __global__ void __launch_bounds__(kGatedThreads, 2)
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-// Between the two halves of a tile a thread keeps a, b, s(i) and the state in front of each of its elements;
-// x, dy and the logits stay in shared memory and what else is needed is evaluated again from them (two
-// exponentials cheaper than the registers: keeping everything leaves one CTA per SM).
-template <typename ST, bool DECAY, int LOAD>
-__global__ void __launch_bounds__(kGatedThreads, 2)
+// Between the two halves of a tile a thread keeps a, b and the state in front of each of its elements; x, dy
+// and the logits stay in shared memory and what else is needed is evaluated again from them.
+template <typename ST, bool DECAY, int SHAPE, int LOAD>
+__global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOAD), GatedTile<ST, DECAY, true, SHAPE>::kCtas)
     gated_bwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
 {
-    using T = GatedTile<ST, DECAY, true>;
+    using T = GatedTile<ST, DECAY, true, SHAPE>;
     constexpr int K = T::K, R = T::R;
     static_assert(R == kGatedCheckpoint, "one checkpoint per tile");
     constexpr int kDy = (T::kArrays - 1) * R * 32;
-    __shared__ float4 runs[2][kGatedWarps][32];      // (Y, P) of both channels, forward direction
-    __shared__ float2 back[2][kGatedWarps][32];      // Y of both channels, adjoint direction (same P)
-    __shared__ float entering[kGatedChannels];
-    __shared__ float2 dsum[kGatedWarps][32];
+    __shared__ float4 runs[2][T::W][32];      // (Y, P) of both channels, forward direction
+    __shared__ float2 back[2][T::W][32];      // Y of both channels, adjoint direction (same P)
+    __shared__ __align__(8) float entering[2][kGatedChannels];      // tiles take turns
+    __shared__ float2 dsum[T::W][32];
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    gated_tiles<ST, DECAY, true, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t ticket, uint32_t it, uint32_t epoch,
-                                                    const typename T::Word* stage, const float* rates, auto refill, volatile int* abort_flag) {
-        const int ch = w.dt * kGatedChannels + 2 * lane;
+    F2 dl = f2(0.0f);      // this thread's share of the decay gradient, over a job
+
+    gated_tiles<ST, DECAY, true, SHAPE, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
+                                                    const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
+        const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
-        TileDesc* desc = p.desc + ((long long)ticket * kGatedChannels + tid);
+        TileDesc* desc = p.desc + (((long long)w.job * p.units + w.b * p.dtiles + w.block()) * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && w.g > 0) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
-        float h[2];
-        load_two<float>(p.ckpt, ((long long)w.b * p.nck + w.k) * p.D + ch, have, h);
+        if (tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
+        const float2 h0 = f2_get(load_state(p.ckpt, ((long long)w.b * p.nck + w.k) * p.D + ch, have));
         const GatedRun run = gated_run<K>(p, w.b, s0, lane);
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
-        float rate[2] = {0.0f, 0.0f};
-        if (DECAY) rate[0] = rates[2 * lane], rate[1] = rates[2 * lane + 1];
+        F2 rate = f2(0.0f);
+        if (DECAY) rate = f2(rates[2 * lane], rates[2 * lane + 1]);
 
         // add: b u, later the state in front of the element
-        float a[K][2], bb[K][2], gi[K][2], add[K][2];
+        F2 a[K], bb[K], add[K];
         auto gates = [&](auto small) {
+            const typename T::Word* at = words;
+#pragma unroll
+            for (int j = 0; j < K; ++j, at += wstep) {
+                const F2 xv = Two<ST>::get(at[0]), fv = Two<ST>::get(at[R * 32]);
+                if (DECAY) {
+                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], bb[j]);
+                    add[j] = f2_mul(bb[j], f2_mul(logistic2<T::kFast>(Two<ST>::get(at[2 * R * 32])), xv));
+                } else {
+                    logistic_pair2<T::kFast>(fv, a[j], bb[j]);
+                    add[j] = f2_mul(bb[j], xv);
+                }
+            }
+        };
+        if (DECAY && !__all_sync(0xffffffffu, rates[2 * lane] < 0.25f && rates[2 * lane + 1] < 0.25f)) gates(std::false_type{});
+        else gates(std::true_type{});
+        // `edge`: sequences start or end in this run, or rows belong to none
+        const bool edge = run.cut || run.end;
+        auto of_sequence = [&](const float* states, int j) {
+            return load_state(states, (long long)__shfl_sync(0xffffffffu, run.seq, j) * p.D + ch, have);
+        };
+        const typename T::Word* const words_end = words + (K - 1) * wstep;
+        auto gradient = [&](const typename T::Word* at, int j, bool edge) {
+            F2 dy = Two<ST>::get(at[kDy]);
+            if (edge && p.dhT && (run.end >> j & 1u)) dy = f2_add(dy, of_sequence(p.dhT, j));
+            return dy;
+        };
+        F2 Y = f2(0.0f), P = f2(1.0f), q = f2(0.0f);
+        const typename T::Word* at = words_end;
+        if (edge) {
 #pragma unroll
             for (int j = 0; j < K; ++j) {
-                float xv[2], fv[2], iv[2];
-                Two<ST>::unpack(words[j * wstep], xv);
-                Two<ST>::unpack(words[j * wstep + R * 32], fv);
-                if (DECAY) Two<ST>::unpack(words[j * wstep + 2 * R * 32], iv);
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    if (DECAY) {
-                        float b2;
-                        decay_factors<T::kFast, decltype(small)::value>(rate[v] * logistic<T::kFast>(fv[v]), a[j][v], b2);
-                        bb[j][v] = approx_sqrt(b2);
-                        gi[j][v] = logistic<T::kFast>(iv[v]);
-                        add[j][v] = bb[j][v] * (gi[j][v] * xv[v]);
-                    } else {
-                        logistic_pair<T::kFast>(fv[v], a[j][v], bb[j][v]);
-                        add[j][v] = bb[j][v] * xv[v];
-                    }
-                }
+                const bool cut = run.cut >> j & 1u;
+                if (!(run.valid >> j & 1u)) a[j] = bb[j] = add[j] = f2(0.0f);
+                if (cut) Y = p.h0 && (run.start >> j & 1u) ? of_sequence(p.h0, j) : f2(0.0f);
+                Y = f2_fma(a[j], Y, add[j]);
+                P = cut ? f2(kCut) : f2_mul(P, a[j]);
             }
-        };
-        if (DECAY && !__all_sync(0xffffffffu, rate[0] < 0.25f && rate[1] < 0.25f)) gates(std::false_type{});
-        else gates(std::true_type{});
-        // initial states and final gradients of sequences that start or end in this run
-        auto state_of = [&](const float* states, uint32_t mask, int j, float* v) {
-            v[0] = v[1] = 0.0f;
-            if (states && (mask >> j & 1u)) {
-                const int q = __shfl_sync(0xffffffffu, run.seq, j);
-                load_two<float>(states, (long long)q * p.D + ch, have, v);
+#pragma unroll
+            for (int j = K - 1; j >= 0; --j, at -= wstep) q = (run.cut >> j & 1u) ? f2(0.0f) : f2_mul(a[j], f2_add(gradient(at, j, true), q));
+        } else {
+#pragma unroll
+            for (int j = 0; j < K; ++j) {
+                Y = f2_fma(a[j], Y, add[j]);
+                P = f2_mul(P, a[j]);
             }
-        };
-        auto gradient = [&](int j, float* v) {
-            Two<ST>::unpack(words[j * wstep + kDy], v);
-            if (p.dhT && (run.end >> j & 1u)) {
-                float e[2];
-                state_of(p.dhT, run.end, j, e);
-                v[0] += e[0];
-                v[1] += e[1];
-            }
-        };
-        if (~run.valid & ((1u << K) - 1u)) {
 #pragma unroll
-            for (int j = 0; j < K; ++j)
-                if (!(run.valid >> j & 1u)) {
-                    a[j][0] = a[j][1] = bb[j][0] = bb[j][1] = add[j][0] = add[j][1] = 0.0f;
-                    if (DECAY) gi[j][0] = gi[j][1] = 0.0f;
-                }
-        }
-        Pair agg[2] = {pair_identity(), pair_identity()};
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const bool cut = run.cut >> j & 1u;
-            float start[2] = {0.0f, 0.0f};
-            if (cut) state_of(p.h0, run.start, j, start);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                agg[v].y = fmaf(a[j][v], cut ? start[v] : agg[v].y, add[j][v]);
-                agg[v].p = cut ? kCut : agg[v].p * a[j][v];
-            }
-        }
-        float q[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int j = K - 1; j >= 0; --j) {
-            float dy[2];
-            gradient(j, dy);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) q[v] = (run.cut >> j & 1u) ? 0.0f : a[j][v] * (dy[v] + q[v]);
+            for (int j = K - 1; j >= 0; --j, at -= wstep) q = f2_mul(a[j], f2_add(gradient(at, j, false), q));
         }
         float4(*set)[32] = runs[it & 1];
         float2(*bset)[32] = back[it & 1];
-        set[warp][lane] = make_float4(agg[0].y, agg[0].p, agg[1].y, agg[1].p);
-        bset[warp][lane] = make_float2(q[0], q[1]);
-        __syncthreads();
+        const float2 y2 = f2_get(Y), p2 = f2_get(P);
+        set[warp][lane] = make_float4(y2.x, p2.x, y2.y, p2.y);
+        bset[warp][lane] = f2_get(q);
+        gated_sync<T::W>();
         if (LOAD == kLoadTma && *abort_flag) return false;
-        refill();
+        next();
 
         if (tid < kGatedChannels) {
             Pair total = pair_identity();
 #pragma unroll
-            for (int i = kGatedWarps - 1; i >= 0; --i) {
+            for (int i = T::W - 1; i >= 0; --i) {
                 const float P = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1].y;
                 const float Y = reinterpret_cast<const float*>(&bset[i][tid >> 1])[tid & 1];
                 total = join(total, Pair{Y, P});
             }
-            entering[tid] = gated_link(p, desc, seen, w.g, total, epoch);
+            gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
         }
         // the state that enters this run, from the checkpoint
-        for (int i = 0; i < warp; ++i) {
-            const float4 r = set[i][lane];
-            h[0] = enter(h[0], Pair{r.x, r.y});
-            h[1] = enter(h[1], Pair{r.z, r.w});
-        }
+        float hx = h0.x, hy = h0.y;
         Pair after[2] = {pair_identity(), pair_identity()};
-        for (int i = kGatedWarps - 1; i > warp; --i) {
+#pragma unroll
+        for (int i = 0; i < T::W - 1; ++i) {
             const float4 r = set[i][lane];
-            const float2 y = bset[i][lane];
-            after[0] = join(after[0], Pair{y.x, r.y});
-            after[1] = join(after[1], Pair{y.y, r.w});
-        }
-#pragma unroll
-        for (int j = 0; j < K; ++j) {
-            if (run.cut >> j & 1u) state_of(p.h0, run.start, j, h);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const float before = h[v];
-                h[v] = fmaf(a[j][v], before, add[j][v]);
-                add[j][v] = before;
+            if (i < warp) {
+                hx = enter(hx, Pair{r.x, r.y});
+                hy = enter(hy, Pair{r.z, r.w});
             }
         }
-        __syncthreads();
 #pragma unroll
-        for (int v = 0; v < 2; ++v) q[v] = enter(entering[2 * lane + v], after[v]);
-        float dl[2] = {0.0f, 0.0f};
+        for (int i = T::W - 1; i > 0; --i) {
+            const float4 r = set[i][lane];
+            const float2 y = bset[i][lane];
+            if (i > warp) {
+                after[0] = join(after[0], Pair{y.x, r.y});
+                after[1] = join(after[1], Pair{y.y, r.w});
+            }
+        }
+        F2 h = f2(hx, hy);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            if (edge && (run.cut >> j & 1u)) h = p.h0 && (run.start >> j & 1u) ? of_sequence(p.h0, j) : f2(0.0f);
+            const F2 before = h;
+            h = f2_fma(a[j], before, add[j]);
+            add[j] = before;
+        }
+        if (w.first()) gated_sync<T::W>();
+        const float* in = entering[it & 1];
+        q = f2(enter(in[2 * lane], after[0]), enter(in[2 * lane + 1], after[1]));
+        if (w.first()) dl = f2(0.0f);
         const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
         const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
         const long long at0 = row0 * p.D + ch, astep = p.reverse ? -(long long)p.D : p.D;
+        // gradients of element j; q becomes what flows on to the element before it
+        at = words_end;
+        auto element = [&](int j, bool edge, F2& odx, F2& odf, F2& odi) {
+            const F2 xv = Two<ST>::get(at[0]);
+            const F2 grad = f2_add(gradient(at, j, edge), q), hp = add[j];
+            q = f2_mul(a[j], grad);
+            const F2 wb = f2_mul(grad, bb[j]);
+            if (DECAY) {
+                F2 s, n;
+                logistic_pair2<T::kFast>(Two<ST>::get(at[R * 32]), s, n);
+                const float2 b = f2_get(bb[j]);
+                // -a/b, left out where the factor b has vanished (its share is the root of a log a below 1e-38)
+                const F2 minus_slope = f2_mul(a[j], f2(b.x > 0.0f ? -approx_rcp(b.x) : 0.0f, b.y > 0.0f ? -approx_rcp(b.y) : 0.0f));
+                const F2 gi = logistic2<T::kFast>(Two<ST>::get(at[2 * R * 32])), u = f2_mul(gi, xv);
+                // d(log a) * log a, with log a = -rate s
+                const F2 t = f2_mul(f2_mul(q, f2_fma(u, minus_slope, hp)), f2_mul(f2_mul(rate, f2(-1.0f)), s));
+                odx = f2_mul(wb, gi);
+                odi = f2_mul(wb, f2_mul(u, f2_fma(gi, f2(-1.0f), f2(1.0f))));
+                odf = f2_mul(t, n);
+                if (!edge || (run.valid >> j & 1u)) dl = f2_add(dl, t);
+            } else {
+                odx = wb;
+                odf = f2_mul(f2_mul(q, bb[j]), f2_fma(xv, f2(-1.0f), hp));
+                odi = odx;
+            }
+        };
+        if (edge || !pair) {
 #pragma unroll
-        for (int j = K - 1; j >= 0; --j) {
-            const bool cut = run.cut >> j & 1u, ok = run.valid >> j & 1u;
-            float xv[2], fv[2], dy[2], odx[2], odf[2], odi[2], oq[2];
-            Two<ST>::unpack(words[j * wstep], xv);
-            gradient(j, dy);
-            if (DECAY) Two<ST>::unpack(words[j * wstep + R * 32], fv);
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const float grad = dy[v] + q[v], b = bb[j][v], hp = add[j][v];
-                oq[v] = a[j][v] * grad;
-                q[v] = cut ? 0.0f : oq[v];
-                const float wb = grad * b;
-                if (DECAY) {
-                    float s, n;
-                    logistic_pair<T::kFast>(fv[v], s, n);
-                    const float u = gi[j][v] * xv[v];
-                    const float slope = b > 0.0f ? a[j][v] * approx_rcp(b) : 0.0f;
-                    // d(log a) * log a, with log a = -rate s
-                    const float t = oq[v] * fmaf(-u, slope, hp) * (-rate[v] * s);
-                    if (ok) dl[v] += t;
-                    odx[v] = wb * gi[j][v];
-                    odi[v] = wb * (u * (1.0f - gi[j][v]));
-                    odf[v] = t * n;
-                } else {
-                    odx[v] = wb;
-                    odf[v] = oq[v] * b * (hp - xv[v]);
+            for (int j = K - 1; j >= 0; --j, at -= wstep) {
+                F2 odx, odf, odi;
+                element(j, true, odx, odf, odi);
+                if (p.dh0 && (run.start >> j & 1u)) store_two<float>(p.dh0, (long long)__shfl_sync(0xffffffffu, run.seq, j) * p.D + ch, have, q, false);
+                if (run.cut >> j & 1u) q = f2(0.0f);
+                if (s0 + j < p.nrows) {
+                    if (!(run.valid >> j & 1u)) odx = odf = odi = f2(0.0f);
+                    store_two<ST>(p.dx, at0 + j * astep, have, odx, pair);
+                    store_two<ST>(p.df, at0 + j * astep, have, odf, pair);
+                    if (DECAY) store_two<ST>(p.di, at0 + j * astep, have, odi, pair);
                 }
             }
-            if (s0 + j < p.nrows) {
-                if (!ok) odx[0] = odx[1] = odf[0] = odf[1] = odi[0] = odi[1] = 0.0f;
-                store_two<ST>(p.dx, at0 + j * astep, have, odx, pair);
-                store_two<ST>(p.df, at0 + j * astep, have, odf, pair);
-                if (DECAY) store_two<ST>(p.di, at0 + j * astep, have, odi, pair);
-                if (p.dh0 && (run.start >> j & 1u)) {
-                    const int n = __shfl_sync(0xffffffffu, run.seq, j);
-                    store_two<float>(p.dh0, (long long)n * p.D + ch, have, oq);
-                }
+        } else {
+            long long to = at0 + (K - 1) * astep;
+#pragma unroll
+            for (int j = K - 1; j >= 0; --j, at -= wstep) {
+                F2 odx, odf, odi;
+                element(j, false, odx, odf, odi);
+                *reinterpret_cast<typename T::Word*>(static_cast<ST*>(p.dx) + to) = Two<ST>::put(odx);
+                *reinterpret_cast<typename T::Word*>(static_cast<ST*>(p.df) + to) = Two<ST>::put(odf);
+                if (DECAY) *reinterpret_cast<typename T::Word*>(static_cast<ST*>(p.di) + to) = Two<ST>::put(odi);
+                to -= astep;
             }
         }
-        if (DECAY) {
-            dsum[warp][lane] = make_float2(dl[0], dl[1]);
-            __syncthreads();
-            if (tid < kGatedChannels && w.dt * kGatedChannels + tid < p.D) {
+        if (DECAY && w.last()) {
+            dsum[warp][lane] = f2_get(dl);
+            gated_sync<T::W>();
+            if (tid < kGatedChannels && w.block() * kGatedChannels + tid < p.D) {
                 float s = 0.0f;
 #pragma unroll
-                for (int i = 0; i < kGatedWarps; ++i) s += reinterpret_cast<const float*>(&dsum[i][tid >> 1])[tid & 1];
-                p.dlam[((long long)w.b * p.nk + w.k) * p.D + w.dt * kGatedChannels + tid] = s;
+                for (int i = 0; i < T::W; ++i) s += reinterpret_cast<const float*>(&dsum[i][tid >> 1])[tid & 1];
+                p.dlam[((long long)w.b * p.jobs + w.job) * p.D + w.block() * kGatedChannels + tid] = s;
             }
         }
         return true;

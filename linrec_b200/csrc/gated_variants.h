@@ -10,28 +10,43 @@ struct GatedKernel {
     GatedFn fn;
     int smem;        // dynamic shared memory
     int rows;        // positions per tile
+    int threads;
 };
 
-GatedKernel gated_kernel_f32(bool bwd, bool decay, int load);
-GatedKernel gated_kernel_bf16(bool bwd, bool decay, int load);
-GatedKernel gated_kernel_f16(bool bwd, bool decay, int load);
+// shape: 0 or 1 (GatedTile); 32-bit operands and rows off 16-byte boundaries have one shape each.
+GatedKernel gated_kernel_f32(bool bwd, bool decay, int load, int shape);
+GatedKernel gated_kernel_bf16(bool bwd, bool decay, int load, int shape);
+GatedKernel gated_kernel_f16(bool bwd, bool decay, int load, int shape);
 
-template <typename ST, bool DECAY, int LOAD>
+template <typename ST, bool DECAY, int SHAPE, int LOAD>
 GatedKernel gated_pick(bool bwd)
 {
     using namespace linrec;
-    if (bwd) return {gated_bwd_kernel<ST, DECAY, LOAD>, GatedTile<ST, DECAY, true>::kDynSmem, GatedTile<ST, DECAY, true>::R};
-    return {gated_fwd_kernel<ST, DECAY, LOAD>, GatedTile<ST, DECAY, false>::kDynSmem, GatedTile<ST, DECAY, false>::R};
+    using F = GatedTile<ST, DECAY, false, SHAPE>;
+    using B = GatedTile<ST, DECAY, true, SHAPE>;
+    if (bwd) return {gated_bwd_kernel<ST, DECAY, SHAPE, LOAD>, B::kDynSmem, B::R, B::threads(LOAD)};
+    return {gated_fwd_kernel<ST, DECAY, SHAPE, LOAD>, F::kDynSmem, F::R, F::threads(LOAD)};
+}
+
+template <typename ST, bool DECAY>
+GatedKernel gated_pick(bool bwd, int load, int shape)
+{
+    using namespace linrec;
+    if constexpr (sizeof(ST) == 4) {
+        // 32-bit elements always lie on 4-byte boundaries
+        if (load == kLoadTma) return gated_pick<ST, DECAY, 1, kLoadTma>(bwd);
+        return gated_pick<ST, DECAY, 1, kLoadWord>(bwd);
+    } else {
+        if (load == kLoadTma) return shape ? gated_pick<ST, DECAY, 1, kLoadTma>(bwd) : gated_pick<ST, DECAY, 0, kLoadTma>(bwd);
+        if (load == kLoadWord) return gated_pick<ST, DECAY, 0, kLoadWord>(bwd);
+        return gated_pick<ST, DECAY, 0, kLoadAny>(bwd);
+    }
 }
 
 template <typename ST>
-GatedKernel gated_pick(bool bwd, bool decay, int load)
+GatedKernel gated_pick(bool bwd, bool decay, int load, int shape)
 {
-    using namespace linrec;
-    if (load == kLoadTma) return decay ? gated_pick<ST, true, kLoadTma>(bwd) : gated_pick<ST, false, kLoadTma>(bwd);
-    // 32-bit elements always lie on 4-byte boundaries
-    if (sizeof(ST) == 4 || load == kLoadWord) return decay ? gated_pick<ST, true, kLoadWord>(bwd) : gated_pick<ST, false, kLoadWord>(bwd);
-    if constexpr (sizeof(ST) == 2) return decay ? gated_pick<ST, true, kLoadAny>(bwd) : gated_pick<ST, false, kLoadAny>(bwd);
+    return decay ? gated_pick<ST, true>(bwd, load, shape) : gated_pick<ST, false>(bwd, load, shape);
 }
 
 }  // namespace linrec_variants
