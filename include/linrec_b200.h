@@ -343,8 +343,9 @@ LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const v
  * activation: 0 none, 1 v s(v), 2 s(v), with s the logistic function.  weight and bias: nchan floats, or NULL
  * for ones and zeros.  stats: nsamples * groups pairs (mean, 1/sqrt(var + eps)), written by the forward pass
  * if given, required by the backward pass.  Results have rows at stride nchan.  dweight and dbias may be
- * NULL; otherwise the backward pass needs linrec_b200_group_norm_scratch_size bytes of scratch.  What follows the recurrence
- * in a layer with heads: one position per sample, heads as groups.  No counterpart in the reference. */
+ * NULL.  Either pass may need scratch (linrec_b200_group_norm_scratch_size for the same arguments; need not be
+ * cleared, 16-byte aligned; a call's own until its kernels have run).  What follows the recurrence in a layer with
+ * heads: one position per sample, heads as groups.  No counterpart in the reference. */
 typedef struct linrec_group_norm_args {
     const void* x;
     const void* gate;            /* or NULL */
@@ -357,7 +358,7 @@ typedef struct linrec_group_norm_args {
     int64_t nsamples, positions, nchan, groups;
     float* stats;
     void* y;                     /* forward */
-    const void* dy;              /* backward, as are all below */
+    const void* dy;              /* backward, as are the next five */
     int64_t dy_stride;
     void* dx;
     void* dgate;
@@ -366,7 +367,7 @@ typedef struct linrec_group_norm_args {
     void* scratch;
     size_t scratch_bytes;
 } linrec_group_norm_args;
-LINREC_API size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args);
+LINREC_API size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args, int bwd);
 LINREC_API int linrec_b200_group_norm_fwd(const linrec_group_norm_args* args, void* stream);
 LINREC_API int linrec_b200_group_norm_bwd(const linrec_group_norm_args* args, void* stream);
 

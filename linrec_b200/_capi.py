@@ -124,7 +124,7 @@ def _load() -> ctypes.CDLL:
     lib.linrec_b200_gated_step.argtypes = [vp, vp, vp, i64, i64, i64, vp, ctypes.c_float, vp, vp, i64, i64, vp, i32, i64, i64, i32, vp]
     lib.linrec_b200_gated_step.restype = i32
     pn = ctypes.POINTER(GroupNormArgs)
-    lib.linrec_b200_group_norm_scratch_size.argtypes = [pn]
+    lib.linrec_b200_group_norm_scratch_size.argtypes = [pn, i32]
     lib.linrec_b200_group_norm_scratch_size.restype = sz
     for name in ("fwd", "bwd"):
         fn = getattr(lib, "linrec_b200_group_norm_" + name)

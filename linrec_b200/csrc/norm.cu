@@ -17,38 +17,108 @@ int check(const linrec_group_norm_args* a)
     return LINREC_OK;
 }
 
-int parts_of(const linrec_group_norm_args& a)
-{
-    const long long rows = a.nsamples * a.positions;
-    return (int)(rows < 256 ? (rows > 0 ? rows : 1) : 256);
-}
+// How a problem is laid out; the scratch sizes follow from it, so it depends on sizes and alignment alone (the
+// grid is sized for 148 SMs whatever the device).
+constexpr long long kCtas = 148 * 4;
 
-NormParams params_of(const linrec_group_norm_args& a)
+struct Plan {
+    bool rows;
+    int V;               // elements per thread and access: 8 on 16-byte boundaries, else 1
+    int nv;              // rows: pieces per lane
+    int lanes, gb, rp;   // rows
+    int cpb, sub, slices, xblocks;
+    long long yblocks;   // rows: CTAs along the rows; planes: slices of all samples
+    long long parts;     // partial sums of the parameters' gradients
+};
+
+bool on_16(const void* p, int64_t stride, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; }
+
+Plan plan_of(const linrec_group_norm_args& a, bool aligned)
 {
-    NormParams p{};
-    p.x = a.x; p.gate = a.gate; p.dy = a.dy;
-    p.sx = a.x_stride; p.sg = a.gate_stride; p.sdy = a.dy_stride;
-    p.w = a.weight; p.b = a.bias; p.eps = a.eps; p.act = a.activation;
-    p.n = a.nsamples; p.L = a.positions; p.C = (int)a.nchan; p.G = (int)a.groups; p.c = (int)(a.nchan / a.groups);
-    p.stats = reinterpret_cast<float2*>(a.stats);
-    p.y = a.y; p.dx = a.dx; p.dgate = a.dgate;
-    p.part = static_cast<float2*>(a.scratch); p.parts = parts_of(a);
-    p.dw = a.dweight; p.db = a.dbias;
+    Plan p{};
+    const int c = (int)(a.nchan / a.groups);
+    const int size = a.dtype == LINREC_DTYPE_F32 ? 4 : 2;
+    p.V = aligned && c % 8 == 0 && a.nchan * size % 16 == 0 ? 8 : 1;
+    const int pieces = (c + p.V - 1) / p.V;
+    if (a.positions == 1 && pieces <= (p.V == 8 ? 128 : 1024)) {
+        p.rows = true;
+        p.nv = p.V == 8 ? (pieces <= 32 ? 1 : 4) : pieces <= 256 ? 8 : 32;
+        p.lanes = 1;
+        while (p.lanes < 32 && p.lanes * p.nv < pieces) p.lanes *= 2;
+        const int slots = linrec::kNormThreads / p.lanes;
+        p.gb = (int)(a.groups < slots ? a.groups : slots);
+        p.rp = slots / p.gb;
+        p.xblocks = linrec_host::ceil_div_i(a.groups, p.gb);
+        const long long want = kCtas / p.xblocks > 0 ? kCtas / p.xblocks : 1, most = (a.nsamples + p.rp - 1) / p.rp;
+        p.yblocks = p.parts = most < want ? most : want;
+        return p;
+    }
+    const int wide = linrec::kNormThreads * p.V;
+    if (c <= wide) {
+        p.cpb = (int)(a.groups < wide / c ? a.groups : wide / c) * c;
+        p.sub = 1;
+        p.xblocks = linrec_host::ceil_div_i(a.nchan, p.cpb);
+    } else {
+        p.cpb = wide;
+        p.sub = (c + wide - 1) / wide;
+        p.xblocks = (int)a.groups * p.sub;
+    }
+    // slices of at least four rounds of a CTA's threads, and no more CTAs than fill the device once
+    const int threads_per_row = p.cpb / p.V, Y = linrec::kNormThreads / threads_per_row > 0 ? linrec::kNormThreads / threads_per_row : 1;
+    long long want = kCtas / ((long long)p.xblocks * a.nsamples), most = a.positions / (4 * Y);
+    if (want > most) want = most;
+    p.slices = (int)(want < 1 ? 1 : want);
+    p.yblocks = a.nsamples * p.slices;
+    const long long full = kCtas / p.xblocks > 0 ? kCtas / p.xblocks : 1;
+    p.parts = p.yblocks < full ? p.yblocks : full;
     return p;
 }
 
-template <typename ST>
-int run(bool bwd, const NormParams& p, cudaStream_t stream)
+// Room for either alignment: a caller asks for the size before the kernels see the pointers.
+size_t part_bytes(const linrec_group_norm_args& a, const Plan& p) { return (size_t)p.parts * (size_t)a.nchan * sizeof(float2); }
+size_t group_bytes(const linrec_group_norm_args& a, const Plan& p)
 {
-    const dim3 units((unsigned)(p.n * p.G));
-    if (!bwd) return linrec_host::launch("group norm", linrec::norm_fwd_kernel<ST>, units, 256, 0, stream, p);
-    int rc = linrec_host::launch("group norm backward", linrec::norm_bwd_kernel<ST>, units, 256, 0, stream, p);
-    if (rc != LINREC_OK || (!p.dw && !p.db)) return rc;
-    rc = linrec_host::launch("group norm parameters", linrec::norm_param_kernel<ST>,
-                             dim3((unsigned)linrec_host::ceil_div_i(p.C, 128), (unsigned)p.parts), 128, 0, stream, p);
+    return p.rows ? 0 : (size_t)p.yblocks * p.sub * (size_t)a.groups * sizeof(float4);
+}
+
+template <typename ST, int V, bool GATE>
+int run_rows(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)pl.xblocks, (unsigned)pl.yblocks);
+    using Fn = void (*)(const NormParams);
+    constexpr int kShort = V == 8 ? 1 : 8, kLong = V == 8 ? 4 : 32;
+    if (!bwd) {
+        const Fn fn = pl.nv == kShort ? (Fn)linrec::norm_rows_fwd_kernel<ST, V, kShort, GATE> : (Fn)linrec::norm_rows_fwd_kernel<ST, V, kLong, GATE>;
+        return linrec_host::launch("group norm", fn, grid, linrec::kNormThreads, 0, stream, p);
+    }
+    const Fn fn = pl.nv == kShort ? (Fn)linrec::norm_rows_bwd_kernel<ST, V, kShort, GATE> : (Fn)linrec::norm_rows_bwd_kernel<ST, V, kLong, GATE>;
+    const size_t smem = p.part && p.rp > 1 ? (size_t)p.rp * p.gb * p.c * sizeof(float2) : 0;
+    int occ = 0;
+    const int rc = linrec_host::occupancy(reinterpret_cast<const void*>(fn), linrec::kNormThreads, linrec::kNormThreads * V * pl.nv * sizeof(float2), occ);
     if (rc != LINREC_OK) return rc;
-    return linrec_host::launch("group norm parameters", linrec::norm_param_sum_kernel, dim3((unsigned)linrec_host::ceil_div_i(p.C, 32)), 256,
-                               0, stream, (const float2*)p.part, p.parts, p.C, p.dw, p.db);
+    return linrec_host::launch("group norm backward", fn, grid, linrec::kNormThreads, smem, stream, p);
+}
+
+template <typename ST, int V, bool GATE>
+int run_planes(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)(pl.xblocks * pl.yblocks));
+    int rc;
+    if (!bwd) {
+        rc = linrec_host::launch("group norm statistics", linrec::norm_planes_stats_kernel<ST, V>, grid, linrec::kNormThreads, 0, stream, p);
+        if (rc != LINREC_OK) return rc;
+        return linrec_host::launch("group norm", linrec::norm_planes_apply_kernel<ST, V, GATE>, grid, linrec::kNormThreads, 0, stream, p);
+    }
+    rc = linrec_host::launch("group norm sums", linrec::norm_planes_sums_kernel<ST, V, GATE>, dim3((unsigned)(pl.xblocks * pl.parts)), linrec::kNormThreads, 0, stream, p);
+    if (rc != LINREC_OK) return rc;
+    return linrec_host::launch("group norm backward", linrec::norm_planes_dx_kernel<ST, V, GATE>, grid, linrec::kNormThreads, 0, stream, p);
+}
+
+template <typename ST, int V>
+int run(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
+{
+    if (pl.rows) return p.gate ? run_rows<ST, V, true>(bwd, p, pl, stream) : run_rows<ST, V, false>(bwd, p, pl, stream);
+    return p.gate ? run_planes<ST, V, true>(bwd, p, pl, stream) : run_planes<ST, V, false>(bwd, p, pl, stream);
 }
 
 int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
@@ -69,24 +139,52 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     if (!a.x || a.x_stride < a.nchan || (a.gate && a.gate_stride < a.nchan)) return LINREC_ERR_INVALID_ARG;
     if (!bwd && !a.y) return LINREC_ERR_INVALID_ARG;
     if (bwd && (!a.dy || a.dy_stride < a.nchan || !a.dx || !a.stats || (a.gate && !a.dgate))) return LINREC_ERR_INVALID_ARG;
-    if (bwd && (a.dweight || a.dbias) && (!a.scratch || a.scratch_bytes < linrec_b200_group_norm_scratch_size(args)))
-        return LINREC_ERR_INVALID_ARG;
+    const size_t need = linrec_b200_group_norm_scratch_size(args, bwd);
+    if (need && (!a.scratch || a.scratch_bytes < need || reinterpret_cast<uintptr_t>(a.scratch) % 16 != 0)) return LINREC_ERR_WORKSPACE;
     linrec_host::DeviceInfo dev;
     rc = linrec_host::device_facts(dev);
     if (rc != LINREC_OK) return rc;
-    const NormParams p = params_of(a);
-    return a.dtype == LINREC_DTYPE_F32 ? run<float>(bwd, p, stream)
-         : a.dtype == LINREC_DTYPE_BF16 ? run<__nv_bfloat16>(bwd, p, stream) : run<__half>(bwd, p, stream);
+
+    const int size = a.dtype == LINREC_DTYPE_F32 ? 4 : 2;
+    bool aligned = on_16(a.x, a.x_stride, size) && (!a.gate || on_16(a.gate, a.gate_stride, size));
+    if (!bwd) aligned = aligned && on_16(a.y, a.nchan, size);
+    else aligned = aligned && on_16(a.dy, a.dy_stride, size) && on_16(a.dx, a.nchan, size) && (!a.gate || on_16(a.dgate, a.nchan, size));
+    const Plan pl = plan_of(a, aligned);
+    if (!pl.rows && pl.yblocks > 0x7fffffffLL / pl.xblocks) return LINREC_ERR_INVALID_ARG;
+    NormParams p{};
+    p.x = a.x; p.gate = a.gate; p.dy = a.dy;
+    p.sx = a.x_stride; p.sg = a.gate_stride; p.sdy = a.dy_stride;
+    p.w = a.weight; p.b = a.bias; p.eps = a.eps; p.act = a.activation;
+    p.n = a.nsamples; p.L = a.positions; p.C = (int)a.nchan; p.G = (int)a.groups; p.c = (int)(a.nchan / a.groups);
+    p.stats = reinterpret_cast<float2*>(a.stats);
+    p.y = bwd ? nullptr : a.y; p.dx = a.dx; p.dgate = a.dgate;
+    p.lanes = pl.lanes; p.gb = pl.gb; p.rp = pl.rp; p.cpb = pl.cpb; p.sub = pl.sub; p.slices = pl.slices; p.xblocks = pl.xblocks;
+    char* scratch = static_cast<char*>(a.scratch);
+    p.gpart = reinterpret_cast<float4*>(scratch);
+    const bool params = bwd && (a.dweight || a.dbias);
+    p.part = params ? reinterpret_cast<float2*>(scratch + group_bytes(a, pl)) : nullptr;
+    if (a.dtype == LINREC_DTYPE_F32) rc = pl.V == 8 ? run<float, 8>(bwd, p, pl, stream) : run<float, 1>(bwd, p, pl, stream);
+    else if (a.dtype == LINREC_DTYPE_BF16) rc = pl.V == 8 ? run<__nv_bfloat16, 8>(bwd, p, pl, stream) : run<__nv_bfloat16, 1>(bwd, p, pl, stream);
+    else rc = pl.V == 8 ? run<__half, 8>(bwd, p, pl, stream) : run<__half, 1>(bwd, p, pl, stream);
+    if (rc != LINREC_OK || !params) return rc;
+    return linrec_host::launch("group norm parameters", linrec::norm_param_sum_kernel, dim3((unsigned)linrec_host::ceil_div_i(p.C, 32)), 1024, 0,
+                               stream, (const float2*)p.part, (int)pl.parts, p.C, a.dweight, a.dbias);
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args)
+size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args, int bwd)
 {
-    if (check(args) != LINREC_OK) return 0;
-    return (size_t)parts_of(*args) * (size_t)args->nchan * sizeof(float2);
+    if (check(args) != LINREC_OK || args->nsamples == 0 || args->positions == 0 || args->nchan == 0) return 0;
+    size_t most = 0;
+    for (bool aligned : {false, true}) {
+        const Plan p = plan_of(*args, aligned);
+        const size_t n = group_bytes(*args, p) + (bwd && (args->dweight || args->dbias) ? part_bytes(*args, p) : 0);
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 int linrec_b200_group_norm_fwd(const linrec_group_norm_args* args, void* stream) { return launch_norm(false, args, stream); }

@@ -64,8 +64,14 @@ def _describe(x, gate, weight, bias, groups, act, eps, stats):
     return a, (xr, gr)
 
 
-def _call(entry, name, device, a) -> None:
+def _call(bwd, device, a) -> None:
+    entry, name = ((_capi.lib.linrec_b200_group_norm_bwd, "linrec_b200_group_norm_bwd") if bwd else
+                   (_capi.lib.linrec_b200_group_norm_fwd, "linrec_b200_group_norm_fwd"))
     with _on_device(device):
+        need = _capi.lib.linrec_b200_group_norm_scratch_size(ctypes.byref(a), bwd)
+        if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=device)
+            a.scratch, a.scratch_bytes = scratch.data_ptr(), need
         _capi.raise_for(entry(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream), name)
 
 
@@ -75,7 +81,7 @@ def _forward(x, gate, weight, bias, groups, act, eps, want_stats):
     if y.numel():
         a, keep = _describe(x, gate, weight, bias, groups, act, eps, stats)
         a.y = y.data_ptr()
-        _call(_capi.lib.linrec_b200_group_norm_fwd, "linrec_b200_group_norm_fwd", x.device, a)
+        _call(False, x.device, a)
     return y, stats
 
 
@@ -101,11 +107,7 @@ class _GroupNormFn(torch.autograd.Function):
             a, keep = _describe(x, gate, weight, bias, *ctx.args, stats)
             dy, a.dy_stride = _as_rows(dy)
             a.dy, a.dx, a.dgate, a.dweight, a.dbias = dy.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw), _ptr(db)
-            scratch = None
-            if dw is not None or db is not None:
-                scratch = torch.empty(_capi.lib.linrec_b200_group_norm_scratch_size(ctypes.byref(a)), dtype=torch.uint8, device=dev)
-                a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel()
-            _call(_capi.lib.linrec_b200_group_norm_bwd, "linrec_b200_group_norm_bwd", dev, a)
+            _call(True, dev, a)
         return dx, dgate, dw, db, None, None, None
 
 

@@ -54,6 +54,7 @@ def _args(**kw):
     (_capi.ERR_INVALID_ARG, {"nsamples": 1 << 40, "positions": 1 << 40}),
     (_capi.ERR_NOT_IMPLEMENTED, {"activation": 3}),
     (_capi.ERR_NOT_IMPLEMENTED, {"dtype": _capi.DTYPE_F64}),
+    (_capi.ERR_WORKSPACE, {}),
     (_capi.OK, {"nsamples": 0, "x": None}),
 ])
 def test_c_entry_refuses(code, kw):
@@ -65,5 +66,5 @@ def test_c_backward_refuses():
     for missing in full:
         assert _capi.lib.linrec_b200_group_norm_bwd(ctypes.byref(_args(**{**full, missing: None if missing != "dy_stride" else 0})), None) == _capi.ERR_INVALID_ARG
     # parameter gradients need scratch
-    assert _capi.lib.linrec_b200_group_norm_bwd(ctypes.byref(_args(**full, dweight=16)), None) == _capi.ERR_INVALID_ARG
+    assert _capi.lib.linrec_b200_group_norm_bwd(ctypes.byref(_args(**full, dweight=16)), None) == _capi.ERR_WORKSPACE
     assert _capi.lib.linrec_b200_group_norm_bwd(None, None) == _capi.ERR_INVALID_ARG

@@ -56,7 +56,8 @@ def _compare(got, want):
 # (shape, groups): one position per sample, several, whole rows as one group, odd sizes, groups wider than a warp
 SHAPES = [((1, 16), 1), ((3, 64), 2), ((7, 96), 6), ((33, 1000), 8), ((5, 1002), 6), ((4, 4096), 32), ((300, 256), 16), ((2, 8192), 1),
           ((3, 5000), 1), ((9, 17 * 24), 17), ((2, 40, 64), 8), ((3, 7, 5, 48), 3), ((2, 333, 1002), 6), ((1, 2000, 32), 32), ((4, 100, 6), 1),
-          ((65, 2, 130), 2), ((2, 600, 512), 4), ((1, 33, 16384), 2), ((1, 40000), 5)]
+          ((65, 2, 130), 2), ((2, 600, 512), 4), ((1, 33, 16384), 2), ((1, 40000), 5),
+          ((1500, 3, 24), 3), ((5000, 48), 3), ((900, 1), 1)]
 
 
 @pytest.mark.parametrize("shape,groups", SHAPES, ids=lambda s: "x".join(map(str, s)) if isinstance(s, tuple) else f"g{s}")
