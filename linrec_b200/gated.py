@@ -21,13 +21,15 @@ Storage types float32, bfloat16 and float16; gates, products and states are floa
 from __future__ import annotations
 
 import ctypes
+import functools
+import math
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .norm import _as_rows, _check_cuda, _fail, _ptr, _STORAGE, group_norm_act
-from .ops import _DTYPES, _on_device, _workspace
+from .norm import _as_float, _as_rows, _check_cuda, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
+from .ops import _DTYPES, _workspace
 
 __all__ = ["linrec_gated", "linrec_gated_step", "linrec_gated_norm", "linrec_gated_norm_step"]
 
@@ -51,7 +53,7 @@ def _check_operands(inputs, forget, input_gate, decay, decay_scale) -> None:
             _fail("decay must have one value per channel")
         if not decay.is_floating_point():
             _fail("decay must be a floating-point tensor")
-        if not float(decay_scale) > 0.0 or float(decay_scale) == float("inf"):
+        if not 0.0 < decay_scale < math.inf:
             _fail("decay_scale must be positive and finite")
 
 
@@ -71,32 +73,48 @@ def _scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
 
 
 # ---- the scan ----------------------------------------------------------------------------------------
-def _describe(inputs, forget, input_gate, decay, scale, cu, nseq, reverse):
-    """The C struct for one problem, and the row-uniform tensors it points to."""
-    D = inputs.size(-1)
-    nrows = inputs.numel() // D if D else 0
-    a = _capi.GatedArgs()
-    x, a.x_stride = _as_rows(inputs)
-    f, a.forget_stride = _as_rows(forget)
-    a.x, a.forget = x.data_ptr(), f.data_ptr()
-    i = None
-    if input_gate is not None:
-        i, a.input_gate_stride = _as_rows(input_gate)
-        a.input_gate, a.decay, a.decay_scale = i.data_ptr(), decay.data_ptr(), scale
-    a.dtype, a.reverse = _DTYPES[inputs.dtype], int(reverse)
-    a.nseq, a.nrows, a.nchan = nseq, nrows, D
-    if cu is None:
-        a.seqlen = inputs.size(-2)
-    else:
-        a.cu_seqlens, a.cu_is_64 = cu.data_ptr(), int(cu.dtype == torch.int64)
-    return a, (x, f, i)
+@functools.lru_cache(maxsize=4096)
+def _sizes(nseq, seqlen, nrows, D, packed):
+    """Workspace bytes and checkpoint rows of a problem (the same in both passes and for every type)."""
+    a = _capi.GatedArgs(nseq=nseq, seqlen=seqlen, nrows=nrows, nchan=D, cu_seqlens=16 if packed else None)
+    ref = ctypes.byref(a)
+    return _capi.lib.linrec_b200_gated_workspace_size(ref), _capi.lib.linrec_b200_gated_checkpoint_rows(ref)
 
 
-def _run(entry, name, device, a) -> None:
-    with _on_device(device):
-        stream = torch.cuda.current_stream(device).cuda_stream
-        ws = _scratch(device, stream, _capi.lib.linrec_b200_gated_workspace_size(ctypes.byref(a)))
-        _capi.raise_for(entry(ctypes.byref(a), None, ws.data_ptr(), ws.numel(), stream), name)
+class _Problem:
+    """One scan: sizes, and the C struct for its passes."""
+
+    def __init__(self, inputs, forget, input_gate, decay, initial, cu, scale, reverse):
+        shape = inputs.shape
+        self.D = D = shape[-1]
+        self.nrows = inputs.numel() // D if D else 0
+        self.seqlen = shape[-2]
+        if cu is not None:
+            self.nseq = cu.numel() - 1
+            self.lead = (self.nseq,)
+        else:
+            self.lead = shape[:-2]
+            self.nseq = math.prod(self.lead)
+        self.sizes = _sizes(self.nseq, self.seqlen, self.nrows, D, cu is not None) if self.nrows else (0, 0)
+        self.dtype, self.device = inputs.dtype, inputs.device
+        x, sx = _as_rows(inputs)
+        f, sf = _as_rows(forget)
+        i, si = (None, 0) if input_gate is None else _as_rows(input_gate)
+        self.keep = (x, f, i)
+        # (the field order of linrec_gated_args)
+        self.args = _capi.GatedArgs(x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), scale, _DTYPES[self.dtype], reverse,
+                                    cu is not None and cu.dtype == torch.int64, _ptr(cu), self.nseq, self.seqlen, self.nrows, D,
+                                    _ptr(initial))
+
+    def run(self, bwd: bool) -> None:
+        entry, name = ((_capi.lib.linrec_b200_gated_bwd, "linrec_b200_gated_bwd") if bwd else
+                       (_capi.lib.linrec_b200_gated_fwd, "linrec_b200_gated_fwd"))
+
+        def launch(stream):
+            ws = _scratch(self.device, stream, self.sizes[0])
+            _capi.raise_for(entry(ctypes.byref(self.args), None, ws.data_ptr(), ws.numel(), stream), name)
+
+        _on(self.device, launch)
 
 
 def _states_like(other, shape, device, always: bool):
@@ -108,25 +126,18 @@ def _states_like(other, shape, device, always: bool):
 
 
 def _forward(inputs, forget, input_gate, decay, initial, cu, scale, reverse, want_state, want_checkpoints):
-    D = inputs.size(-1)
-    lead = inputs.shape[:-2] if cu is None else (cu.numel() - 1,)
-    nseq = 1
-    for n in lead:
-        nseq *= n
-    a, keep = _describe(inputs, forget, input_gate, decay, scale, cu, nseq, reverse)
-    y = torch.empty(inputs.shape, dtype=inputs.dtype, device=inputs.device)
-    a.y, a.initial_state = y.data_ptr(), _ptr(initial)
-    final = None
+    p = _Problem(inputs, forget, input_gate, decay, initial, cu, scale, reverse)
+    y = torch.empty(inputs.shape, dtype=p.dtype, device=p.device)
+    p.args.y = y.data_ptr()
+    final = checkpoints = None
     if want_state:
-        final = _states_like(initial, (*lead, D), inputs.device, always=cu is not None or inputs.size(-2) == 0)
-        a.final_state = final.data_ptr()
-    checkpoints = None
+        final = _states_like(initial, (*p.lead, p.D), p.device, always=cu is not None or p.seqlen == 0)
+        p.args.final_state = final.data_ptr()
     if want_checkpoints:
-        checkpoints = torch.empty(_capi.lib.linrec_b200_gated_checkpoint_rows(ctypes.byref(a)) * D, dtype=torch.float32,
-                                  device=inputs.device)
-        a.checkpoints = checkpoints.data_ptr()
-    if y.numel():
-        _run(_capi.lib.linrec_b200_gated_fwd, "linrec_b200_gated_fwd", inputs.device, a)
+        checkpoints = torch.empty(p.sizes[1] * p.D, dtype=torch.float32, device=p.device)
+        p.args.checkpoints = checkpoints.data_ptr()
+    if p.nrows:
+        p.run(False)
     return y, final, checkpoints
 
 
@@ -145,29 +156,29 @@ class _GatedFn(torch.autograd.Function):
         inputs, forget, input_gate, decay, initial, cu, checkpoints = ctx.saved_tensors
         if dy is None and dfinal is None:
             return (None,) * 9
-        D, dev = inputs.size(-1), inputs.device
-        nseq = cu.numel() - 1 if cu is not None else (inputs.numel() // (inputs.size(-2) * D) if inputs.numel() else 0)
-        a, keep = _describe(inputs, forget, input_gate, decay, ctx.scale, cu, nseq, ctx.reverse)
+        p = _Problem(inputs, forget, input_gate, decay, initial, cu, ctx.scale, ctx.reverse)
+        a, dev = p.args, p.device
         dy = torch.zeros_like(inputs) if dy is None else dy
         dy, a.dy_stride = _as_rows(dy)
-        a.dy, a.checkpoints, a.initial_state = dy.data_ptr(), checkpoints.data_ptr(), _ptr(initial)
+        a.dy, a.checkpoints = dy.data_ptr(), checkpoints.data_ptr()
         if dfinal is not None:
             dfinal = dfinal.contiguous()
             a.d_final_state = dfinal.data_ptr()
-        dx, df = (torch.empty(inputs.shape, dtype=inputs.dtype, device=dev) for _ in range(2))
+        dx = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
+        df = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
         a.dx, a.dforget = dx.data_ptr(), df.data_ptr()
         di = ddecay = dinitial = scratch = None
         if decay is not None:
-            di = torch.empty(inputs.shape, dtype=inputs.dtype, device=dev)
-            ddecay = torch.empty_like(decay) if inputs.numel() else torch.zeros_like(decay)
-            scratch = torch.empty(_capi.lib.linrec_b200_gated_scratch_size(ctypes.byref(a)), dtype=torch.uint8, device=dev)
+            di = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
+            ddecay = torch.empty_like(decay) if p.nrows else torch.zeros_like(decay)
+            scratch = torch.empty(p.sizes[1] * p.D, dtype=torch.float32, device=dev)
             a.dinput_gate, a.ddecay = di.data_ptr(), ddecay.data_ptr()
-            a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel()
+            a.scratch, a.scratch_bytes = scratch.data_ptr(), scratch.numel() * 4
         if initial is not None and ctx.needs_input_grad[4]:
-            dinitial = _states_like(dfinal, initial.shape, dev, always=cu is not None or inputs.size(-2) == 0)
+            dinitial = _states_like(dfinal, initial.shape, dev, always=cu is not None or p.seqlen == 0)
             a.d_initial_state = dinitial.data_ptr()
-        if inputs.numel():
-            _run(_capi.lib.linrec_b200_gated_bwd, "linrec_b200_gated_bwd", dev, a)
+        if p.nrows:
+            p.run(True)
         return dx, df, di, ddecay, dinitial, None, None, None, None
 
 
@@ -204,11 +215,10 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
             _fail("initial_state must be a floating-point tensor")
     _check_cuda(inputs, forget, input_gate, decay, initial_state, cu_seqlens)
     # casts outside the operator: autograd casts the gradients back
-    decay = None if decay is None else decay.float().contiguous()
-    initial_state = None if initial_state is None else initial_state.float().contiguous()
+    decay, initial_state = _as_float(decay), _as_float(initial_state)
     cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
     args = (inputs, forget, input_gate, decay, initial_state, cu_seqlens, float(decay_scale), bool(reverse), bool(return_state))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+    if _wants_grad(*args[:5]):
         y, final = _GatedFn.apply(*args)
     else:
         y, final, _ = _forward(*args, False)
@@ -245,7 +255,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         if slots.numel() != rows:
             _fail("slots must name one state row per row of the inputs")
     _check_cuda(inputs, forget, input_gate, decay, state, slots)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (inputs, forget, input_gate, decay, state)):
+    if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")
     y = torch.empty((rows, D), dtype=inputs.dtype, device=inputs.device)
     if y.numel() == 0:
@@ -253,15 +263,11 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
     x, sx = _as_rows(inputs)
     f, sf = _as_rows(forget)
     i, si = (None, 0) if input_gate is None else _as_rows(input_gate)
-    decay = None if decay is None else decay.float().contiguous()
+    decay = _as_float(decay)
     slots = None if slots is None else slots.contiguous()
-    with _on_device(inputs.device):
-        stream = torch.cuda.current_stream(inputs.device).cuda_stream
-        rc = _capi.lib.linrec_b200_gated_step(x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), float(decay_scale),
-                                              y.data_ptr(), state.data_ptr(), max(state.stride(0), D), state.size(0),
-                                              _ptr(slots), int(slots is not None and slots.dtype == torch.int64),
-                                              rows, D, _DTYPES[inputs.dtype], stream)
-    _capi.raise_for(rc, "linrec_b200_gated_step")
+    args = (x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), decay_scale, y.data_ptr(), state.data_ptr(), max(state.stride(0), D),
+            state.size(0), _ptr(slots), slots is not None and slots.dtype == torch.int64, rows, D, _DTYPES[inputs.dtype])
+    _on(inputs.device, lambda stream: _capi.raise_for(_capi.lib.linrec_b200_gated_step(*args, stream), "linrec_b200_gated_step"))
     torch.autograd.graph.increment_version(state)
     return y
 

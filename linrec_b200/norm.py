@@ -10,16 +10,18 @@ Storage types float32, bfloat16 and float16; statistics, parameters and their gr
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .ops import _DTYPES, _on_device, _row_layout
+from .ops import _DTYPES, _row_layout
 
 __all__ = ["group_norm_act"]
 
 _STORAGE = (torch.float32, torch.bfloat16, torch.float16)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 
 
@@ -27,61 +29,84 @@ def _fail(what: str):
     raise RuntimeError(f"linrec: {what}")
 
 
-def _check_cuda(*ts) -> None:
-    ts = [t for t in ts if t is not None]
-    if not all(t.is_cuda for t in ts):
+def _check_cuda(first, *others) -> None:
+    if not first.is_cuda:
         _fail("tensors must be CUDA tensors (there is no CPU implementation)")
-    if any(t.device != ts[0].device for t in ts[1:]):
-        _fail("tensors must be on the same device")
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            _fail("tensors must be CUDA tensors (there is no CPU implementation)" if not t.is_cuda else
+                  "tensors must be on the same device")
 
 
 def _as_rows(t: torch.Tensor):
     """(`t` or a dense copy, elements between consecutive rows): the kernels take rows at one stride."""
-    if t.numel() == 0:
+    if t.is_contiguous():
         return t, t.size(-1)
-    layout = _row_layout(t) if t.size(-1) == 1 or t.stride(-1) == 1 else None
+    layout = _row_layout(t) if t.numel() and (t.size(-1) == 1 or t.stride(-1) == 1) else None
     if layout is None:
         t = t.contiguous()
         return t, t.size(-1)
     return t, layout[2]
 
 
+def _as_float(t):
+    """A parameter or state as dense float32 (the cast is autograd's to undo)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.float().contiguous()
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _describe(x, gate, weight, bias, groups, act, eps, stats):
-    a = _capi.GroupNormArgs()
-    C = x.size(-1)
-    xr, a.x_stride = _as_rows(x)
-    gr = None
-    if gate is not None:
-        gr, a.gate_stride = _as_rows(gate)
-    a.x, a.gate, a.weight, a.bias, a.stats = xr.data_ptr(), _ptr(gr), _ptr(weight), _ptr(bias), _ptr(stats)
-    a.eps, a.activation, a.dtype = eps, act, _DTYPES[x.dtype]
-    a.nsamples, a.nchan, a.groups = x.size(0), C, groups
-    a.positions = x.numel() // (x.size(0) * C) if x.numel() else 0
-    return a, (xr, gr)
+def _wants_grad(*ts) -> bool:
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
-def _call(bwd, device, a) -> None:
+def _on(device: torch.device, launch) -> None:
+    """`launch(stream)` with `device` current."""
+    if torch.cuda.current_device() == device.index:
+        launch(_raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            launch(_raw_stream(device.index))
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_size(dtype, nsamples, positions, C, groups, bwd, params) -> int:
+    a = _capi.GroupNormArgs(dtype=dtype, nsamples=nsamples, positions=positions, nchan=C, groups=groups, eps=1.0)
+    a.dweight = 16 if params else None
+    return _capi.lib.linrec_b200_group_norm_scratch_size(ctypes.byref(a), bwd)
+
+
+def _call(bwd, x, gate, weight, bias, groups, act, eps, stats, y=None, dy=None, dx=None, dgate=None, dw=None, db=None) -> None:
+    N, C = x.size(0), x.size(-1)
+    L = x.numel() // (N * C)
+    dtype = _DTYPES[x.dtype]
+    x, sx = _as_rows(x)
+    gate, sg = (None, 0) if gate is None else _as_rows(gate)
+    dy, sdy = (None, 0) if dy is None else _as_rows(dy)
+    need = _scratch_size(dtype, N, L, C, groups, bwd, dw is not None or db is not None)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    # (the field order of linrec_group_norm_args)
+    a = _capi.GroupNormArgs(x.data_ptr(), _ptr(gate), sx, sg, _ptr(weight), _ptr(bias), eps, act, dtype, N, L, C, groups, _ptr(stats), _ptr(y),
+                            _ptr(dy), sdy, _ptr(dx), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(scratch), need)
     entry, name = ((_capi.lib.linrec_b200_group_norm_bwd, "linrec_b200_group_norm_bwd") if bwd else
                    (_capi.lib.linrec_b200_group_norm_fwd, "linrec_b200_group_norm_fwd"))
-    with _on_device(device):
-        need = _capi.lib.linrec_b200_group_norm_scratch_size(ctypes.byref(a), bwd)
-        if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=device)
-            a.scratch, a.scratch_bytes = scratch.data_ptr(), need
-        _capi.raise_for(entry(ctypes.byref(a), torch.cuda.current_stream(device).cuda_stream), name)
+    _on(x.device, lambda stream: _capi.raise_for(entry(ctypes.byref(a), stream), name))
 
 
 def _forward(x, gate, weight, bias, groups, act, eps, want_stats):
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     stats = torch.empty(x.size(0) * groups * 2, dtype=torch.float32, device=x.device) if want_stats else None
     if y.numel():
-        a, keep = _describe(x, gate, weight, bias, groups, act, eps, stats)
-        a.y = y.data_ptr()
-        _call(False, x.device, a)
+        _call(False, x, gate, weight, bias, groups, act, eps, stats, y=y)
     return y, stats
 
 
@@ -104,10 +129,7 @@ class _GroupNormFn(torch.autograd.Function):
         dw = make(weight) if weight is not None and ctx.needs_input_grad[2] else None
         db = make(bias) if bias is not None and ctx.needs_input_grad[3] else None
         if x.numel():
-            a, keep = _describe(x, gate, weight, bias, *ctx.args, stats)
-            dy, a.dy_stride = _as_rows(dy)
-            a.dy, a.dx, a.dgate, a.dweight, a.dbias = dy.data_ptr(), dx.data_ptr(), _ptr(dgate), _ptr(dw), _ptr(db)
-            _call(True, dev, a)
+            _call(True, x, gate, weight, bias, *ctx.args, stats, dy=dy, dx=dx, dgate=dgate, dw=dw, db=db)
         return dx, dgate, dw, db, None, None, None
 
 
@@ -138,9 +160,8 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
         _fail("gate must have the sizes and the dtype of x")
     _check_cuda(x, gate, weight, bias)
-    weight = None if weight is None else weight.float().contiguous()
-    bias = None if bias is None else bias.float().contiguous()
+    weight, bias = _as_float(weight), _as_float(bias)
     args = (x, gate, weight, bias, groups, _ACTIVATIONS[activation], float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if _wants_grad(x, gate, weight, bias):
         return _GroupNormFn.apply(*args)
     return _forward(*args, False)[0]
