@@ -1,5 +1,5 @@
 // Host side of the group norm (include/linrec_b200.h): argument checks and launches.
-#include "norm_kernels.cuh"
+#include "norm_variants.h"
 #include "host.h"
 
 namespace {
@@ -24,7 +24,7 @@ constexpr long long kCtas = 148 * 4;
 struct Plan {
     bool rows;
     int V;               // elements per thread and access: 8 on 16-byte boundaries, else 1
-    int nv;              // rows: pieces per lane
+    int many;            // rows: 0 few, 1 many pieces per lane
     int lanes, gb, rp;   // rows
     int cpb, sub, slices, xblocks;
     long long yblocks;   // rows: CTAs along the rows; planes: slices of all samples
@@ -33,7 +33,7 @@ struct Plan {
 
 bool on_16(const void* p, int64_t stride, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0; }
 
-Plan plan_of(const linrec_group_norm_args& a, bool aligned)
+Plan plan_of(const linrec_group_norm_args& a, bool aligned, bool bwd)
 {
     Plan p{};
     const int c = (int)(a.nchan / a.groups);
@@ -42,14 +42,17 @@ Plan plan_of(const linrec_group_norm_args& a, bool aligned)
     const int pieces = (c + p.V - 1) / p.V;
     if (a.positions == 1 && pieces <= (p.V == 8 ? 128 : 1024)) {
         p.rows = true;
-        p.nv = p.V == 8 ? (pieces <= 32 ? 1 : 4) : pieces <= 256 ? 8 : 32;
+        const int* nv = linrec_variants::kNormPieces[p.V == 8];
+        p.many = pieces > 32 * nv[0];
         p.lanes = 1;
-        while (p.lanes < 32 && p.lanes * p.nv < pieces) p.lanes *= 2;
+        while (p.lanes < 32 && p.lanes * nv[p.many] < pieces) p.lanes *= 2;
         const int slots = linrec::kNormThreads / p.lanes;
         p.gb = (int)(a.groups < slots ? a.groups : slots);
         p.rp = slots / p.gb;
         p.xblocks = linrec_host::ceil_div_i(a.groups, p.gb);
-        const long long want = kCtas / p.xblocks > 0 ? kCtas / p.xblocks : 1, most = (a.nsamples + p.rp - 1) / p.rp;
+        // as many CTAs as are resident at a time, so that all of them take the same number of rows
+        const long long ctas = 148 * (p.V == 1 ? 2 : p.many ? (bwd ? 1 : 2) : bwd ? 3 : 4);
+        const long long want = ctas / p.xblocks > 0 ? ctas / p.xblocks : 1, most = (a.nsamples + p.rp - 1) / p.rp;
         p.yblocks = p.parts = most < want ? most : want;
         return p;
     }
@@ -81,44 +84,29 @@ size_t group_bytes(const linrec_group_norm_args& a, const Plan& p)
     return p.rows ? 0 : (size_t)p.yblocks * p.sub * (size_t)a.groups * sizeof(float4);
 }
 
-template <typename ST, int V, bool GATE>
-int run_rows(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
+int run(bool bwd, const NormParams& p, const Plan& pl, const linrec_variants::NormKernels& k, cudaStream_t stream)
 {
-    const dim3 grid((unsigned)pl.xblocks, (unsigned)pl.yblocks);
-    using Fn = void (*)(const NormParams);
-    constexpr int kShort = V == 8 ? 1 : 8, kLong = V == 8 ? 4 : 32;
-    if (!bwd) {
-        const Fn fn = pl.nv == kShort ? (Fn)linrec::norm_rows_fwd_kernel<ST, V, kShort, GATE> : (Fn)linrec::norm_rows_fwd_kernel<ST, V, kLong, GATE>;
-        return linrec_host::launch("group norm", fn, grid, linrec::kNormThreads, 0, stream, p);
+    if (pl.rows) {
+        const dim3 grid((unsigned)pl.xblocks, (unsigned)pl.yblocks);
+        if (!bwd) return linrec_host::launch("group norm", k.rows_fwd[pl.many], grid, linrec::kNormThreads, 0, stream, p);
+        const linrec_variants::NormFn fn = k.rows_bwd[pl.many];
+        const size_t sums = (size_t)p.rp * p.gb * p.c * sizeof(float2), smem = p.part && (p.rp > 1 || pl.V == 1) ? sums : 0;
+        int occ = 0;      // raises the limit of shared memory to the most the kernel can be asked for
+        const int most = linrec::kNormThreads * pl.V * linrec_variants::kNormPieces[pl.V == 8][pl.many] * (int)sizeof(float2);
+        const int rc = linrec_host::occupancy(reinterpret_cast<const void*>(fn), linrec::kNormThreads, (size_t)most, occ);
+        if (rc != LINREC_OK) return rc;
+        return linrec_host::launch("group norm backward", fn, grid, linrec::kNormThreads, smem, stream, p);
     }
-    const Fn fn = pl.nv == kShort ? (Fn)linrec::norm_rows_bwd_kernel<ST, V, kShort, GATE> : (Fn)linrec::norm_rows_bwd_kernel<ST, V, kLong, GATE>;
-    const size_t smem = p.part && p.rp > 1 ? (size_t)p.rp * p.gb * p.c * sizeof(float2) : 0;
-    int occ = 0;
-    const int rc = linrec_host::occupancy(reinterpret_cast<const void*>(fn), linrec::kNormThreads, linrec::kNormThreads * V * pl.nv * sizeof(float2), occ);
-    if (rc != LINREC_OK) return rc;
-    return linrec_host::launch("group norm backward", fn, grid, linrec::kNormThreads, smem, stream, p);
-}
-
-template <typename ST, int V, bool GATE>
-int run_planes(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
-{
     const dim3 grid((unsigned)(pl.xblocks * pl.yblocks));
     int rc;
     if (!bwd) {
-        rc = linrec_host::launch("group norm statistics", linrec::norm_planes_stats_kernel<ST, V>, grid, linrec::kNormThreads, 0, stream, p);
+        rc = linrec_host::launch("group norm statistics", k.stats, grid, linrec::kNormThreads, 0, stream, p);
         if (rc != LINREC_OK) return rc;
-        return linrec_host::launch("group norm", linrec::norm_planes_apply_kernel<ST, V, GATE>, grid, linrec::kNormThreads, 0, stream, p);
+        return linrec_host::launch("group norm", k.apply, grid, linrec::kNormThreads, 0, stream, p);
     }
-    rc = linrec_host::launch("group norm sums", linrec::norm_planes_sums_kernel<ST, V, GATE>, dim3((unsigned)(pl.xblocks * pl.parts)), linrec::kNormThreads, 0, stream, p);
+    rc = linrec_host::launch("group norm sums", k.sums, dim3((unsigned)(pl.xblocks * pl.parts)), linrec::kNormThreads, 0, stream, p);
     if (rc != LINREC_OK) return rc;
-    return linrec_host::launch("group norm backward", linrec::norm_planes_dx_kernel<ST, V, GATE>, grid, linrec::kNormThreads, 0, stream, p);
-}
-
-template <typename ST, int V>
-int run(bool bwd, const NormParams& p, const Plan& pl, cudaStream_t stream)
-{
-    if (pl.rows) return p.gate ? run_rows<ST, V, true>(bwd, p, pl, stream) : run_rows<ST, V, false>(bwd, p, pl, stream);
-    return p.gate ? run_planes<ST, V, true>(bwd, p, pl, stream) : run_planes<ST, V, false>(bwd, p, pl, stream);
+    return linrec_host::launch("group norm backward", k.dx, grid, linrec::kNormThreads, 0, stream, p);
 }
 
 int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
@@ -149,7 +137,7 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     bool aligned = on_16(a.x, a.x_stride, size) && (!a.gate || on_16(a.gate, a.gate_stride, size));
     if (!bwd) aligned = aligned && on_16(a.y, a.nchan, size);
     else aligned = aligned && on_16(a.dy, a.dy_stride, size) && on_16(a.dx, a.nchan, size) && (!a.gate || on_16(a.dgate, a.nchan, size));
-    const Plan pl = plan_of(a, aligned);
+    const Plan pl = plan_of(a, aligned, bwd);
     if (!pl.rows && pl.yblocks > 0x7fffffffLL / pl.xblocks) return LINREC_ERR_INVALID_ARG;
     NormParams p{};
     p.x = a.x; p.gate = a.gate; p.dy = a.dy;
@@ -163,9 +151,10 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     p.gpart = reinterpret_cast<float4*>(scratch);
     const bool params = bwd && (a.dweight || a.dbias);
     p.part = params ? reinterpret_cast<float2*>(scratch + group_bytes(a, pl)) : nullptr;
-    if (a.dtype == LINREC_DTYPE_F32) rc = pl.V == 8 ? run<float, 8>(bwd, p, pl, stream) : run<float, 1>(bwd, p, pl, stream);
-    else if (a.dtype == LINREC_DTYPE_BF16) rc = pl.V == 8 ? run<__nv_bfloat16, 8>(bwd, p, pl, stream) : run<__nv_bfloat16, 1>(bwd, p, pl, stream);
-    else rc = pl.V == 8 ? run<__half, 8>(bwd, p, pl, stream) : run<__half, 1>(bwd, p, pl, stream);
+    const bool gate = a.gate != nullptr;
+    rc = run(bwd, p, pl, a.dtype == LINREC_DTYPE_F32 ? linrec_variants::norm_kernels_f32(pl.V, gate, a.activation)
+                       : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::norm_kernels_bf16(pl.V, gate, a.activation)
+                                                      : linrec_variants::norm_kernels_f16(pl.V, gate, a.activation), stream);
     if (rc != LINREC_OK || !params) return rc;
     return linrec_host::launch("group norm parameters", linrec::norm_param_sum_kernel, dim3((unsigned)linrec_host::ceil_div_i(p.C, 32)), 1024, 0,
                                stream, (const float2*)p.part, (int)pl.parts, p.C, a.dweight, a.dbias);
@@ -180,7 +169,7 @@ size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args, i
     if (check(args) != LINREC_OK || args->nsamples == 0 || args->positions == 0 || args->nchan == 0) return 0;
     size_t most = 0;
     for (bool aligned : {false, true}) {
-        const Plan p = plan_of(*args, aligned);
+        const Plan p = plan_of(*args, aligned, bwd != 0);
         const size_t n = group_bytes(*args, p) + (bwd && (args->dweight || args->dbias) ? part_bytes(*args, p) : 0);
         most = n > most ? n : most;
     }

@@ -45,87 +45,116 @@ struct NormParams {
     float4* gpart;                // [n][slices * sub][G]: (mean, squares, count) forward, (sum k, sum k xhat) backward
 };
 
-// V elements of one row as floats; `VEC`: the address is on a 16-byte boundary and all V exist.
-template <typename ST, int V>
-__device__ __forceinline__ void norm_load(const void* base, long long offset, float* v)
+// Eight adjacent elements on a 16-byte boundary: as loaded, and as pairs of floats.
+template <typename ST>
+struct Eight {
+    uint4 w[sizeof(ST) / 2];
+    __device__ __forceinline__ void load(const void* base, long long offset)
+    {
+        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const ST*>(base) + offset);
+        w[0] = q[0];
+        if constexpr (sizeof(ST) == 4) w[1] = q[1];
+    }
+    __device__ __forceinline__ void clear()
+    {
+        w[0] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (sizeof(ST) == 4) w[1] = w[0];
+    }
+    __device__ __forceinline__ void get(F2 (&v)[4]) const
+    {
+        if constexpr (sizeof(ST) == 4) {
+            v[0] = f2(__uint_as_float(w[0].x), __uint_as_float(w[0].y)), v[1] = f2(__uint_as_float(w[0].z), __uint_as_float(w[0].w));
+            v[2] = f2(__uint_as_float(w[1].x), __uint_as_float(w[1].y)), v[3] = f2(__uint_as_float(w[1].z), __uint_as_float(w[1].w));
+        } else {
+            v[0] = Two<ST>::get(w[0].x), v[1] = Two<ST>::get(w[0].y), v[2] = Two<ST>::get(w[0].z), v[3] = Two<ST>::get(w[0].w);
+        }
+    }
+};
+template <typename ST>
+__device__ __forceinline__ void store_eight(void* base, long long offset, const F2 (&v)[4])
 {
-    const ST* q = static_cast<const ST*>(base) + offset;
-    if constexpr (V == 8 && sizeof(ST) == 2) {
-        const uint4 w = *reinterpret_cast<const uint4*>(q);
-        Two<ST>::unpack(w.x, v), Two<ST>::unpack(w.y, v + 2), Two<ST>::unpack(w.z, v + 4), Two<ST>::unpack(w.w, v + 6);
-    } else if constexpr (V == 8) {
-        const float4 a = *reinterpret_cast<const float4*>(q), b = *reinterpret_cast<const float4*>(q + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    uint4* q = reinterpret_cast<uint4*>(static_cast<ST*>(base) + offset);
+    if constexpr (sizeof(ST) == 4) {
+        const float2 a = f2_get(v[0]), b = f2_get(v[1]), c = f2_get(v[2]), d = f2_get(v[3]);
+        q[0] = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+        q[1] = make_uint4(__float_as_uint(c.x), __float_as_uint(c.y), __float_as_uint(d.x), __float_as_uint(d.y));
     } else {
-        v[0] = to_f32<ST>(*q);
+        q[0] = make_uint4(Two<ST>::put(v[0]), Two<ST>::put(v[1]), Two<ST>::put(v[2]), Two<ST>::put(v[3]));
     }
 }
-template <typename ST, int V>
-__device__ __forceinline__ void norm_store(void* base, long long offset, const float* v)
-{
-    ST* q = static_cast<ST*>(base) + offset;
-    if constexpr (V == 8 && sizeof(ST) == 2) {
-        *reinterpret_cast<uint4*>(q) = make_uint4(Two<ST>::pack(v), Two<ST>::pack(v + 2), Two<ST>::pack(v + 4), Two<ST>::pack(v + 6));
-    } else if constexpr (V == 8) {
-        reinterpret_cast<float4*>(q)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(q)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *q = from_f32<ST>(v[0]);
-    }
-}
-template <int V>
-__device__ __forceinline__ void norm_param(const float* p, int ch, float missing, float* v)
+__device__ __forceinline__ void param_eight(const float* p, int ch, float missing, F2 (&v)[4])
 {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = p ? __ldg(p + ch + e) : missing;
+    for (int e = 0; e < 4; ++e) v[e] = p ? f2(__ldg(p + ch + 2 * e), __ldg(p + ch + 2 * e + 1)) : f2(missing);
+}
+__device__ __forceinline__ float f2_sum(F2 a)
+{
+    const float2 v = f2_get(a);
+    return v.x + v.y;
 }
 
-// act(v) and its derivative.
-template <bool FAST>
-__device__ __forceinline__ void activate(int act, float v, float& value, float& slope)
+// act(v), and act(v) with its derivative, of two elements.
+template <bool FAST, int ACT>
+__device__ __forceinline__ F2 activated2(F2 v)
 {
-    if (act == kActNone) {
+    if (ACT == kActNone) return v;
+    const F2 p = logistic2<FAST>(v);
+    return ACT == kActSilu ? f2_mul(v, p) : p;
+}
+template <bool FAST, int ACT>
+__device__ __forceinline__ void activate2(F2 v, F2& value, F2& slope)
+{
+    if (ACT == kActNone) {
         value = v;
-        slope = 1.0f;
+        slope = f2(1.0f);
         return;
     }
-    float p, n;
-    logistic_pair<FAST>(v, p, n);
-    if (act == kActSilu) {
-        value = v * p;
-        slope = p * fmaf(v, n, 1.0f);
+    if (ACT == kActSilu) {
+        // p (1 + v s(-v)); s(-v) as 1 - p: where that loses its bits it is next to nothing beside 1/v
+        const F2 p = logistic2<FAST>(v), n = f2_fma(p, f2(-1.0f), f2(1.0f));
+        value = f2_mul(v, p);
+        slope = f2_fma(value, n, p);
     } else {
-        value = p;
-        slope = p * n;
+        F2 n;
+        logistic_pair2<FAST>(v, value, n);
+        slope = f2_mul(value, n);
     }
 }
-template <bool FAST>
-__device__ __forceinline__ float activated(int act, float v)
-{
-    if (act == kActNone) return v;
-    const float p = logistic<FAST>(v);
-    // (minus infinity times a logistic value of zero is taken as it is: NaN, as in v * s(v))
-    return act == kActSilu ? v * p : p;
-}
 
-// One element forward.
-template <bool FAST, bool GATE>
-__device__ __forceinline__ float norm_value(int act, float x, float gate, float mean, float inv, float w, float b)
+// One element forward and backward (rows that are off 16-byte boundaries).
+template <bool FAST, bool GATE, int ACT>
+__device__ __forceinline__ float norm_value(float x, float gate, float mean, float inv, float w, float b)
 {
     const float z = fmaf((x - mean) * inv, w, b);
-    return GATE ? z * activated<FAST>(act, gate) : activated<FAST>(act, z);
+    const float a = f2_get(activated2<FAST, ACT>(f2(GATE ? gate : z))).x;
+    return GATE ? z * a : a;
 }
-// One element backward: xhat, the gradient dz of z, and the gate's gradient.
-template <bool FAST, bool GATE>
-__device__ __forceinline__ void norm_gradient(int act, float x, float gate, float dy, float2 st, float w, float b, float& xhat, float& dz,
-                                              float& dgate)
+template <bool FAST, bool GATE, int ACT>
+__device__ __forceinline__ void norm_gradient(float x, float gate, float dy, float2 st, float w, float b, float& xhat, float& dz, float& dgate)
 {
     xhat = (x - st.x) * st.y;
     const float z = fmaf(xhat, w, b);
-    float v, slope;
-    activate<FAST>(act, GATE ? gate : z, v, slope);
+    F2 v2, s2;
+    activate2<FAST, ACT>(f2(GATE ? gate : z), v2, s2);
+    const float v = f2_get(v2).x, slope = f2_get(s2).x;
     dz = dy * (GATE ? v : slope);
     dgate = GATE ? dy * z * slope : 0.0f;
+}
+// Eight elements backward: xhat and the gradient dz of z, and the gate's gradient.
+template <bool FAST, bool GATE, int ACT>
+__device__ __forceinline__ void norm_gradient8(const F2 (&x)[4], const F2 (&gate)[4], const F2 (&dy)[4], float2 st, const F2 (&w)[4],
+                                               const F2 (&b)[4], F2 (&xhat)[4], F2 (&dz)[4], F2 (&dgate)[4])
+{
+    const F2 inv = f2(st.y), off = f2(-st.x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        xhat[e] = f2_mul(f2_add(x[e], off), inv);
+        const F2 z = f2_fma(xhat[e], w[e], b[e]);
+        F2 v, slope;
+        activate2<FAST, ACT>(GATE ? gate[e] : z, v, slope);
+        dz[e] = f2_mul(dy[e], GATE ? v : slope);
+        if (GATE) dgate[e] = f2_mul(f2_mul(dy[e], z), slope);
+    }
 }
 
 // ---- rows -----------------------------------------------------------------------------------------------
@@ -151,163 +180,277 @@ __device__ __forceinline__ NormSlot norm_slot(const NormParams& p)
     return s;
 }
 
-// NV pieces of V elements per lane.  The next row's operands are requested before this row is worked on.
-template <typename ST, int V, int NV, bool GATE>
-__global__ void __launch_bounds__(kNormThreads) norm_rows_fwd_kernel(const NormParams p)
+// NV pieces of eight elements per lane.  With one piece the next row's operands are requested before this row
+// is worked on, as they come (four registers for eight elements).
+template <typename ST, int NV, bool GATE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     const NormSlot s = norm_slot(p);
     ptx::grid_dependency_wait();
     bool have[NV];
     int ch[NV];
-    float w[NV][V], b[NV][V];
+    F2 w[NV][4], b[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int e = (i * p.lanes + s.lane) * V;
+        const int e = (i * p.lanes + s.lane) * 8;
         have[i] = s.active && e < p.c;
         ch[i] = s.g * p.c + e;
         if (have[i]) {
-            norm_param<V>(p.w, ch[i], 1.0f, w[i]);
-            norm_param<V>(p.b, ch[i], 0.0f, b[i]);
+            param_eight(p.w, ch[i], 1.0f, w[i]);
+            param_eight(p.b, ch[i], 0.0f, b[i]);
         }
     }
     const long long step = (long long)gridDim.y * p.rp;
     long long n = (long long)blockIdx.y * p.rp + s.r;
     const float count = 1.0f / (float)p.c;
-    float x[NV][V], gt[NV][V];
-    auto fetch = [&](long long row, float (&to)[NV][V], float (&tg)[NV][V]) {
+    Eight<ST> rx[NV], rg[NV];
+    auto fetch = [&](long long row) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool in = have[i] && row < p.n;
-#pragma unroll
-            for (int e = 0; e < V; ++e) to[i][e] = tg[i][e] = 0.0f;
-            if (in) norm_load<ST, V>(p.x, row * p.sx + ch[i], to[i]);
-            if (GATE && in) norm_load<ST, V>(p.gate, row * p.sg + ch[i], tg[i]);
+            rx[i].clear();
+            if (have[i] && row < p.n) {
+                rx[i].load(p.x, row * p.sx + ch[i]);
+                if (GATE) rg[i].load(p.gate, row * p.sg + ch[i]);
+            }
         }
     };
-    fetch(n, x, gt);
+    fetch(n);
     // (all threads of a CTA take the same number of turns: the shuffles need whole warps)
     for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
-        float nx[NV][V], ng[NV][V];
-        fetch(n + step, nx, ng);
-        float sum = 0.0f;
+        F2 x[NV][4];
+        Eight<ST> gate[NV];
+        F2 sum = f2(0.0f);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            rx[i].get(x[i]);
+            if (GATE) gate[i] = rg[i];
 #pragma unroll
-            for (int e = 0; e < V; ++e) sum += x[i][e];
-        const float mean = lanes_sum(sum, p.lanes) * count;
-        float sq = 0.0f;
+            for (int e = 0; e < 4; ++e) sum = f2_add(sum, x[i][e]);
+        }
+        fetch(n + step);
+        const float mean = lanes_sum(f2_sum(sum), p.lanes) * count;
+        F2 sq = f2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (have[i])
 #pragma unroll
-                for (int e = 0; e < V; ++e) sq = fmaf(x[i][e] - mean, x[i][e] - mean, sq);
-        const float inv = 1.0f / sqrtf(fmaf(lanes_sum(sq, p.lanes), count, p.eps));
+                for (int e = 0; e < 4; ++e) {
+                    x[i][e] = f2_add(x[i][e], f2(-mean));
+                    sq = f2_fma(x[i][e], x[i][e], sq);
+                }
+        const float inv = 1.0f / sqrtf(fmaf(lanes_sum(f2_sum(sq), p.lanes), count, p.eps));
         if (n < p.n) {
             if (p.stats && s.lane == 0 && s.active) p.stats[n * p.G + s.g] = make_float2(mean, inv);
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (have[i]) {
-                    float y[V];
+                    F2 gt[4], y[4];
+                    if (GATE) gate[i].get(gt);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) y[e] = norm_value<kFast, GATE>(p.act, x[i][e], gt[i][e], mean, inv, w[i][e], b[i][e]);
-                    norm_store<ST, V>(p.y, n * p.C + ch[i], y);
+                    for (int e = 0; e < 4; ++e) {
+                        const F2 z = f2_fma(f2_mul(x[i][e], f2(inv)), w[i][e], b[i][e]);
+                        y[e] = GATE ? f2_mul(z, activated2<kFast, ACT>(gt[e])) : activated2<kFast, ACT>(z);
+                    }
+                    store_eight<ST>(p.y, n * p.C + ch[i], y);
                 }
         }
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[i][e] = nx[i][e], gt[i][e] = ng[i][e];
     }
 }
 
-template <typename ST, int V, int NV, bool GATE>
-__global__ void __launch_bounds__(kNormThreads) norm_rows_bwd_kernel(const NormParams p)
+// One element per access, NV per lane (rows off 16-byte boundaries, or groups that are not whole sixteens of bytes).
+template <typename ST, int NV, bool GATE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_fwd_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
-    extern __shared__ __align__(16) float2 norm_sums[];      // [gb * c][rp] sums of (dz xhat, dz), if rp > 1
+    const NormSlot s = norm_slot(p);
+    ptx::grid_dependency_wait();
+    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + p.lanes - 1) / p.lanes : 0;      // elements of this lane
+    const long long step = (long long)gridDim.y * p.rp;
+    long long n = (long long)blockIdx.y * p.rp + s.r;
+    const float count = 1.0f / (float)p.c;
+    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
+        const bool row = n < p.n;
+        const ST* x = static_cast<const ST*>(p.x) + n * p.sx + ch0;
+        const ST* gate = static_cast<const ST*>(p.gate) + n * p.sg + ch0;
+        float v[NV], sum = 0.0f, sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = row && i < mine ? to_f32<ST>(x[i * p.lanes + s.lane]) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sum += v[i];
+        const float mean = lanes_sum(sum, p.lanes) * count;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sq = i < mine ? fmaf(v[i] - mean, v[i] - mean, sq) : sq;
+        const float inv = 1.0f / sqrtf(fmaf(lanes_sum(sq, p.lanes), count, p.eps));
+        if (!row) continue;
+        if (p.stats && s.lane == 0 && s.active) p.stats[n * p.G + s.g] = make_float2(mean, inv);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (i < mine) {
+                const int e = i * p.lanes + s.lane, ch = ch0 + e;
+                static_cast<ST*>(p.y)[n * p.C + ch] = from_f32<ST>(norm_value<kFast, GATE, ACT>(
+                    v[i], GATE ? to_f32<ST>(gate[e]) : 0.0f, mean, inv, p.w ? __ldg(p.w + ch) : 1.0f, p.b ? __ldg(p.b + ch) : 0.0f));
+            }
+    }
+}
+
+// The sums of (dz xhat, dz) of a CTA's rows, which lie as [rp][channels of the CTA] in shared memory, to the parts.
+__device__ __forceinline__ void norm_rows_leave(const NormParams& p, const float2* sums)
+{
+    __syncthreads();
+    const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
+    for (int i = (int)threadIdx.x; i < nch; i += kNormThreads) {
+        float2 v = sums[i];
+        for (int r = 1; r < p.rp; ++r) {
+            const float2 u = sums[r * nch + i];
+            v.x += u.x;
+            v.y += u.y;
+        }
+        p.part[(long long)blockIdx.y * p.C + c0 + i] = v;
+    }
+}
+
+template <typename ST, int NV, bool GATE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, NV == 1 ? 3 : 1) norm_rows_bwd_kernel(const NormParams p)
+{
+    constexpr bool kFast = sizeof(ST) == 2;
+    extern __shared__ __align__(16) float2 norm_sums[];
     const NormSlot s = norm_slot(p);
     ptx::grid_dependency_wait();
     bool have[NV];
     int ch[NV];
-    float w[NV][V], b[NV][V], dw[NV][V], db[NV][V];
+    F2 w[NV][4], b[NV][4], dw[NV][4], db[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int e0 = (i * p.lanes + s.lane) * V;
+        const int e0 = (i * p.lanes + s.lane) * 8;
         have[i] = s.active && e0 < p.c;
         ch[i] = s.g * p.c + e0;
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[i][e] = b[i][e] = dw[i][e] = db[i][e] = 0.0f;
+        for (int e = 0; e < 4; ++e) w[i][e] = b[i][e] = dw[i][e] = db[i][e] = f2(0.0f);
         if (have[i]) {
-            norm_param<V>(p.w, ch[i], 1.0f, w[i]);
-            norm_param<V>(p.b, ch[i], 0.0f, b[i]);
+            param_eight(p.w, ch[i], 1.0f, w[i]);
+            param_eight(p.b, ch[i], 0.0f, b[i]);
         }
     }
+    const long long step = (long long)gridDim.y * p.rp;
+    const float count = 1.0f / (float)p.c;
+    long long n = (long long)blockIdx.y * p.rp + s.r;
+    Eight<ST> rx[NV], rg[NV], rd[NV];
+    float2 rst = make_float2(0.0f, 0.0f);
+    auto fetch = [&](long long row) {
+        if (row < p.n && s.active) rst = p.stats[row * p.G + s.g];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (have[i] && row < p.n) {
+                rx[i].load(p.x, row * p.sx + ch[i]);
+                rd[i].load(p.dy, row * p.sdy + ch[i]);
+                if (GATE) rg[i].load(p.gate, row * p.sg + ch[i]);
+            } else {
+                rx[i].clear(), rd[i].clear(), rg[i].clear();
+            }
+        }
+    };
+    fetch(n);
+    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
+        const bool row = n < p.n;
+        const float2 st = rst;
+        F2 xhat[NV][4], k[NV][4], s1 = f2(0.0f), s2 = f2(0.0f);
+        Eight<ST> cx[NV], cg[NV], cd[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) cx[i] = rx[i], cg[i] = rg[i], cd[i] = rd[i];
+        fetch(n + step);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            F2 x[4], gt[4], dy[4], dg[4];
+            cx[i].get(x);
+            cd[i].get(dy);
+            if (GATE) cg[i].get(gt);
+            norm_gradient8<kFast, GATE, ACT>(x, gt, dy, st, w[i], b[i], xhat[i], k[i], dg);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // (rows and pieces that do not exist have dy = 0 and therefore add nothing)
+                dw[i][e] = f2_fma(k[i][e], xhat[i][e], dw[i][e]);
+                db[i][e] = f2_add(db[i][e], k[i][e]);
+                k[i][e] = f2_mul(k[i][e], w[i][e]);
+                s1 = f2_add(s1, k[i][e]);
+                s2 = f2_fma(k[i][e], xhat[i][e], s2);
+            }
+            if (GATE && have[i] && row) store_eight<ST>(p.dgate, n * p.C + ch[i], dg);
+        }
+        const float m1 = lanes_sum(f2_sum(s1), p.lanes) * count, m2 = lanes_sum(f2_sum(s2), p.lanes) * count;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (have[i] && row) {
+                F2 dx[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dx[e] = f2_mul(f2_fma(xhat[i][e], f2(-m2), f2_add(k[i][e], f2(-m1))), f2(st.y));
+                store_eight<ST>(p.dx, n * p.C + ch[i], dx);
+            }
+    }
+    if (!p.part) return;
+    const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
+    float2* out = p.rp == 1 ? p.part + (long long)blockIdx.y * p.C : norm_sums + s.r * nch - c0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (have[i])
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 a = f2_get(dw[i][e]), c = f2_get(db[i][e]);
+                out[ch[i] + 2 * e] = make_float2(a.x, c.x);
+                out[ch[i] + 2 * e + 1] = make_float2(a.y, c.y);
+            }
+    if (p.rp > 1) norm_rows_leave(p, norm_sums);
+}
+
+// One element per access; the sums of (dz xhat, dz) live in shared memory, every thread at its own places.
+template <typename ST, int NV, bool GATE, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_bwd_kernel(const NormParams p)
+{
+    constexpr bool kFast = sizeof(ST) == 2;
+    extern __shared__ __align__(16) float2 norm_sums[];
+    const NormSlot s = norm_slot(p);
+    ptx::grid_dependency_wait();
+    const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
+    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + p.lanes - 1) / p.lanes : 0;
+    float2* sums = norm_sums + s.r * nch + ch0 - c0 + s.lane;
+    if (p.part)
+        for (int i = 0; i < mine; ++i) sums[i * p.lanes] = make_float2(0.0f, 0.0f);
     const long long step = (long long)gridDim.y * p.rp;
     const float count = 1.0f / (float)p.c;
     long long n = (long long)blockIdx.y * p.rp + s.r;
     for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
         const bool row = n < p.n;
         const float2 st = row && s.active ? p.stats[n * p.G + s.g] : make_float2(0.0f, 0.0f);
-        float xhat[NV][V], k[NV][V], s1 = 0.0f, s2 = 0.0f;
+        float xhat[NV], k[NV], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) xhat[i][e] = k[i][e] = 0.0f;
-            if (have[i] && row) {
-                float x[V], gt[V], dy[V], dg[V];
-                norm_load<ST, V>(p.x, n * p.sx + ch[i], x);
-                norm_load<ST, V>(p.dy, n * p.sdy + ch[i], dy);
-                if (GATE) norm_load<ST, V>(p.gate, n * p.sg + ch[i], gt);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    float dz;
-                    norm_gradient<kFast, GATE>(p.act, x[e], GATE ? gt[e] : 0.0f, dy[e], st, w[i][e], b[i][e], xhat[i][e], dz, dg[e]);
-                    dw[i][e] = fmaf(dz, xhat[i][e], dw[i][e]);
-                    db[i][e] += dz;
-                    k[i][e] = dz * w[i][e];
-                    s1 += k[i][e];
-                    s2 = fmaf(k[i][e], xhat[i][e], s2);
+            xhat[i] = k[i] = 0.0f;
+            if (row && i < mine) {
+                const int ch = ch0 + i * p.lanes + s.lane;
+                const float w = p.w ? __ldg(p.w + ch) : 1.0f;
+                float dz, dg;
+                norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[n * p.sx + ch]),
+                                                GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[n * p.sg + ch]) : 0.0f,
+                                                to_f32<ST>(static_cast<const ST*>(p.dy)[n * p.sdy + ch]), st, w, p.b ? __ldg(p.b + ch) : 0.0f,
+                                                xhat[i], dz, dg);
+                if (p.part) {
+                    float2 v = sums[i * p.lanes];
+                    v.x = fmaf(dz, xhat[i], v.x);
+                    v.y += dz;
+                    sums[i * p.lanes] = v;
                 }
-                if (GATE) norm_store<ST, V>(p.dgate, n * p.C + ch[i], dg);
+                k[i] = dz * w;
+                s1 += k[i];
+                s2 = fmaf(k[i], xhat[i], s2);
+                if (GATE) static_cast<ST*>(p.dgate)[n * p.C + ch] = from_f32<ST>(dg);
             }
         }
         const float m1 = lanes_sum(s1, p.lanes) * count, m2 = lanes_sum(s2, p.lanes) * count;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (have[i] && row) {
-                float dx[V];
-#pragma unroll
-                for (int e = 0; e < V; ++e) dx[e] = st.y * (k[i][e] - m1 - xhat[i][e] * m2);
-                norm_store<ST, V>(p.dx, n * p.C + ch[i], dx);
-            }
+            if (row && i < mine) static_cast<ST*>(p.dx)[n * p.C + ch0 + i * p.lanes + s.lane] = from_f32<ST>(st.y * (k[i] - m1 - xhat[i] * m2));
     }
-    if (!p.part) return;
-    float2* out = p.part + (long long)blockIdx.y * p.C;
-    if (p.rp == 1) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (have[i])
-#pragma unroll
-                for (int e = 0; e < V; ++e) out[ch[i] + e] = make_float2(dw[i][e], db[i][e]);
-        return;
-    }
-    const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (have[i])
-#pragma unroll
-            for (int e = 0; e < V; ++e) norm_sums[s.r * nch + ch[i] + e - c0] = make_float2(dw[i][e], db[i][e]);
-    __syncthreads();
-    for (int i = (int)threadIdx.x; i < nch; i += kNormThreads) {
-        float2 v = norm_sums[i];
-        for (int r = 1; r < p.rp; ++r) {
-            const float2 u = norm_sums[r * nch + i];
-            v.x += u.x;
-            v.y += u.y;
-        }
-        out[c0 + i] = v;
-    }
+    if (p.part) norm_rows_leave(p, norm_sums);
 }
 
 // ---- planes -----------------------------------------------------------------------------------------------
@@ -407,61 +550,91 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_stats_kernel(const N
     ptx::grid_dependency_wait();
     const int ch = k.c0 + k.tx * V;
     float4 mine = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (k.active && k.l0 + k.ty < k.l1) {
+    long long l = k.l0 + k.ty;
+    if (k.active && l < k.l1) {
         const long long row0 = k.n * p.L;
-        float v[V], about = 0.0f, s = 0.0f, q = 0.0f;
-        long long l = k.l0 + k.ty;
-        norm_load<ST, V>(p.x, (row0 + l) * p.sx + ch, v);
-        about = v[0];
-        float count = 0.0f;
+        float about, s, q, count = (float)V * (float)((k.l1 - l + k.Y - 1) / k.Y);
+        about = to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]);
+        if constexpr (V == 8) {
+            const F2 off = f2(-about);
+            F2 s2 = f2(0.0f), q2 = f2(0.0f);
 #pragma unroll 4
-        for (; l < k.l1; l += k.Y) {
-            norm_load<ST, V>(p.x, (row0 + l) * p.sx + ch, v);
+            for (; l < k.l1; l += k.Y) {
+                Eight<ST> r;
+                F2 v[4];
+                r.load(p.x, (row0 + l) * p.sx + ch);
+                r.get(v);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float d = v[e] - about;
+                for (int e = 0; e < 4; ++e) {
+                    const F2 d = f2_add(v[e], off);
+                    s2 = f2_add(s2, d);
+                    q2 = f2_fma(d, d, q2);
+                }
+            }
+            s = f2_sum(s2), q = f2_sum(q2);
+        } else {
+            s = q = 0.0f;
+#pragma unroll 4
+            for (; l < k.l1; l += k.Y) {
+                const float d = to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]) - about;
                 s += d;
                 q = fmaf(d, d, q);
             }
-            count += (float)V;
         }
-        mine = make_float4(about + s / count, fmaxf(fmaf(-s / count, s, q), 0.0f), count, 0.0f);
-        if (!(q == q)) mine.y = q;      // (fmaxf drops NaN)
+        const float m = s / count, squares = fmaf(-m, s, q);
+        mine = make_float4(about + m, squares < 0.0f ? 0.0f : squares, count, 0.0f);
     }
-    norm_leave<V>(p, k, mine, shared, norm_merge);
+    norm_leave<V>(p, k, mine, shared, [](float4 a, float4 b) { return norm_merge(a, b); });
 }
 
-template <typename ST, int V, bool GATE>
+template <typename ST, int V, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads) norm_planes_apply_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     __shared__ float2 st[kNormThreads * V];
     const NormBlock k = norm_block<V>(p, blockIdx.x / (unsigned)p.xblocks, (int)blockIdx.x % p.xblocks);
     ptx::grid_dependency_wait();
-    norm_collect(p, k, st, norm_merge, [&](float4 v) { return make_float2(v.x, 1.0f / sqrtf(v.y / v.z + p.eps)); });
+    norm_collect(p, k, st, [](float4 a, float4 b) { return norm_merge(a, b); },
+                 [&](float4 v) { return make_float2(v.x, 1.0f / sqrtf(v.y / v.z + p.eps)); });
     if (!k.active) return;
     const int ch = k.c0 + k.tx * V;
     const float2 mine = st[k.groups > 1 ? k.tx * V / p.c : 0];
-    float w[V], b[V];
-    norm_param<V>(p.w, ch, 1.0f, w);
-    norm_param<V>(p.b, ch, 0.0f, b);
     const long long row0 = k.n * p.L;
+    if constexpr (V == 8) {
+        F2 w[4], b[4];
+        param_eight(p.w, ch, 1.0f, w);
+        param_eight(p.b, ch, 0.0f, b);
 #pragma unroll 2
-    for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
-        float x[V], gt[V], y[V];
-        norm_load<ST, V>(p.x, (row0 + l) * p.sx + ch, x);
-        if (GATE) norm_load<ST, V>(p.gate, (row0 + l) * p.sg + ch, gt);
+        for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
+            Eight<ST> rx, rg;
+            F2 x[4], gt[4], y[4];
+            rx.load(p.x, (row0 + l) * p.sx + ch);
+            if (GATE) rg.load(p.gate, (row0 + l) * p.sg + ch);
+            rx.get(x);
+            if (GATE) rg.get(gt);
 #pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = norm_value<kFast, GATE>(p.act, x[e], GATE ? gt[e] : 0.0f, mine.x, mine.y, w[e], b[e]);
-        norm_store<ST, V>(p.y, (row0 + l) * p.C + ch, y);
+            for (int e = 0; e < 4; ++e) {
+                const F2 z = f2_fma(f2_mul(f2_add(x[e], f2(-mine.x)), f2(mine.y)), w[e], b[e]);
+                y[e] = GATE ? f2_mul(z, activated2<kFast, ACT>(gt[e])) : activated2<kFast, ACT>(z);
+            }
+            store_eight<ST>(p.y, (row0 + l) * p.C + ch, y);
+        }
+    } else {
+        const float w = p.w ? p.w[ch] : 1.0f, b = p.b ? p.b[ch] : 0.0f;
+#pragma unroll 4
+        for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y)
+            static_cast<ST*>(p.y)[(row0 + l) * p.C + ch] = from_f32<ST>(norm_value<kFast, GATE, ACT>(
+                to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
+                GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f, mine.x, mine.y, w, b));
     }
 }
 
 // Sums of k and k xhat per slice and group, and of (dz xhat, dz) per slice and channel.
-template <typename ST, int V, bool GATE>
+template <typename ST, int V, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
+    constexpr int H = V == 8 ? 4 : 1;
     __shared__ float4 shared[kNormThreads];
     __shared__ float2 chan[kNormThreads * V];
     const int xblock = (int)blockIdx.x % p.xblocks;
@@ -469,46 +642,76 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const No
     NormBlock k = norm_block<V>(p, blockIdx.x / (unsigned)p.xblocks, xblock);
     ptx::grid_dependency_wait();
     const int ch = k.c0 + k.tx * V;
-    float dw[V], db[V], w[V], b[V];
+    F2 dw[H], db[H], w[4], b[4];
 #pragma unroll
-    for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.0f;
+    for (int e = 0; e < H; ++e) dw[e] = db[e] = f2(0.0f);
     if (k.active) {
-        norm_param<V>(p.w, ch, 1.0f, w);
-        norm_param<V>(p.b, ch, 0.0f, b);
+        if constexpr (V == 8) {
+            param_eight(p.w, ch, 1.0f, w);
+            param_eight(p.b, ch, 0.0f, b);
+        } else {
+            w[0] = f2(p.w ? p.w[ch] : 1.0f);
+            b[0] = f2(p.b ? p.b[ch] : 0.0f);
+        }
     }
     // a CTA takes several samples where there are many: their channel sums share one part
     for (long long item = blockIdx.x / (unsigned)p.xblocks; item < items; item += turns) {
         k = norm_block<V>(p, item, xblock);
-        float s1 = 0.0f, s2 = 0.0f;
+        F2 s1 = f2(0.0f), s2 = f2(0.0f);
         if (k.active) {
             const float2 st = p.stats[k.n * p.G + ch / p.c];
             const long long row0 = k.n * p.L;
 #pragma unroll 2
             for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
-                float x[V], gt[V], dy[V];
-                norm_load<ST, V>(p.x, (row0 + l) * p.sx + ch, x);
-                norm_load<ST, V>(p.dy, (row0 + l) * p.sdy + ch, dy);
-                if (GATE) norm_load<ST, V>(p.gate, (row0 + l) * p.sg + ch, gt);
+                if constexpr (V == 8) {
+                    Eight<ST> rx, rg, rd;
+                    F2 x[4], gt[4], dy[4], xhat[4], dz[4], dg[4];
+                    rx.load(p.x, (row0 + l) * p.sx + ch);
+                    rd.load(p.dy, (row0 + l) * p.sdy + ch);
+                    if (GATE) rg.load(p.gate, (row0 + l) * p.sg + ch);
+                    rx.get(x);
+                    rd.get(dy);
+                    if (GATE) rg.get(gt);
+                    norm_gradient8<kFast, GATE, ACT>(x, gt, dy, st, w, b, xhat, dz, dg);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
+                    for (int e = 0; e < 4; ++e) {
+                        const F2 t = f2_mul(dz[e], w[e]);
+                        s1 = f2_add(s1, t);
+                        s2 = f2_fma(t, xhat[e], s2);
+                        dw[e] = f2_fma(dz[e], xhat[e], dw[e]);
+                        db[e] = f2_add(db[e], dz[e]);
+                    }
+                } else {
                     float xhat, dz, dg;
-                    norm_gradient<kFast, GATE>(p.act, x[e], GATE ? gt[e] : 0.0f, dy[e], st, w[e], b[e], xhat, dz, dg);
-                    const float t = dz * w[e];
-                    s1 += t;
-                    s2 = fmaf(t, xhat, s2);
-                    dw[e] = fmaf(dz, xhat, dw[e]);
-                    db[e] += dz;
+                    norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
+                                                    GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f,
+                                                    to_f32<ST>(static_cast<const ST*>(p.dy)[(row0 + l) * p.sdy + ch]), st, f2_get(w[0]).x,
+                                                    f2_get(b[0]).x, xhat, dz, dg);
+                    // both sums of the channel in one pair, (dz xhat, dz)
+                    dw[0] = f2_fma(f2(dz), f2(xhat, 1.0f), dw[0]);
+                    s1 = f2_fma(f2(dz * f2_get(w[0]).x), f2(1.0f, xhat), s1);
                 }
             }
         }
-        norm_leave<V>(p, k, make_float4(s1, s2, 0.0f, 0.0f), shared, norm_add);
+        const float2 a = f2_get(s1);
+        norm_leave<V>(p, k, V == 8 ? make_float4(a.x + a.y, f2_sum(s2), 0.0f, 0.0f) : make_float4(a.x, a.y, 0.0f, 0.0f), shared,
+                      [](float4 a, float4 b) { return norm_add(a, b); });
         __syncthreads();
     }
-    if (k.active)
-#pragma unroll
-        for (int e = 0; e < V; ++e) chan[threadIdx.x * V + e] = make_float2(dw[e], db[e]);
-    __syncthreads();
     if (!p.part) return;
+    if (k.active) {
+        if constexpr (V == 8) {
+#pragma unroll
+            for (int e = 0; e < H; ++e) {
+                const float2 a = f2_get(dw[e]), c = f2_get(db[e]);
+                chan[threadIdx.x * 8 + 2 * e] = make_float2(a.x, c.x);
+                chan[threadIdx.x * 8 + 2 * e + 1] = make_float2(a.y, c.y);
+            }
+        } else {
+            chan[threadIdx.x] = f2_get(dw[0]);
+        }
+    }
+    __syncthreads();
     for (int i = (int)threadIdx.x; i < k.nch; i += kNormThreads) {
         float2 v = chan[i];
         for (int y = 1; y < k.Y; ++y) {
@@ -520,7 +723,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const No
     }
 }
 
-template <typename ST, int V, bool GATE>
+template <typename ST, int V, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads) norm_planes_dx_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
@@ -528,29 +731,43 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_dx_kernel(const Norm
     const NormBlock k = norm_block<V>(p, blockIdx.x / (unsigned)p.xblocks, (int)blockIdx.x % p.xblocks);
     ptx::grid_dependency_wait();
     const float count = 1.0f / ((float)p.L * (float)p.c);
-    norm_collect(p, k, means, norm_add, [&](float4 v) { return make_float2(v.x * count, v.y * count); });
+    norm_collect(p, k, means, [](float4 a, float4 b) { return norm_add(a, b); }, [&](float4 v) { return make_float2(v.x * count, v.y * count); });
     if (!k.active) return;
     const int ch = k.c0 + k.tx * V;
     const float2 m = means[k.groups > 1 ? k.tx * V / p.c : 0];
-    float w[V], b[V];
-    norm_param<V>(p.w, ch, 1.0f, w);
-    norm_param<V>(p.b, ch, 0.0f, b);
     const float2 st = p.stats[k.n * p.G + ch / p.c];
     const long long row0 = k.n * p.L;
+    if constexpr (V == 8) {
+        F2 w[4], b[4];
+        param_eight(p.w, ch, 1.0f, w);
+        param_eight(p.b, ch, 0.0f, b);
 #pragma unroll 2
-    for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
-        float x[V], gt[V], dy[V], dx[V], dg[V];
-        norm_load<ST, V>(p.x, (row0 + l) * p.sx + ch, x);
-        norm_load<ST, V>(p.dy, (row0 + l) * p.sdy + ch, dy);
-        if (GATE) norm_load<ST, V>(p.gate, (row0 + l) * p.sg + ch, gt);
+        for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
+            Eight<ST> rx, rg, rd;
+            F2 x[4], gt[4], dy[4], xhat[4], dz[4], dg[4];
+            rx.load(p.x, (row0 + l) * p.sx + ch);
+            rd.load(p.dy, (row0 + l) * p.sdy + ch);
+            if (GATE) rg.load(p.gate, (row0 + l) * p.sg + ch);
+            rx.get(x);
+            rd.get(dy);
+            if (GATE) rg.get(gt);
+            norm_gradient8<kFast, GATE, ACT>(x, gt, dy, st, w, b, xhat, dz, dg);
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float xhat, dz;
-            norm_gradient<kFast, GATE>(p.act, x[e], GATE ? gt[e] : 0.0f, dy[e], st, w[e], b[e], xhat, dz, dg[e]);
-            dx[e] = st.y * (dz * w[e] - m.x - xhat * m.y);
+            for (int e = 0; e < 4; ++e) dz[e] = f2_mul(f2_fma(xhat[e], f2(-m.y), f2_fma(dz[e], w[e], f2(-m.x))), f2(st.y));
+            store_eight<ST>(p.dx, (row0 + l) * p.C + ch, dz);
+            if (GATE) store_eight<ST>(p.dgate, (row0 + l) * p.C + ch, dg);
         }
-        norm_store<ST, V>(p.dx, (row0 + l) * p.C + ch, dx);
-        if (GATE) norm_store<ST, V>(p.dgate, (row0 + l) * p.C + ch, dg);
+    } else {
+        const float w = p.w ? p.w[ch] : 1.0f, b = p.b ? p.b[ch] : 0.0f;
+#pragma unroll 4
+        for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
+            float xhat, dz, dg;
+            norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
+                                            GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f,
+                                            to_f32<ST>(static_cast<const ST*>(p.dy)[(row0 + l) * p.sdy + ch]), st, w, b, xhat, dz, dg);
+            static_cast<ST*>(p.dx)[(row0 + l) * p.C + ch] = from_f32<ST>(st.y * (dz * w - m.x - xhat * m.y));
+            if (GATE) static_cast<ST*>(p.dgate)[(row0 + l) * p.C + ch] = from_f32<ST>(dg);
+        }
     }
 }
 
