@@ -19,7 +19,7 @@ int check(const linrec_group_norm_args* a)
 
 // How a problem is laid out; the scratch sizes follow from it, so it depends on sizes and alignment alone (the
 // grid is sized for 148 SMs whatever the device).
-constexpr long long kCtas = 148 * 4;
+constexpr long long kCtas = 148 * 3;
 
 struct Plan {
     bool rows;
@@ -137,6 +137,7 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     bool aligned = on_16(a.x, a.x_stride, size) && (!a.gate || on_16(a.gate, a.gate_stride, size));
     if (!bwd) aligned = aligned && on_16(a.y, a.nchan, size);
     else aligned = aligned && on_16(a.dy, a.dy_stride, size) && on_16(a.dx, a.nchan, size) && (!a.gate || on_16(a.dgate, a.nchan, size));
+    aligned = aligned && on_16(a.weight, 0, 1) && on_16(a.bias, 0, 1);
     const Plan pl = plan_of(a, aligned, bwd);
     if (!pl.rows && pl.yblocks > 0x7fffffffLL / pl.xblocks) return LINREC_ERR_INVALID_ARG;
     NormParams p{};
@@ -146,7 +147,7 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     p.n = a.nsamples; p.L = a.positions; p.C = (int)a.nchan; p.G = (int)a.groups; p.c = (int)(a.nchan / a.groups);
     p.stats = reinterpret_cast<float2*>(a.stats);
     p.y = bwd ? nullptr : a.y; p.dx = a.dx; p.dgate = a.dgate;
-    p.lanes = pl.lanes; p.gb = pl.gb; p.rp = pl.rp; p.cpb = pl.cpb; p.sub = pl.sub; p.slices = pl.slices; p.xblocks = pl.xblocks;
+    p.lanes = pl.lanes; p.gb = pl.gb; p.rp = pl.rp; p.cpb = pl.cpb; p.sub = pl.sub; p.slices = pl.slices; p.xblocks = pl.xblocks; p.per = pl.slices > 0 ? (a.positions + pl.slices - 1) / pl.slices : 0;
     char* scratch = static_cast<char*>(a.scratch);
     p.gpart = reinterpret_cast<float4*>(scratch);
     const bool params = bwd && (a.dweight || a.dbias);

@@ -42,9 +42,16 @@ struct NormParams {
     // planes
     int cpb, sub;                 // channels per CTA; CTAs that a group is spread over (1: a CTA holds whole groups)
     int slices, xblocks;          // slices of a sample's positions; CTAs across the channels
+    long long per;                // positions in a slice
     float4* gpart;                // [n][slices * sub][G]: (mean, squares, count) forward, (sum k, sum k xhat) backward
 };
 
+// Operands are loaded as read-only data: a kernel's loads may then be issued ahead of its stores.
+template <typename ST>
+__device__ __forceinline__ float load_one(const void* base, long long offset)
+{
+    return to_f32<ST>(__ldg(static_cast<const ST*>(base) + offset));
+}
 // Eight adjacent elements on a 16-byte boundary: as loaded, and as pairs of floats.
 template <typename ST>
 struct Eight {
@@ -52,8 +59,8 @@ struct Eight {
     __device__ __forceinline__ void load(const void* base, long long offset)
     {
         const uint4* q = reinterpret_cast<const uint4*>(static_cast<const ST*>(base) + offset);
-        w[0] = q[0];
-        if constexpr (sizeof(ST) == 4) w[1] = q[1];
+        w[0] = __ldg(q);
+        if constexpr (sizeof(ST) == 4) w[1] = __ldg(q + 1);
     }
     __device__ __forceinline__ void clear()
     {
@@ -85,7 +92,11 @@ __device__ __forceinline__ void store_eight(void* base, long long offset, const 
 __device__ __forceinline__ void param_eight(const float* p, int ch, float missing, F2 (&v)[4])
 {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = p ? f2(__ldg(p + ch + 2 * e), __ldg(p + ch + 2 * e + 1)) : f2(missing);
+    for (int e = 0; e < 4; e += 2) {
+        const float4 q = p ? __ldg(reinterpret_cast<const float4*>(p + ch + 2 * e)) : make_float4(missing, missing, missing, missing);
+        v[e] = f2(q.x, q.y);
+        v[e + 1] = f2(q.z, q.w);
+    }
 }
 __device__ __forceinline__ float f2_sum(F2 a)
 {
@@ -275,7 +286,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_fwd_kernel(const N
         const ST* gate = static_cast<const ST*>(p.gate) + n * p.sg + ch0;
         float v[NV], sum = 0.0f, sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = row && i < mine ? to_f32<ST>(x[i * p.lanes + s.lane]) : 0.0f;
+        for (int i = 0; i < NV; ++i) v[i] = row && i < mine ? load_one<ST>(x, i * p.lanes + s.lane) : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) sum += v[i];
         const float mean = lanes_sum(sum, p.lanes) * count;
@@ -289,7 +300,7 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_fwd_kernel(const N
             if (i < mine) {
                 const int e = i * p.lanes + s.lane, ch = ch0 + e;
                 static_cast<ST*>(p.y)[n * p.C + ch] = from_f32<ST>(norm_value<kFast, GATE, ACT>(
-                    v[i], GATE ? to_f32<ST>(gate[e]) : 0.0f, mean, inv, p.w ? __ldg(p.w + ch) : 1.0f, p.b ? __ldg(p.b + ch) : 0.0f));
+                    v[i], GATE ? load_one<ST>(gate, e) : 0.0f, mean, inv, p.w ? __ldg(p.w + ch) : 1.0f, p.b ? __ldg(p.b + ch) : 0.0f));
             }
     }
 }
@@ -429,9 +440,9 @@ __global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_bwd_kernel(const N
                 const int ch = ch0 + i * p.lanes + s.lane;
                 const float w = p.w ? __ldg(p.w + ch) : 1.0f;
                 float dz, dg;
-                norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[n * p.sx + ch]),
-                                                GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[n * p.sg + ch]) : 0.0f,
-                                                to_f32<ST>(static_cast<const ST*>(p.dy)[n * p.sdy + ch]), st, w, p.b ? __ldg(p.b + ch) : 0.0f,
+                norm_gradient<kFast, GATE, ACT>(load_one<ST>(p.x, n * p.sx + ch),
+                                                GATE ? load_one<ST>(p.gate, n * p.sg + ch) : 0.0f,
+                                                load_one<ST>(p.dy, n * p.sdy + ch), st, w, p.b ? __ldg(p.b + ch) : 0.0f,
                                                 xhat[i], dz, dg);
                 if (p.part) {
                     float2 v = sums[i * p.lanes];
@@ -466,11 +477,10 @@ template <int V>
 __device__ __forceinline__ NormBlock norm_block(const NormParams& p, long long item, int xblock)
 {
     NormBlock k;
-    const long long per = (p.L + p.slices - 1) / p.slices;
-    k.n = item / p.slices;
-    const int slice = (int)(item - k.n * p.slices);
-    k.l0 = per * slice;
-    k.l1 = min(p.L, k.l0 + per);
+    k.n = (unsigned)item / (unsigned)p.slices;
+    const int slice = (int)((unsigned)item - (unsigned)k.n * (unsigned)p.slices);
+    k.l0 = p.per * slice;
+    k.l1 = min(p.L, k.l0 + p.per);
     if (p.sub == 1) {
         const int gb = p.cpb / p.c;
         k.g0 = xblock * gb;
@@ -499,7 +509,7 @@ __device__ __forceinline__ float4 norm_merge(float4 a, float4 b)
 {
     if (b.z == 0.0f) return a;
     if (a.z == 0.0f) return b;
-    const float n = a.z + b.z, d = b.x - a.x, f = b.z / n;
+    const float n = a.z + b.z, d = b.x - a.x, f = __fdividef(b.z, n);
     return make_float4(fmaf(d, f, a.x), a.y + fmaf(d * d, a.z * f, b.y), n, 0.0f);
 }
 __device__ __forceinline__ float4 norm_add(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, 0.0f, 0.0f); }
@@ -528,22 +538,30 @@ __device__ __forceinline__ void norm_leave(const NormParams& p, const NormBlock&
 template <typename Merge, typename Finish>
 __device__ __forceinline__ void norm_collect(const NormParams& p, const NormBlock& k, float2* result, Merge merge, Finish finish)
 {
+    __shared__ float4 some[kNormThreads / 32][32];
     const int warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31, slots = p.slices * p.sub;
-    for (int g = warp; g < k.groups; g += kNormThreads / 32) {
+    // neighbouring lanes take neighbouring groups, the warps share the slices
+    for (int g0 = 0; g0 < k.groups; g0 += 32) {
+        const int g = g0 + lane;
+        const bool in = g < k.groups;
+        const float4* from = p.gpart + k.n * slots * p.G + k.g0 + g;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int i = lane; i < slots; i += 32) v = merge(v, p.gpart[(k.n * slots + i) * p.G + k.g0 + g]);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v = merge(v, shfl_down4(v, o));
-        if (lane == 0) {
+        if (in)
+#pragma unroll 4
+            for (int i = warp; i < slots; i += kNormThreads / 32) v = merge(v, from[(long long)i * p.G]);
+        some[warp][lane] = v;
+        __syncthreads();
+        if (warp == 0 && in) {
+            for (int i = 1; i < kNormThreads / 32; ++i) v = merge(v, some[i][lane]);
             result[g] = finish(v);
             if (p.stats && k.slot == 0 && p.y) p.stats[k.n * p.G + k.g0 + g] = result[g];
         }
+        __syncthreads();
     }
-    __syncthreads();
 }
 
 template <typename ST, int V>
-__global__ void __launch_bounds__(kNormThreads) norm_planes_stats_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_planes_stats_kernel(const NormParams p)
 {
     __shared__ float4 shared[kNormThreads];
     const NormBlock k = norm_block<V>(p, blockIdx.x / (unsigned)p.xblocks, (int)blockIdx.x % p.xblocks);
@@ -554,7 +572,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_stats_kernel(const N
     if (k.active && l < k.l1) {
         const long long row0 = k.n * p.L;
         float about, s, q, count = (float)V * (float)((k.l1 - l + k.Y - 1) / k.Y);
-        about = to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]);
+        about = load_one<ST>(p.x, (row0 + l) * p.sx + ch);
         if constexpr (V == 8) {
             const F2 off = f2(-about);
             F2 s2 = f2(0.0f), q2 = f2(0.0f);
@@ -576,7 +594,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_stats_kernel(const N
             s = q = 0.0f;
 #pragma unroll 4
             for (; l < k.l1; l += k.Y) {
-                const float d = to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]) - about;
+                const float d = load_one<ST>(p.x, (row0 + l) * p.sx + ch) - about;
                 s += d;
                 q = fmaf(d, d, q);
             }
@@ -588,7 +606,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_stats_kernel(const N
 }
 
 template <typename ST, int V, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_planes_apply_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_planes_apply_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     __shared__ float2 st[kNormThreads * V];
@@ -624,14 +642,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_apply_kernel(const N
 #pragma unroll 4
         for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y)
             static_cast<ST*>(p.y)[(row0 + l) * p.C + ch] = from_f32<ST>(norm_value<kFast, GATE, ACT>(
-                to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
-                GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f, mine.x, mine.y, w, b));
+                load_one<ST>(p.x, (row0 + l) * p.sx + ch),
+                GATE ? load_one<ST>(p.gate, (row0 + l) * p.sg + ch) : 0.0f, mine.x, mine.y, w, b));
     }
 }
 
 // Sums of k and k xhat per slice and group, and of (dz xhat, dz) per slice and channel.
 template <typename ST, int V, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_planes_sums_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     constexpr int H = V == 8 ? 4 : 1;
@@ -683,9 +701,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const No
                     }
                 } else {
                     float xhat, dz, dg;
-                    norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
-                                                    GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f,
-                                                    to_f32<ST>(static_cast<const ST*>(p.dy)[(row0 + l) * p.sdy + ch]), st, f2_get(w[0]).x,
+                    norm_gradient<kFast, GATE, ACT>(load_one<ST>(p.x, (row0 + l) * p.sx + ch),
+                                                    GATE ? load_one<ST>(p.gate, (row0 + l) * p.sg + ch) : 0.0f,
+                                                    load_one<ST>(p.dy, (row0 + l) * p.sdy + ch), st, f2_get(w[0]).x,
                                                     f2_get(b[0]).x, xhat, dz, dg);
                     // both sums of the channel in one pair, (dz xhat, dz)
                     dw[0] = f2_fma(f2(dz), f2(xhat, 1.0f), dw[0]);
@@ -724,7 +742,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_sums_kernel(const No
 }
 
 template <typename ST, int V, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_planes_dx_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, 3) norm_planes_dx_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     __shared__ float2 means[kNormThreads * V];
@@ -762,9 +780,9 @@ __global__ void __launch_bounds__(kNormThreads) norm_planes_dx_kernel(const Norm
 #pragma unroll 4
         for (long long l = k.l0 + k.ty; l < k.l1; l += k.Y) {
             float xhat, dz, dg;
-            norm_gradient<kFast, GATE, ACT>(to_f32<ST>(static_cast<const ST*>(p.x)[(row0 + l) * p.sx + ch]),
-                                            GATE ? to_f32<ST>(static_cast<const ST*>(p.gate)[(row0 + l) * p.sg + ch]) : 0.0f,
-                                            to_f32<ST>(static_cast<const ST*>(p.dy)[(row0 + l) * p.sdy + ch]), st, w, b, xhat, dz, dg);
+            norm_gradient<kFast, GATE, ACT>(load_one<ST>(p.x, (row0 + l) * p.sx + ch),
+                                            GATE ? load_one<ST>(p.gate, (row0 + l) * p.sg + ch) : 0.0f,
+                                            load_one<ST>(p.dy, (row0 + l) * p.sdy + ch), st, w, b, xhat, dz, dg);
             static_cast<ST*>(p.dx)[(row0 + l) * p.C + ch] = from_f32<ST>(st.y * (dz * w - m.x - xhat * m.y));
             if (GATE) static_cast<ST*>(p.dgate)[(row0 + l) * p.C + ch] = from_f32<ST>(dg);
         }
