@@ -271,37 +271,38 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_k
 
 // One element per access, NV per lane (rows off 16-byte boundaries, or groups that are not whole sixteens of bytes).
 template <typename ST, int NV, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_fwd_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_fwd_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
+    const int lanes = NV > 8 ? 32 : p.lanes;      // (many pieces: a whole warp, and constant distances)
     const NormSlot s = norm_slot(p);
     ptx::grid_dependency_wait();
-    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + p.lanes - 1) / p.lanes : 0;      // elements of this lane
+    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + lanes - 1) / lanes : 0;      // elements of this lane
+    const float *w = p.w + ch0 + s.lane, *b = p.b + ch0 + s.lane;
     const long long step = (long long)gridDim.y * p.rp;
     long long n = (long long)blockIdx.y * p.rp + s.r;
     const float count = 1.0f / (float)p.c;
     for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
         const bool row = n < p.n;
-        const ST* x = static_cast<const ST*>(p.x) + n * p.sx + ch0;
-        const ST* gate = static_cast<const ST*>(p.gate) + n * p.sg + ch0;
+        const ST* x = static_cast<const ST*>(p.x) + n * p.sx + ch0 + s.lane;
+        const ST* gate = static_cast<const ST*>(p.gate) + n * p.sg + ch0 + s.lane;
+        ST* y = static_cast<ST*>(p.y) + n * p.C + ch0 + s.lane;
         float v[NV], sum = 0.0f, sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = row && i < mine ? load_one<ST>(x, i * p.lanes + s.lane) : 0.0f;
+        for (int i = 0; i < NV; ++i) v[i] = row && i < mine ? load_one<ST>(x, i * lanes) : 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) sum += v[i];
-        const float mean = lanes_sum(sum, p.lanes) * count;
+        const float mean = lanes_sum(sum, lanes) * count;
 #pragma unroll
         for (int i = 0; i < NV; ++i) sq = i < mine ? fmaf(v[i] - mean, v[i] - mean, sq) : sq;
-        const float inv = 1.0f / sqrtf(fmaf(lanes_sum(sq, p.lanes), count, p.eps));
+        const float inv = 1.0f / sqrtf(fmaf(lanes_sum(sq, lanes), count, p.eps));
         if (!row) continue;
         if (p.stats && s.lane == 0 && s.active) p.stats[n * p.G + s.g] = make_float2(mean, inv);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (i < mine) {
-                const int e = i * p.lanes + s.lane, ch = ch0 + e;
-                static_cast<ST*>(p.y)[n * p.C + ch] = from_f32<ST>(norm_value<kFast, GATE, ACT>(
-                    v[i], GATE ? load_one<ST>(gate, e) : 0.0f, mean, inv, p.w ? __ldg(p.w + ch) : 1.0f, p.b ? __ldg(p.b + ch) : 0.0f));
-            }
+            if (i < mine)
+                y[i * lanes] = from_f32<ST>(norm_value<kFast, GATE, ACT>(v[i], GATE ? load_one<ST>(gate, i * lanes) : 0.0f, mean, inv,
+                                                                         p.w ? __ldg(w + i * lanes) : 1.0f, p.b ? __ldg(b + i * lanes) : 0.0f));
     }
 }
 
@@ -415,51 +416,55 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 3 : 1) norm_rows_bwd_k
 
 // One element per access; the sums of (dz xhat, dz) live in shared memory, every thread at its own places.
 template <typename ST, int NV, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads, 2) norm_rows1_bwd_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_bwd_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
+    const int lanes = NV > 8 ? 32 : p.lanes;      // (many pieces: a whole warp, and constant distances)
     extern __shared__ __align__(16) float2 norm_sums[];
     const NormSlot s = norm_slot(p);
     ptx::grid_dependency_wait();
     const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
-    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + p.lanes - 1) / p.lanes : 0;
+    const int ch0 = s.g * p.c, mine = s.active ? (p.c - s.lane + lanes - 1) / lanes : 0;
     float2* sums = norm_sums + s.r * nch + ch0 - c0 + s.lane;
     if (p.part)
-        for (int i = 0; i < mine; ++i) sums[i * p.lanes] = make_float2(0.0f, 0.0f);
+        for (int i = 0; i < mine; ++i) sums[i * lanes] = make_float2(0.0f, 0.0f);
+    const float *w = p.w + ch0 + s.lane, *b = p.b + ch0 + s.lane;
     const long long step = (long long)gridDim.y * p.rp;
     const float count = 1.0f / (float)p.c;
     long long n = (long long)blockIdx.y * p.rp + s.r;
     for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
         const bool row = n < p.n;
         const float2 st = row && s.active ? p.stats[n * p.G + s.g] : make_float2(0.0f, 0.0f);
+        const ST* x = static_cast<const ST*>(p.x) + n * p.sx + ch0 + s.lane;
+        const ST* dy = static_cast<const ST*>(p.dy) + n * p.sdy + ch0 + s.lane;
+        const ST* gate = static_cast<const ST*>(p.gate) + n * p.sg + ch0 + s.lane;
+        ST* dx = static_cast<ST*>(p.dx) + n * p.C + ch0 + s.lane;
+        ST* dgate = static_cast<ST*>(p.dgate) + n * p.C + ch0 + s.lane;
         float xhat[NV], k[NV], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             xhat[i] = k[i] = 0.0f;
             if (row && i < mine) {
-                const int ch = ch0 + i * p.lanes + s.lane;
-                const float w = p.w ? __ldg(p.w + ch) : 1.0f;
+                const float wi = p.w ? __ldg(w + i * lanes) : 1.0f;
                 float dz, dg;
-                norm_gradient<kFast, GATE, ACT>(load_one<ST>(p.x, n * p.sx + ch),
-                                                GATE ? load_one<ST>(p.gate, n * p.sg + ch) : 0.0f,
-                                                load_one<ST>(p.dy, n * p.sdy + ch), st, w, p.b ? __ldg(p.b + ch) : 0.0f,
-                                                xhat[i], dz, dg);
+                norm_gradient<kFast, GATE, ACT>(load_one<ST>(x, i * lanes), GATE ? load_one<ST>(gate, i * lanes) : 0.0f,
+                                                load_one<ST>(dy, i * lanes), st, wi, p.b ? __ldg(b + i * lanes) : 0.0f, xhat[i], dz, dg);
                 if (p.part) {
-                    float2 v = sums[i * p.lanes];
+                    float2 v = sums[i * lanes];
                     v.x = fmaf(dz, xhat[i], v.x);
                     v.y += dz;
-                    sums[i * p.lanes] = v;
+                    sums[i * lanes] = v;
                 }
-                k[i] = dz * w;
+                k[i] = dz * wi;
                 s1 += k[i];
                 s2 = fmaf(k[i], xhat[i], s2);
-                if (GATE) static_cast<ST*>(p.dgate)[n * p.C + ch] = from_f32<ST>(dg);
+                if (GATE) dgate[i * lanes] = from_f32<ST>(dg);
             }
         }
-        const float m1 = lanes_sum(s1, p.lanes) * count, m2 = lanes_sum(s2, p.lanes) * count;
+        const float m1 = lanes_sum(s1, lanes) * count, m2 = lanes_sum(s2, lanes) * count;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (row && i < mine) static_cast<ST*>(p.dx)[n * p.C + ch0 + i * p.lanes + s.lane] = from_f32<ST>(st.y * (k[i] - m1 - xhat[i] * m2));
+            if (row && i < mine) dx[i * lanes] = from_f32<ST>(st.y * (k[i] - m1 - xhat[i] * m2));
     }
     if (p.part) norm_rows_leave(p, norm_sums);
 }
