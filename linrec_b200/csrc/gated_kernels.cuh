@@ -916,70 +916,129 @@ __device__ __forceinline__ long long step_slot(const GatedStepParams& p, int r)
     return s >= 0 && s < p.nslots ? s : -1;
 }
 
-// One row per block row; a thread owns V channels.  A slot that several rows name holds ONE sequence whose
-// tokens are the rows in order: the first of them walks through all, the others leave.
-template <typename ST, bool DECAY>
-__global__ void __launch_bounds__(128) gated_step_kernel(const GatedStepParams p)
+// V adjacent channels of a row (V = 4: one access, on a boundary of four elements).
+template <typename ST, int V>
+__device__ __forceinline__ void step_load(const void* base, long long offset, float* v)
+{
+    const ST* q = static_cast<const ST*>(base) + offset;
+    if constexpr (V == 4 && sizeof(ST) == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(q);
+        v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else if constexpr (V == 4) {
+        const uint2 w = *reinterpret_cast<const uint2*>(q);
+        Two<ST>::unpack(w.x, v), Two<ST>::unpack(w.y, v + 2);
+    } else {
+        v[0] = to_f32<ST>(*q);
+    }
+}
+template <typename ST, int V>
+__device__ __forceinline__ void step_store(void* base, long long offset, const float* v)
+{
+    ST* q = static_cast<ST*>(base) + offset;
+    if constexpr (V == 4 && sizeof(ST) == 4) *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (V == 4) *reinterpret_cast<uint2*>(q) = make_uint2(Two<ST>::pack(v), Two<ST>::pack(v + 2));
+    else *q = from_f32<ST>(v[0]);
+}
+
+constexpr int kStepThreads = 128;
+
+// ROWS rows and 128 V channels per CTA.  Bound by memory: an element moves 6 or 8 bytes of operands and results
+// in 16 bits and 8 of state; several rows per CTA keep that much more in flight and share the decay parameters and
+// the search below.
+// A slot that several rows name holds ONE sequence whose tokens are the rows in order: the first of them walks
+// through all, the others leave them to it.  Every CTA compares its rows' slots with all rows'.
+template <typename ST, bool DECAY, int V, int ROWS>
+__global__ void __launch_bounds__(kStepThreads) gated_step_kernel(const GatedStepParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
+    __shared__ unsigned shared_flags;      // bit r: an earlier row has row r's slot; bit 16 + r: a later one
     __shared__ int nearest;
     const int tid = (int)threadIdx.x;
-    const int ch = ((int)blockIdx.y * 128 + tid) * 2;
-    const int have = p.D - ch;
-    int row = (int)blockIdx.x;
+    const int ch = ((int)blockIdx.y * kStepThreads + tid) * V;
+    const bool have = ch < p.D;
+    const int row0 = (int)blockIdx.x * ROWS;
+    if (tid == 0) shared_flags = 0u;
     ptx::grid_dependency_wait();
-    const long long slot = step_slot(p, row);
-    if (slot < 0) {
-        const float zero[2] = {0.0f, 0.0f};
-        store_two<ST>(p.y, (long long)row * p.D + ch, have, zero);
-        return;
-    }
-    bool earlier = false, later = false;
-    if (p.slots)
-        for (int r = tid; r < p.rows; r += 128)
-            if (r != row && step_slot(p, r) == slot) (r < row ? earlier : later) = true;
-    if (__syncthreads_or(earlier)) return;
-    const bool chain = __syncthreads_or(later);
-
-    float h[2] = {0.0f, 0.0f}, rate[2] = {0.0f, 0.0f};
-    load_two<float>(p.state, slot * p.sstate + ch, have, h);
-    if (DECAY) {
+    long long slot[ROWS];
+    float x[ROWS][V], f[ROWS][V], g[ROWS][V], h[ROWS][V], rate[V];
 #pragma unroll
-        for (int v = 0; v < 2; ++v)
-            if (v < have) rate[v] = p.scale * softplus(p.decay[ch + v]);
+    for (int r = 0; r < ROWS; ++r) {
+        slot[r] = row0 + r < p.rows ? step_slot(p, row0 + r) : -1;
+        if (slot[r] >= 0 && have) {
+            step_load<float, V>(p.state, slot[r] * p.sstate + ch, h[r]);
+            step_load<ST, V>(p.x, (long long)(row0 + r) * p.sx + ch, x[r]);
+            step_load<ST, V>(p.f, (long long)(row0 + r) * p.sf + ch, f[r]);
+            if (DECAY) step_load<ST, V>(p.ig, (long long)(row0 + r) * p.si + ch, g[r]);
+        }
     }
-    while (true) {
-        float xv[2], fv[2], iv[2];
-        load_two<ST>(p.x, (long long)row * p.sx + ch, have, xv);
-        load_two<ST>(p.f, (long long)row * p.sf + ch, have, fv);
-        if (DECAY) load_two<ST>(p.ig, (long long)row * p.si + ch, have, iv);
+    if (DECAY && have)
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
+        for (int v = 0; v < V; ++v) rate[v] = p.scale * softplus(__ldg(p.decay + ch + v));
+    unsigned flags = 0u;
+    if (p.slots) {
+        for (int n = tid; n < p.rows; n += kStepThreads) {
+            const long long other = step_slot(p, n);
+            if (other < 0) continue;
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r)
+                if (other == slot[r] && n != row0 + r) flags |= n < row0 + r ? 1u << r : 65536u << r;
+        }
+        flags = __reduce_or_sync(0xffffffffu, flags);
+        __syncthreads();
+        if ((tid & 31) == 0 && flags) atomicOr(&shared_flags, flags);
+        __syncthreads();
+        flags = shared_flags;
+    }
+    auto advance = [&](const float* xv, const float* fv, const float* gv, float* hv) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
             if (DECAY) {
                 float a, b2;
                 decay_factors<kFast, false>(rate[v] * logistic<kFast>(fv[v]), a, b2);
-                h[v] = fmaf(a, h[v], approx_sqrt(b2) * (logistic<kFast>(iv[v]) * xv[v]));
+                hv[v] = fmaf(a, hv[v], approx_sqrt(b2) * (logistic<kFast>(gv[v]) * xv[v]));
             } else {
                 float s, n;
                 logistic_pair<kFast>(fv[v], s, n);
-                h[v] = fmaf(s, h[v], n * xv[v]);
+                hv[v] = fmaf(s, hv[v], n * xv[v]);
             }
         }
-        store_two<ST>(p.y, (long long)row * p.D + ch, have, h);
-        if (!chain) break;
-        __syncthreads();
-        if (tid == 0) nearest = 0x7fffffff;
-        __syncthreads();
-        for (int r = row + 1 + tid; r < p.rows; r += 128)
-            if (step_slot(p, r) == slot) {
-                atomicMin(&nearest, r);
-                break;
+    };
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        int row = row0 + r;
+        if (row >= p.rows || (flags >> r & 1u)) continue;
+        if (slot[r] < 0) {
+            const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (have) step_store<ST, V>(p.y, (long long)row * p.D + ch, zero);
+            continue;
+        }
+        if (have) {
+            advance(x[r], f[r], g[r], h[r]);
+            step_store<ST, V>(p.y, (long long)row * p.D + ch, h[r]);
+        }
+        while (flags >> (16 + r) & 1u) {      // the sequence's next token, if there is one
+            __syncthreads();
+            if (tid == 0) nearest = 0x7fffffff;
+            __syncthreads();
+            for (int n = row + 1 + tid; n < p.rows; n += kStepThreads)
+                if (step_slot(p, n) == slot[r]) {
+                    atomicMin(&nearest, n);
+                    break;
+                }
+            __syncthreads();
+            row = nearest;
+            if (row == 0x7fffffff) break;
+            if (have) {
+                float xn[V], fn[V], gn[V];
+                step_load<ST, V>(p.x, (long long)row * p.sx + ch, xn);
+                step_load<ST, V>(p.f, (long long)row * p.sf + ch, fn);
+                if (DECAY) step_load<ST, V>(p.ig, (long long)row * p.si + ch, gn);
+                advance(xn, fn, gn, h[r]);
+                step_store<ST, V>(p.y, (long long)row * p.D + ch, h[r]);
             }
-        __syncthreads();
-        if (nearest == 0x7fffffff) break;
-        row = nearest;
+        }
+        if (have) step_store<float, V>(p.state, slot[r] * p.sstate + ch, h[r]);
     }
-    store_two<float>(p.state, slot * p.sstate + ch, have, h);
 }
 
 }  // namespace linrec

@@ -367,7 +367,7 @@ def test_no_rows():
 
 
 # ---- one token ---------------------------------------------------------------------------------------
-@pytest.mark.parametrize("rows,D", [(1, 1), (3, 64), (7, 257), (33, 1000), (2, 2048), (130, 40)])
+@pytest.mark.parametrize("rows,D", [(1, 1), (3, 64), (7, 257), (33, 1000), (2, 2048), (130, 40), (600, 4100), (600, 1003)])
 @pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
 def test_step(rows, D, decay, dtype):
