@@ -179,6 +179,28 @@ __device__ __forceinline__ void logistic_pair2(F2 v, F2& p, F2& n)
     }
 }
 
+// s(v) and s(-v) = e^-v s(v) of both channels, for operands that are tested for NaN elsewhere (the bound on the
+// exponent, which keeps 0 * inf out, lets NaN through as a number).
+template <bool FAST>
+__device__ __forceinline__ void logistic_both2(F2 v, F2& p, F2& n)
+{
+    if (FAST) {
+        const float2 t = f2_get(f2_mul(v, f2(-1.44269504f)));
+        const F2 e = f2(approx_exp2(fminf(t.x, 126.0f)), approx_exp2(fminf(t.y, 126.0f)));
+        const float2 d = f2_get(f2_add(e, f2(1.0f)));
+        p = f2(approx_rcp(d.x), approx_rcp(d.y));
+        n = f2_mul(e, p);
+    } else {
+        logistic_pair2<false>(v, p, n);
+    }
+}
+__device__ __forceinline__ float approx_rsqrt(float v)
+{
+    float r;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // Two adjacent channels as one word of shared or global memory.
 template <typename ST>
 struct Two;

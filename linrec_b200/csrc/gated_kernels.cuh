@@ -88,9 +88,9 @@ __device__ __forceinline__ void decay_factors(float y, float& a, float& b2)
     b2 = d * (1.0f + a);
 }
 
-// The same for two channels.
+// The same for two channels: a and b^2.
 template <bool FAST, bool SMALL>
-__device__ __forceinline__ void decay_factors2(F2 y, F2& a, F2& b)
+__device__ __forceinline__ void decay_factors2(F2 y, F2& a, F2& b2)
 {
     if (SMALL) {
         F2 s = f2_fma(y, f2(-1.0f / 720.0f), f2(1.0f / 120.0f));
@@ -99,16 +99,34 @@ __device__ __forceinline__ void decay_factors2(F2 y, F2& a, F2& b)
         s = f2_fma(y, s, f2(-0.5f));
         const F2 d = f2_mul(y, f2_fma(y, s, f2(1.0f)));
         a = f2_fma(d, f2(-1.0f), f2(1.0f));
-        const float2 b2 = f2_get(f2_fma(d, a, d));
-        b = f2(approx_sqrt(b2.x), approx_sqrt(b2.y));
+        b2 = f2_fma(d, a, d);
     } else {
         const float2 w = f2_get(y);
         float a0, a1, b0, b1;
         decay_factors<FAST, false>(w.x, a0, b0);
         decay_factors<FAST, false>(w.y, a1, b1);
         a = f2(a0, a1);
-        b = f2(approx_sqrt(b0), approx_sqrt(b1));
+        b2 = f2(b0, b1);
     }
+}
+__device__ __forceinline__ F2 root2(F2 v)
+{
+    const float2 w = f2_get(v);
+    return f2(approx_sqrt(w.x), approx_sqrt(w.y));
+}
+// b s(i).  Fast: with d = 1 + e^-i it is b^2 / sqrt(b^2 d^2), one special function for a root and a reciprocal
+// (they bound the forward pass).  The tiny term keeps b = 0 from giving NaN: b is then taken as 1e-18.
+template <bool FAST>
+__device__ __forceinline__ F2 gated_factor2(F2 b2, F2 i)
+{
+    if (FAST) {
+        const float2 t = f2_get(f2_mul(i, f2(-1.44269504f)));
+        const F2 d = f2_add(f2(approx_exp2(t.x), approx_exp2(t.y)), f2(1.0f));
+        const F2 q = f2_add(b2, f2(1e-36f));
+        const float2 r = f2_get(f2_mul(f2_mul(q, d), d));
+        return f2_mul(q, f2(approx_rsqrt(r.x), approx_rsqrt(r.y)));
+    }
+    return f2_mul(root2(b2), logistic2<false>(i));
 }
 
 // ---- the pair operator with cuts ------------------------------------------------------------------------
@@ -344,6 +362,21 @@ __device__ __forceinline__ void gated_sync()
     asm volatile("bar.sync 1, %0;" ::"n"(W * 32) : "memory");
 }
 
+template <int W>
+__device__ __forceinline__ bool gated_any(const int* flags)
+{
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) any |= flags[i];
+    return any != 0;
+}
+__device__ __forceinline__ F2 gated_enter(float2 in, F2 Y, F2 P, bool cut)
+{
+    if (!cut) return f2_fma(f2(in.x, in.y), P, Y);
+    const float2 y = f2_get(Y), p = f2_get(P);
+    return f2(enter(in.x, Pair{y.x, p.x}), enter(in.y, Pair{y.y, p.y}));
+}
+
 struct GatedMaps {
     CUtensorMap x, f, i, dy;
 };
@@ -551,7 +584,8 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
 {
     using T = GatedTile<ST, DECAY, false, SHAPE>;
     constexpr int K = T::K, R = T::R;
-    __shared__ float4 runs[2][T::W][32];      // (Y, P) of both channels of every thread
+    __shared__ float4 runs[2][T::W][32];      // every thread's Y of both channels, then P
+    __shared__ int cuts[2][T::W];             // does a sequence start in a warp's run?
     __shared__ __align__(8) float entering[2][kGatedChannels];      // tiles take turns
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -576,9 +610,9 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
             for (int j = 0; j < K; ++j, at += wstep) {
                 const F2 xv = Two<ST>::get(at[0]), fv = Two<ST>::get(at[R * 32]);
                 if (DECAY) {
-                    F2 b;
-                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], b);
-                    u[j] = f2_mul(b, f2_mul(logistic2<T::kFast>(Two<ST>::get(at[2 * R * 32])), xv));
+                    F2 b2;
+                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], b2);
+                    u[j] = f2_mul(gated_factor2<T::kFast>(b2, Two<ST>::get(at[2 * R * 32])), xv);
                 } else {
                     F2 n;
                     logistic_pair2<T::kFast>(fv, a[j], n);
@@ -610,7 +644,8 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
         }
         float4(*set)[32] = runs[it & 1];
         const float2 y2 = f2_get(Y), p2 = f2_get(P);
-        set[warp][lane] = make_float4(y2.x, p2.x, y2.y, p2.y);
+        set[warp][lane] = make_float4(y2.x, y2.y, p2.x, p2.y);
+        if (lane == 0) cuts[it & 1][warp] = run.cut != 0u;
         gated_sync<T::W>();
         if (LOAD == kLoadTma && *abort_flag) return false;
         next();
@@ -619,23 +654,36 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
             Pair total = pair_identity();
 #pragma unroll
             for (int i = 0; i < T::W; ++i) {
-                const float2 r = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1];
-                total = join(total, Pair{r.x, r.y});
+                const float* r = reinterpret_cast<const float*>(&set[i][tid >> 1]) + (tid & 1);
+                total = join(total, Pair{r[0], r[2]});
             }
             gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
         }
-        Pair before[2] = {pair_identity(), pair_identity()};
+        // the warps in front of this one, joined; without a cut in the tile no selection is needed
+        F2 bY = f2(0.0f), bP = f2(1.0f);
+        const bool any_cut = gated_any<T::W>(cuts[it & 1]);
+        if (any_cut) {
+            Pair before[2] = {pair_identity(), pair_identity()};
+            for (int i = 0; i < warp; ++i) {
+                const float4 r = set[i][lane];
+                before[0] = join(before[0], Pair{r.x, r.z});
+                before[1] = join(before[1], Pair{r.y, r.w});
+            }
+            bY = f2(before[0].y, before[1].y);
+            bP = f2(before[0].p, before[1].p);
+        } else {
 #pragma unroll
-        for (int i = 0; i < T::W - 1; ++i) {
-            const float4 r = set[i][lane];
-            if (i < warp) {
-                before[0] = join(before[0], Pair{r.x, r.y});
-                before[1] = join(before[1], Pair{r.z, r.w});
+            for (int i = 0; i < T::W - 1; ++i) {
+                const float4 r = set[i][lane];
+                if (i < warp) {
+                    bY = f2_fma(bY, f2(r.z, r.w), f2(r.x, r.y));
+                    bP = f2_mul(bP, f2(r.z, r.w));
+                }
             }
         }
         if (w.first()) gated_sync<T::W>();
         const float* in = entering[it & 1];
-        F2 h = f2(enter(in[2 * lane], before[0]), enter(in[2 * lane + 1], before[1]));
+        F2 h = gated_enter(*reinterpret_cast<const float2*>(in + 2 * lane), bY, bP, any_cut);
         if (p.ckpt && s0 % kGatedCheckpoint == 0 && s0 < p.nrows)
             store_two<float>(p.ckpt, ((long long)w.b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h, false);
         const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
@@ -681,7 +729,8 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
     constexpr int K = T::K, R = T::R;
     static_assert(R == kGatedCheckpoint, "one checkpoint per tile");
     constexpr int kDy = (T::kArrays - 1) * R * 32;
-    __shared__ float4 runs[2][T::W][32];      // (Y, P) of both channels, forward direction
+    __shared__ float4 runs[2][T::W][32];      // every thread's Y of both channels, forward direction, then P
+    __shared__ int cuts[2][T::W];             // does a sequence start in a warp's run?
     __shared__ float2 back[2][T::W][32];      // Y of both channels, adjoint direction (same P)
     __shared__ __align__(8) float entering[2][kGatedChannels];      // tiles take turns
     __shared__ float2 dsum[T::W][32];
@@ -712,7 +761,9 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
             for (int j = 0; j < K; ++j, at += wstep) {
                 const F2 xv = Two<ST>::get(at[0]), fv = Two<ST>::get(at[R * 32]);
                 if (DECAY) {
-                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], bb[j]);
+                    F2 b2;
+                    decay_factors2<T::kFast, decltype(small)::value>(f2_mul(rate, logistic2<T::kFast>(fv)), a[j], b2);
+                    bb[j] = root2(b2);
                     add[j] = f2_mul(bb[j], f2_mul(logistic2<T::kFast>(Two<ST>::get(at[2 * R * 32])), xv));
                 } else {
                     logistic_pair2<T::kFast>(fv, a[j], bb[j]);
@@ -758,7 +809,8 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
         float4(*set)[32] = runs[it & 1];
         float2(*bset)[32] = back[it & 1];
         const float2 y2 = f2_get(Y), p2 = f2_get(P);
-        set[warp][lane] = make_float4(y2.x, p2.x, y2.y, p2.y);
+        set[warp][lane] = make_float4(y2.x, y2.y, p2.x, p2.y);
+        if (lane == 0) cuts[it & 1][warp] = run.cut != 0u;
         bset[warp][lane] = f2_get(q);
         gated_sync<T::W>();
         if (LOAD == kLoadTma && *abort_flag) return false;
@@ -768,33 +820,48 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
             Pair total = pair_identity();
 #pragma unroll
             for (int i = T::W - 1; i >= 0; --i) {
-                const float P = reinterpret_cast<const float2*>(&set[i][tid >> 1])[tid & 1].y;
+                const float P = reinterpret_cast<const float*>(&set[i][tid >> 1])[2 + (tid & 1)];
                 const float Y = reinterpret_cast<const float*>(&bset[i][tid >> 1])[tid & 1];
                 total = join(total, Pair{Y, P});
             }
             gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
         }
         // the state that enters this run, from the checkpoint
-        float hx = h0.x, hy = h0.y;
-        Pair after[2] = {pair_identity(), pair_identity()};
-#pragma unroll
-        for (int i = 0; i < T::W - 1; ++i) {
-            const float4 r = set[i][lane];
-            if (i < warp) {
-                hx = enter(hx, Pair{r.x, r.y});
-                hy = enter(hy, Pair{r.z, r.w});
+        F2 h = f2(h0.x, h0.y), aY = f2(0.0f), aP = f2(1.0f);
+        const bool any_cut = gated_any<T::W>(cuts[it & 1]);
+        if (any_cut) {
+            float hx = h0.x, hy = h0.y;
+            for (int i = 0; i < warp; ++i) {
+                const float4 r = set[i][lane];
+                hx = enter(hx, Pair{r.x, r.z});
+                hy = enter(hy, Pair{r.y, r.w});
             }
-        }
-#pragma unroll
-        for (int i = T::W - 1; i > 0; --i) {
-            const float4 r = set[i][lane];
-            const float2 y = bset[i][lane];
-            if (i > warp) {
-                after[0] = join(after[0], Pair{y.x, r.y});
+            h = f2(hx, hy);
+            Pair after[2] = {pair_identity(), pair_identity()};
+            for (int i = T::W - 1; i > warp; --i) {
+                const float4 r = set[i][lane];
+                const float2 y = bset[i][lane];
+                after[0] = join(after[0], Pair{y.x, r.z});
                 after[1] = join(after[1], Pair{y.y, r.w});
             }
+            aY = f2(after[0].y, after[1].y);
+            aP = f2(after[0].p, after[1].p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::W - 1; ++i) {
+                const float4 r = set[i][lane];
+                if (i < warp) h = f2_fma(h, f2(r.z, r.w), f2(r.x, r.y));
+            }
+#pragma unroll
+            for (int i = T::W - 1; i > 0; --i) {
+                const float4 r = set[i][lane];
+                const float2 y = bset[i][lane];
+                if (i > warp) {
+                    aY = f2_fma(aY, f2(r.z, r.w), f2(y.x, y.y));
+                    aP = f2_mul(aP, f2(r.z, r.w));
+                }
+            }
         }
-        F2 h = f2(hx, hy);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             if (edge && (run.cut >> j & 1u)) h = p.h0 && (run.start >> j & 1u) ? of_sequence(p.h0, j) : f2(0.0f);
@@ -804,7 +871,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
         }
         if (w.first()) gated_sync<T::W>();
         const float* in = entering[it & 1];
-        q = f2(enter(in[2 * lane], after[0]), enter(in[2 * lane + 1], after[1]));
+        q = gated_enter(*reinterpret_cast<const float2*>(in + 2 * lane), aY, aP, any_cut);
         if (w.first()) dl = f2(0.0f);
         const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
         const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
@@ -818,7 +885,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
             const F2 wb = f2_mul(grad, bb[j]);
             if (DECAY) {
                 F2 s, n;
-                logistic_pair2<T::kFast>(Two<ST>::get(at[R * 32]), s, n);
+                logistic_both2<T::kFast>(Two<ST>::get(at[R * 32]), s, n);
                 const float2 b = f2_get(bb[j]);
                 // -a/b, left out where the factor b has vanished (its share is the root of a log a below 1e-38)
                 const F2 minus_slope = f2_mul(a[j], f2(b.x > 0.0f ? -approx_rcp(b.x) : 0.0f, b.y > 0.0f ? -approx_rcp(b.y) : 0.0f));
