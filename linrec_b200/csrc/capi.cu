@@ -1153,6 +1153,43 @@ int static_scratch_address(void** out)
 namespace linrec_host {
 int device_facts(DeviceInfo& out) { return ::device_info(out); }
 int occupancy(const void* fn, int threads, size_t smem, int& out) { return ::occupancy(fn, threads, smem, out); }
+int active_clusters(const void* fn, int threads, size_t smem, int size, int& out)
+{
+    int dev = 0, occ = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return LINREC_ERR_CUDA;
+    // (the calling thread's own answers: no lock on the path every launch takes)
+    struct Known {
+        const void* fn;
+        int dev, size, n;
+    };
+    thread_local Known known[16] = {};
+    thread_local int next = 0;
+    for (const Known& k : known)
+        if (k.fn == fn && k.dev == dev && k.size == size) {
+            out = k.n;
+            return LINREC_OK;
+        }
+    const int rc = ::occupancy(fn, threads, smem, occ);      // raises the kernel's shared-memory limit
+    if (rc != LINREC_OK) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)size);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1u;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    out = 0;
+    if (cudaOccupancyMaxActiveClusters(&out, fn, &cfg) != cudaSuccess) {
+        ::note_cuda_error("cudaOccupancyMaxActiveClusters", cudaGetErrorString(cudaGetLastError()));
+        return LINREC_ERR_CUDA;
+    }
+    known[next] = Known{fn, dev, size, out};
+    next = (next + 1) % 16;
+    return LINREC_OK;
+}
 EncodeTiledFn encode_tiled_fn() { return ::encode_tiled_fn(); }
 void note_cuda_error(const char* where, const char* what) { ::note_cuda_error(where, what); }
 int launch_result(const char* where) { return ::launch_result(where); }

@@ -4,6 +4,7 @@
 #include "host.h"
 
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 
 namespace {
@@ -99,6 +100,26 @@ int tiles_per_job(long long units, int nk, long long slots)
     return want < nk ? want : nk;
 }
 
+// How many CTAs of a cluster share each column (0: not this way): as many as keep all columns running at a
+// time, if that fills a good part of the device.
+int cluster_size(const linrec_variants::GatedKernel& k, long long units, int nk, int sms, int& size)
+{
+    size = 0;
+    const char* e = getenv("GCL");
+    if (e && atoi(e) == 0) return LINREC_OK;
+    long long want = sms / units;
+    if (want > linrec::kGatedClusterMost) want = linrec::kGatedClusterMost;
+    if (want > nk) want = nk;
+    for (; want > 0; --want) {
+        int active = sms;      // of single CTAs, one per SM
+        const int rc = want == 1 ? LINREC_OK : linrec_host::active_clusters(reinterpret_cast<const void*>(k.fn), k.threads, (size_t)k.smem, (int)want, active);
+        if (rc != LINREC_OK) return rc;
+        if (active >= units) break;
+    }
+    if (want > 0) size = (int)want;
+    return LINREC_OK;
+}
+
 int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream_)
 {
     int rc = check(args);
@@ -162,19 +183,31 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
     }
     // as many columns as the small CTAs of an SM-filling grid, or fewer, larger ones
     const int shape = p.units < (bwd ? 2 : 3) * dev.sm_count;
-    const linrec_variants::GatedKernel kernel = a.dtype == LINREC_DTYPE_F32 ? linrec_variants::gated_kernel_f32(bwd, decay, load, shape)
-                                              : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::gated_kernel_bf16(bwd, decay, load, shape)
-                                                                             : linrec_variants::gated_kernel_f16(bwd, decay, load, shape);
+    auto pick = [&](int how) {
+        return a.dtype == LINREC_DTYPE_F32 ? linrec_variants::gated_kernel_f32(bwd, decay, how, shape)
+             : a.dtype == LINREC_DTYPE_BF16 ? linrec_variants::gated_kernel_bf16(bwd, decay, how, shape)
+                                            : linrec_variants::gated_kernel_f16(bwd, decay, how, shape);
+    };
+    linrec_variants::GatedKernel kernel = pick(load);
+    if (load == linrec::kLoadTma && p.units <= dev.sm_count) {
+        const linrec_variants::GatedKernel of_cluster = pick(linrec::kLoadCluster);
+        rc = cluster_size(of_cluster, p.units, linrec_host::ceil_div_i(ax.nrows, of_cluster.rows), dev.sm_count, p.cluster);
+        if (rc != LINREC_OK) return rc;
+        if (p.cluster > 0) {
+            load = linrec::kLoadCluster;
+            kernel = of_cluster;
+        }
+    }
     p.nk = linrec_host::ceil_div_i(ax.nrows, kernel.rows);
     int occ = 0;
     rc = linrec_host::occupancy(reinterpret_cast<const void*>(kernel.fn), kernel.threads, (size_t)kernel.smem, occ);
     if (rc != LINREC_OK) return rc;
     const long long slots = (long long)dev.sm_count * occ;
     p.tiles_per_job = tiles_per_job(p.units, p.nk, slots);
-    p.jobs = linrec_host::ceil_div_i(p.nk, p.tiles_per_job);
+    p.jobs = p.cluster > 0 ? p.cluster : linrec_host::ceil_div_i(p.nk, p.tiles_per_job);
     p.ntickets = (long long)p.jobs * p.units;
     linrec::GatedMaps maps{};
-    if (load == linrec::kLoadTma) {
+    if (linrec::gated_bulk(load)) {
         CUtensorMap* to[4] = {&maps.x, &maps.f, &maps.i, &maps.dy};
         for (int i = 0; i < 4; ++i) {
             if ((i == 2 && !decay) || (i == 3 && !bwd)) continue;
@@ -184,7 +217,10 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
     }
     long long grid = slots;
     if (grid > p.ntickets) grid = p.ntickets;
-    rc = linrec_host::launch("gated recurrence", kernel.fn, dim3((unsigned)grid), kernel.threads, (size_t)kernel.smem, stream, p, maps);
+    if (p.cluster > 0) grid = (long long)p.units * p.cluster;
+    // (a cluster of one is a plain CTA: it exchanges nothing)
+    rc = linrec_host::launch_clusters("gated recurrence", p.cluster > 1 ? p.cluster : 0, kernel.fn, dim3((unsigned)grid), (unsigned)kernel.threads,
+                                      (size_t)kernel.smem, stream, p, maps);
     if (rc != LINREC_OK || !bwd || !decay) return rc;
     return linrec_host::launch("decay gradient", linrec::gated_decay_grad_kernel, dim3((unsigned)linrec_host::ceil_div_i(a.nchan, 32)), 256, 0,
                                stream, (const float*)p.dlam, (long long)p.jobs * p.nb, p.D, p.decay, a.ddecay);

@@ -59,6 +59,7 @@ struct GatedParams {
     int nb;                             // axes (batch entries scanned side by side)
     int D, dtiles, units;               // units = nb * dtiles
     int nk, nck;                        // tiles, checkpoints per axis
+    int cluster;                        // kLoadCluster: CTAs that share a column
     int tiles_per_job, jobs;            // a ticket is a job: consecutive tiles of one column; jobs per column
     long long ntickets;                 // jobs * units
     int reverse;
@@ -244,26 +245,31 @@ __device__ __forceinline__ bool gated_await(const TileDesc* d, int n, uint4& w, 
 // then folds FORWARD from there, one tile after the other: the value is the one that the predecessors'
 // own chain of inclusive values gives, bit for bit, whichever of them were finished when it was read, so
 // results do not depend on timing.  `d` is the descriptor of tile k - 1; tile 0 is always inclusive.
-// Descriptors are requested a window at a time (independent loads, one round trip).
+// Descriptors are requested a window at a time, and a window with holes again as a whole: waiting for one
+// descriptor after the other costs a round trip for each.  The wait is bounded; on expiry the status word is flagged and nothing enters.
 __device__ __forceinline__ float gated_lookback(const TileDesc* d, long long stride, int k, uint32_t epoch, long long budget, uint32_t* status)
 {
     constexpr int W = 8;
     uint4 w[W];
-    int dist = 0;          // tiles k - 1, ..., k - dist hold aggregates
-    bool found = false;
-    while (!found) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = dist + i < k ? desc_load(d - (long long)(dist + i) * stride, epoch) : make_uint4(0u, 0u, 2u, 0u);
-        int here = 0;
+    int dist = 0;          // tiles k - 1, ..., k - dist are known to hold aggregates
+    const long long t0 = clock64();
+    while (true) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            if (found || dist + i >= k) continue;
-            if (!gated_await(d - (long long)(dist + i) * stride, k - 1 - dist - i, w[i], epoch, budget, status)) return 0.0f;
-            if (w[i].z == 2u) found = true;
+            if (dist + i >= k) w[i] = make_uint4(0u, 0u, 2u, 0u);
+            else w[i] = desc_load(d - (long long)(dist + i) * stride, epoch);
+        }
+        int here = 0;              // aggregates in front of the first inclusive value or hole
+        bool found = false, hole = false;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            // (a descriptor of this epoch that another job of the launch wrote cannot be: each has its own place)
+            if (found || hole) continue;
+            if (w[i].z == 0u) hole = true;
+            else if (w[i].z == 2u) found = true;
             else ++here;
         }
-        dist += here;
-        if (found && here == dist) {   // all of the walk is in this window
+        if (found && dist == 0) {
             float v = 0.0f;
 #pragma unroll
             for (int i = W - 1; i >= 0; --i) {
@@ -272,7 +278,18 @@ __device__ __forceinline__ float gated_lookback(const TileDesc* d, long long str
             }
             return v;
         }
-        if (dist >= k) return 0.0f;    // not reached: tile 0 is inclusive
+        if (found) {
+            dist += here;
+            break;
+        }
+        if (!hole) {
+            dist += W;
+        } else if (clock64() - t0 > budget) {
+            atomicOr(status, kStatusLookbackTimeout);
+            return 0.0f;
+        } else {
+            __nanosleep(100);
+        }
     }
     float v = __uint_as_float(desc_load(d - (long long)dist * stride, epoch).x);
     for (int far = dist - 1; far >= 0; far -= W) {
@@ -329,7 +346,12 @@ __device__ __forceinline__ void gated_carry(const GatedParams& p, const GatedWhe
 //               16-byte boundaries)
 //   kLoadWord   4-byte asynchronous copies, every thread its own words, one tile ahead (4-byte boundaries)
 //   kLoadAny    plain loads by the thread, stored to the same place (any alignment)
-constexpr int kLoadTma = 0, kLoadWord = 1, kLoadAny = 2;
+//   kLoadCluster  as kLoadTma, for fewer columns than SMs: the CTAs of a cluster take consecutive tiles of ONE column
+//               and tell one another their totals through shared memory, so that a column's carry never
+//               leaves its cluster and nobody looks back through global memory
+constexpr int kLoadTma = 0, kLoadWord = 1, kLoadAny = 2, kLoadCluster = 3;
+__host__ __device__ constexpr bool gated_bulk(int load) { return load == kLoadTma || load == kLoadCluster; }
+constexpr int kGatedClusterMost = 8;
 
 // Two shapes of a CTA.  SHAPE 0: four warps, several CTAs per SM, whose phases (gates, which the special
 // function unit bounds, and the exchange between warps, which latency bounds) overlap each other's.  SHAPE 1:
@@ -352,7 +374,7 @@ struct GatedTile {
     static constexpr int kStages = SHAPE && BWD ? 3 : 2;
     static constexpr int kDynSmem = kStages * kStageBytes;
     using Word = typename Two<ST>::Word;
-    static constexpr int threads(int load) { return (W + (load == kLoadTma ? 1 : 0)) * 32; }
+    static constexpr int threads(int load) { return (W + (gated_bulk(load) ? 1 : 0)) * 32; }
 };
 
 // A barrier of the warps that own positions.
@@ -361,6 +383,47 @@ __device__ __forceinline__ void gated_sync()
 {
     asm volatile("bar.sync 1, %0;" ::"n"(W * 32) : "memory");
 }
+
+// The totals of a cluster's turn: every CTA sends its 64 channels' (Y, P) to all of the cluster, each transfer
+// counted on the receiver's barrier.  Two sets take turns: a CTA sends its next but one total only after it
+// has received this CTA's next one, which is sent after this one's set has been read.
+struct GatedNoExchange {
+    __device__ __forceinline__ void open() {}
+};
+struct GatedExchange {
+    float2 totals[2][kGatedClusterMost][kGatedChannels];
+    uint64_t arrived[2];
+    int failed;      // a wait ran out: this launch's numbers are void, and it waits for nobody any more
+    __device__ __forceinline__ void open()
+    {
+        failed = 0;
+        ptx::mbar_init(&arrived[0], 1u);
+        ptx::mbar_init(&arrived[1], 1u);
+    }
+    // Run by 64 threads, one channel each: returns what enters this CTA's tile, `carry` is what entered the turn and
+    // becomes what enters the next.
+    __device__ __forceinline__ float turn(const GatedParams& p, uint32_t n, int tid, Pair total, float& carry)
+    {
+        float in = carry;
+        if (p.cluster == 1) {
+            carry = enter(carry, total);
+            return in;
+        }
+        const int set = (int)(n & 1u), rank = (int)(blockIdx.x % (unsigned)p.cluster);
+        if (tid == 0) ptx::mbar_arrive_expect_tx(&arrived[set], (uint32_t)(p.cluster * kGatedChannels * sizeof(float2)));
+        for (int c = 0; c < p.cluster; ++c) ptx::st_async_f32x2(&totals[set][rank][tid], &arrived[set], c, total.y, total.p);
+        if (!*(volatile int*)&failed && !ptx::mbar_wait_bounded_cluster(&arrived[set], (n >> 1) & 1u, p.wait_budget)) {
+            failed = 1;
+            atomicOr(p.header + 1, kStatusLookbackTimeout);
+        }
+        for (int c = 0; c < p.cluster; ++c) {
+            const float2 v = totals[set][c][tid];
+            if (c == rank) in = carry;
+            carry = enter(carry, Pair{v.x, v.y});
+        }
+        return in;
+    }
+};
 
 template <int W>
 __device__ __forceinline__ bool gated_any(const int* flags)
@@ -380,6 +443,21 @@ __device__ __forceinline__ F2 gated_enter(float2 in, F2 Y, F2 P, bool cut)
 struct GatedMaps {
     CUtensorMap x, f, i, dy;
 };
+
+// A cluster's turn t in a column: its CTA `rank` has tile t * cluster + rank (k = nk: none, the column is at its end).
+template <bool BWD>
+__device__ __forceinline__ GatedWhere gated_turn(const GatedParams& p, uint32_t column, int t, int rank)
+{
+    GatedWhere w;
+    w.job = 0;
+    w.b = (int)column / p.dtiles;
+    w.dt = (int)column - w.b * p.dtiles;
+    const int g = t * p.cluster + rank;
+    w.k = g >= p.nk ? p.nk : BWD ? p.nk - 1 - g : g;
+    if (t == 0) w.dt |= GatedWhere::kFirst;
+    if ((t + 1) * p.cluster >= p.nk) w.dt |= GatedWhere::kLast;
+    return w;
+}
 
 // A thread's own words of one tile, by asynchronous 4-byte copies or plain loads.
 template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD>
@@ -423,27 +501,40 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
 
 // The warp behind the others: draws tickets (one ahead, so that the counter's latency is hidden), issues the
 // copies, and evaluates the block's decay parameters, which the other warps find beside the operands.
-template <typename ST, bool DECAY, bool BWD, int SHAPE>
+template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD>
 __device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedMaps& maps, char* stages, uint64_t* full, uint64_t* empty,
                                               GatedWhere* items, float (*rates)[kGatedChannels], volatile int* abort_flag, uint32_t epoch)
 {
     using T = GatedTile<ST, DECAY, BWD, SHAPE>;
     const int lane = (int)threadIdx.x & 31;
     uint32_t ahead = 0, j = 0, ticket = 0;
-    if (lane == 0) ahead = atomicAdd(p.header, 1u);
+    if (LOAD != kLoadCluster && lane == 0) ahead = atomicAdd(p.header, 1u);
     bool gave_up = false, more = true;
+    const int rank = LOAD == kLoadCluster ? (int)(blockIdx.x % (unsigned)p.cluster) : 0;
+    const uint32_t clusters = LOAD == kLoadCluster ? gridDim.x / (unsigned)p.cluster : 1u;
+    uint32_t column = LOAD == kLoadCluster ? blockIdx.x / (unsigned)p.cluster : 0u;      // this cluster's columns: every `clusters`-th
     float rate[2] = {0.0f, 0.0f};
     GatedWhere w;
     w.dt = GatedWhere::kLast;
     for (int t = 0;; ++j, ++t) {
         const int s = (int)(j % T::kStages);
-        if (w.last()) {
-            t = 0;
-            ticket = __shfl_sync(0xffffffffu, ahead, 0);
-            more = (long long)ticket < p.ntickets;
-            if (more && lane == 0) ahead = atomicAdd(p.header, 1u);
+        if (LOAD == kLoadCluster) {
+            // (a job is the whole column, its tiles are dealt out to the cluster's CTAs in turn)
+            if (j > 0 && w.last()) {
+                t = 0;
+                column += clusters;
+            }
+            more = column < (uint32_t)p.units;
+            w = gated_turn<BWD>(p, column, t, rank);
+        } else {
+            if (w.last()) {
+                t = 0;
+                ticket = __shfl_sync(0xffffffffu, ahead, 0);
+                more = (long long)ticket < p.ntickets;
+                if (more && lane == 0) ahead = atomicAdd(p.header, 1u);
+            }
+            w = gated_where<BWD>(p, ticket, t);
         }
-        w = gated_where<BWD>(p, ticket, t);
         const int block = w.block() * kGatedChannels;
         if (DECAY && more && w.first()) {
 #pragma unroll
@@ -462,7 +553,7 @@ __device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedM
         }
         if (lane == 0) {
             items[s] = more ? w : GatedWhere{-1, 0, 0, 0};
-            if (more) {
+            if (more && w.k < p.nk) {
                 const int row = p.reverse ? (int)(p.nrows - (long long)(w.k + 1) * T::R) : w.k * T::R;
                 char* to = stages + s * T::kStageBytes;
                 ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
@@ -483,14 +574,14 @@ __device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedM
         for (uint32_t i = j > (uint32_t)T::kStages ? j - T::kStages : 0u; i < j; ++i)
             (void)ptx::mbar_wait_bounded(&full[i % T::kStages], (i / T::kStages) & 1u, p.wait_budget);
     }
-    if (lane == 0) finish_launch(p.header, epoch);
+    if (LOAD != kLoadCluster && lane == 0) finish_launch(p.header, epoch);
 }
 
 // What both passes have in common: the pipeline of tiles around `body`, which calls `next` behind its first
 // barrier (where a stage is free: forward its own, backward the one of the tile before) and returns false to
 // stop (all threads alike).
-template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD, typename Body>
-__device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMaps& maps, Body body)
+template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD, typename Exchange, typename Body>
+__device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMaps& maps, Exchange& exchange, Body body)
 {
     using T = GatedTile<ST, DECAY, BWD, SHAPE>;
     using Word = typename T::Word;
@@ -504,7 +595,7 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
     __shared__ int abort_flag;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    if (LOAD == kLoadTma) {
+    if (gated_bulk(LOAD)) {
         if (tid == 0) {
 #pragma unroll
             for (int s = 0; s < T::kStages; ++s) {
@@ -513,13 +604,19 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
                 items[s] = GatedWhere{0, 0, 0, 0};
             }
             abort_flag = 0;
+            exchange.open();
             ptx::fence_mbar_init();
         }
         __syncthreads();
+        if (LOAD == kLoadCluster && p.cluster > 1) ptx::cluster_sync();      // the others' barriers exist
         ptx::grid_dependency_wait();
-        const uint32_t epoch = read_epoch(p.header);
+        const uint32_t epoch = LOAD == kLoadCluster ? 0u : read_epoch(p.header);
         if (warp == T::W) {
-            gated_produce<ST, DECAY, BWD, SHAPE>(p, maps, stages, full, empty, items, rates, &abort_flag, epoch);
+            gated_produce<ST, DECAY, BWD, SHAPE, LOAD>(p, maps, stages, full, empty, items, rates, &abort_flag, epoch);
+            if (LOAD == kLoadCluster && p.cluster > 1) {
+                __syncwarp();
+                ptx::cluster_sync();      // nobody sends here any more
+            }
             return;
         }
         for (uint32_t it = 0;; ++it) {
@@ -538,6 +635,10 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
                                  },
                                  (volatile int*)&abort_flag);
             if (!on) break;
+        }
+        if (LOAD == kLoadCluster && p.cluster > 1) {
+            __syncwarp();
+            ptx::cluster_sync();
         }
         return;
     }
@@ -589,14 +690,16 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
     __shared__ __align__(8) float entering[2][kGatedChannels];      // tiles take turns
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    gated_tiles<ST, DECAY, false, SHAPE, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
+    __shared__ __align__(16) std::conditional_t<LOAD == kLoadCluster, GatedExchange, GatedNoExchange> exchange;
+    float carry = 0.0f;      // of a cluster's column, in the 64 threads that link
+    gated_tiles<ST, DECAY, false, SHAPE, LOAD>(p, maps, exchange, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
                                                      const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
         const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
         TileDesc* desc = p.desc + (((long long)w.job * p.units + w.b * p.dtiles + w.block()) * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
+        if (LOAD != kLoadCluster && tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
         const GatedRun run = gated_run<K>(p, w.b, s0, lane);
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
@@ -647,7 +750,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
         set[warp][lane] = make_float4(y2.x, y2.y, p2.x, p2.y);
         if (lane == 0) cuts[it & 1][warp] = run.cut != 0u;
         gated_sync<T::W>();
-        if (LOAD == kLoadTma && *abort_flag) return false;
+        if (gated_bulk(LOAD) && *abort_flag) return false;
         next();
 
         if (tid < kGatedChannels) {
@@ -657,7 +760,12 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
                 const float* r = reinterpret_cast<const float*>(&set[i][tid >> 1]) + (tid & 1);
                 total = join(total, Pair{r[0], r[2]});
             }
-            gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
+            if constexpr (LOAD == kLoadCluster) {
+                if (w.first()) carry = 0.0f;
+                entering[it & 1][tid] = exchange.turn(p, it, tid, total, carry);
+            } else {
+                gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
+            }
         }
         // the warps in front of this one, joined; without a cut in the tile no selection is needed
         F2 bY = f2(0.0f), bP = f2(1.0f);
@@ -681,12 +789,12 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
                 }
             }
         }
-        if (w.first()) gated_sync<T::W>();
+        if (LOAD == kLoadCluster || w.first()) gated_sync<T::W>();
         const float* in = entering[it & 1];
         F2 h = gated_enter(*reinterpret_cast<const float2*>(in + 2 * lane), bY, bP, any_cut);
         if (p.ckpt && s0 % kGatedCheckpoint == 0 && s0 < p.nrows)
             store_two<float>(p.ckpt, ((long long)w.b * p.nck + s0 / kGatedCheckpoint) * p.D + ch, have, h, false);
-        const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
+        const bool pair = (gated_bulk(LOAD) || p.pair) && have > 1;
         const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
         ST* y = static_cast<ST*>(p.y) + row0 * p.D + ch;
         const long long ystep = p.reverse ? -(long long)p.D : p.D;
@@ -727,7 +835,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
 {
     using T = GatedTile<ST, DECAY, true, SHAPE>;
     constexpr int K = T::K, R = T::R;
-    static_assert(R == kGatedCheckpoint, "one checkpoint per tile");
+    static_assert(R % kGatedCheckpoint == 0, "a checkpoint where a tile starts");
     constexpr int kDy = (T::kArrays - 1) * R * 32;
     __shared__ float4 runs[2][T::W][32];      // every thread's Y of both channels, forward direction, then P
     __shared__ int cuts[2][T::W];             // does a sequence start in a warp's run?
@@ -738,15 +846,17 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
 
     F2 dl = f2(0.0f);      // this thread's share of the decay gradient, over a job
 
-    gated_tiles<ST, DECAY, true, SHAPE, LOAD>(p, maps, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
+    __shared__ __align__(16) std::conditional_t<LOAD == kLoadCluster, GatedExchange, GatedNoExchange> exchange;
+    float carry = 0.0f;      // of a cluster's column, in the 64 threads that link
+    gated_tiles<ST, DECAY, true, SHAPE, LOAD>(p, maps, exchange, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
                                                     const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
         const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
         TileDesc* desc = p.desc + (((long long)w.job * p.units + w.b * p.dtiles + w.block()) * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
-        if (tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
-        const float2 h0 = f2_get(load_state(p.ckpt, ((long long)w.b * p.nck + w.k) * p.D + ch, have));
+        if (LOAD != kLoadCluster && tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
+        const float2 h0 = f2_get(load_state(p.ckpt, ((long long)w.b * p.nck + (long long)w.k * (R / kGatedCheckpoint)) * p.D + ch, w.k < p.nk ? have : 0));
         const GatedRun run = gated_run<K>(p, w.b, s0, lane);
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
@@ -813,7 +923,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
         if (lane == 0) cuts[it & 1][warp] = run.cut != 0u;
         bset[warp][lane] = f2_get(q);
         gated_sync<T::W>();
-        if (LOAD == kLoadTma && *abort_flag) return false;
+        if (gated_bulk(LOAD) && *abort_flag) return false;
         next();
 
         if (tid < kGatedChannels) {
@@ -824,7 +934,12 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
                 const float Y = reinterpret_cast<const float*>(&bset[i][tid >> 1])[tid & 1];
                 total = join(total, Pair{Y, P});
             }
-            gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
+            if constexpr (LOAD == kLoadCluster) {
+                if (w.first()) carry = 0.0f;
+                entering[it & 1][tid] = exchange.turn(p, it, tid, total, carry);
+            } else {
+                gated_carry(p, w, desc, seen, total, epoch, &entering[it & 1][tid], &entering[(it + 1) & 1][tid]);
+            }
         }
         // the state that enters this run, from the checkpoint
         F2 h = f2(h0.x, h0.y), aY = f2(0.0f), aP = f2(1.0f);
@@ -869,11 +984,11 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
             h = f2_fma(a[j], before, add[j]);
             add[j] = before;
         }
-        if (w.first()) gated_sync<T::W>();
+        if (LOAD == kLoadCluster || w.first()) gated_sync<T::W>();
         const float* in = entering[it & 1];
         q = gated_enter(*reinterpret_cast<const float2*>(in + 2 * lane), aY, aP, any_cut);
         if (w.first()) dl = f2(0.0f);
-        const bool pair = (LOAD == kLoadTma || p.pair) && have > 1;
+        const bool pair = (gated_bulk(LOAD) || p.pair) && have > 1;
         const long long row0 = (long long)w.b * p.nrows + (p.reverse ? p.nrows - 1 - s0 : s0);
         const long long at0 = row0 * p.D + ch, astep = p.reverse ? -(long long)p.D : p.D;
         // gradients of element j; q becomes what flows on to the element before it
@@ -935,7 +1050,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
                 float s = 0.0f;
 #pragma unroll
                 for (int i = 0; i < T::W; ++i) s += reinterpret_cast<const float*>(&dsum[i][tid >> 1])[tid & 1];
-                p.dlam[((long long)w.b * p.jobs + w.job) * p.D + w.block() * kGatedChannels + tid] = s;
+                p.dlam[((long long)w.b * p.jobs + (LOAD == kLoadCluster ? (int)(blockIdx.x % (unsigned)p.cluster) : w.job)) * p.D + w.block() * kGatedChannels + tid] = s;
             }
         }
         return true;

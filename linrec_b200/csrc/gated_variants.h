@@ -34,9 +34,11 @@ GatedKernel gated_pick(bool bwd, int load, int shape)
     using namespace linrec;
     if constexpr (sizeof(ST) == 4) {
         // 32-bit elements always lie on 4-byte boundaries
+        if (load == kLoadCluster) return gated_pick<ST, DECAY, 1, kLoadCluster>(bwd);
         if (load == kLoadTma) return gated_pick<ST, DECAY, 1, kLoadTma>(bwd);
         return gated_pick<ST, DECAY, 1, kLoadWord>(bwd);
     } else {
+        if (load == kLoadCluster) return gated_pick<ST, DECAY, 1, kLoadCluster>(bwd);
         if (load == kLoadTma) return shape ? gated_pick<ST, DECAY, 1, kLoadTma>(bwd) : gated_pick<ST, DECAY, 0, kLoadTma>(bwd);
         if (load == kLoadWord) return gated_pick<ST, DECAY, 0, kLoadWord>(bwd);
         return gated_pick<ST, DECAY, 0, kLoadAny>(bwd);

@@ -23,6 +23,8 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
 int device_facts(DeviceInfo& out);
 // Resident CTAs per SM; the first query for a kernel also raises its dynamic shared-memory limit.
 int occupancy(const void* fn, int threads, size_t smem, int& out);
+// Clusters of `size` CTAs that can be resident at a time.
+int active_clusters(const void* fn, int threads, size_t smem, int size, int& out);
 EncodeTiledFn encode_tiled_fn();
 void note_cuda_error(const char* where, const char* what);
 // Result of a kernel launch: reads (and clears) the runtime's last error.
@@ -34,22 +36,31 @@ inline int ceil_div_i(long long a, long long b) { return (int)((a + b - 1) / b);
 // Launch with the programmatic-stream-serialization attribute: the kernels call griddepcontrol.wait before
 // their first access to global memory (ptx.cuh).
 template <typename... KArgs, typename... Args>
-int launch(const char* where, void (*fn)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args)
+int launch_clusters(const char* where, int cluster, void (*fn)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1u;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 0 ? 2 : 1;
     (void)cudaLaunchKernelEx(&cfg, fn, static_cast<Args&&>(args)...);
     const int rc = launch_result(where);
     if (rc == LINREC_OK) count_launch();
     return rc;
+}
+
+template <typename... KArgs, typename... Args>
+int launch(const char* where, void (*fn)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t stream, Args&&... args)
+{
+    return launch_clusters(where, 0, fn, grid, block, smem, stream, static_cast<Args&&>(args)...);
 }
 
 }  // namespace linrec_host

@@ -70,6 +70,44 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
     }
 }
 
+// ---- thread-block clusters -----------------------------------------------------------------------
+// All threads of all CTAs of the cluster (the CTAs of a cluster run together, so it ends).
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Stores a pair of floats to the place that `dst` has in the shared memory of the cluster's CTA `rank`, counted as 8
+// bytes on that CTA's `bar`.
+__device__ __forceinline__ void st_async_f32x2(void* dst, uint64_t* bar, int rank, float x, float y)
+{
+    asm volatile(
+        "{\n\t.reg .b32 d, b;\n\t"
+        "mapa.shared::cluster.u32 d, %0, %2;\n\t"
+        "mapa.shared::cluster.u32 b, %1, %2;\n\t"
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [d], {%3, %4}, [b];\n\t}"
+        ::"r"(smem_u32(dst)), "r"(smem_u32(bar)), "r"(rank), "f"(x), "f"(y)
+        : "memory");
+}
+
+// mbar_wait_bounded for a barrier that other CTAs of the cluster complete.
+__device__ __forceinline__ bool mbar_wait_bounded_cluster(uint64_t* bar, uint32_t parity, long long budget)
+{
+    const long long t0 = clock64();
+    while (true) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (clock64() - t0 > budget) return false;
+    }
+}
+
 // ---- tiled bulk-tensor copies (rank 3) ---------------------------------------------------------
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
                                             int c0, int c1, int c2)
