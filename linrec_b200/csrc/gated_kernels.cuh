@@ -473,27 +473,44 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
 #pragma unroll
     for (int a = 0; a < T::kArrays; ++a) {
         const ST* from = static_cast<const ST*>(src[a]) + ch;
-#pragma unroll
-        for (int j = 0; j < T::K; ++j) {
+        auto place = [&](int j) {
             const int sl = warp * T::K + j, r = p.reverse ? T::R - 1 - sl : sl;
-            typename Two<ST>::Word* to = stage + (a * T::R + r) * 32 + lane;
-            const ST* at = from + (row0 + (long long)j * step) * stride[a];
-            const bool in = s0 + j < p.nrows;
-            if (LOAD == kLoadWord) {
+            return stage + (a * T::R + r) * 32 + lane;
+        };
+        auto at = [&](int j) { return from + (row0 + (long long)j * step) * stride[a]; };
+        if (LOAD == kLoadWord) {
+#pragma unroll
+            for (int j = 0; j < T::K; ++j) {
+                const bool in = s0 + j < p.nrows;
+                typename Two<ST>::Word* to = place(j);
                 if (sizeof(ST) == 4) {
-                    if (in && have > 0) ptx::cp_async_4(to, at);
-                    if (in && have > 1) ptx::cp_async_4(reinterpret_cast<char*>(to) + 4, at + 1);
+                    if (in && have > 0) ptx::cp_async_4(to, at(j));
+                    if (in && have > 1) ptx::cp_async_4(reinterpret_cast<char*>(to) + 4, at(j) + 1);
                 } else if (in && have > 1) {
-                    ptx::cp_async_4(to, at);
+                    ptx::cp_async_4(to, at(j));
                 } else if (in && have > 0) {   // the last channel of an odd number
                     float v[2];
-                    load_two<ST>(at, 0, have, v);
+                    load_two<ST>(at(j), 0, have, v);
                     *to = Two<ST>::pack(v);
                 }
-            } else {
-                float v[2] = {0.0f, 0.0f};
-                if (in) load_two<ST>(at, 0, have, v);
-                *to = Two<ST>::pack(v);
+            }
+        } else {
+            // eight rows at a time: all of their loads, then all of their stores
+#pragma unroll
+            for (int j0 = 0; j0 < T::K; j0 += 8) {
+                ST v[8][2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool in = s0 + j0 + j < p.nrows;
+                    v[j][0] = v[j][1] = from_f32<ST>(0.0f);
+                    if (in && have > 0) v[j][0] = __ldg(at(j0 + j));
+                    if (in && have > 1) v[j][1] = __ldg(at(j0 + j) + 1);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float f[2] = {to_f32<ST>(v[j][0]), to_f32<ST>(v[j][1])};
+                    *place(j0 + j) = Two<ST>::pack(f);
+                }
             }
         }
     }
