@@ -273,12 +273,12 @@ int64_t linrec_b200_gated_checkpoint_rows(const linrec_gated_args* args)
 
 int linrec_b200_gated_fwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream)
 {
-    return launch_gated(false, args, opts, workspace, workspace_bytes, stream);
+    return linrec_host::guarded([&] { return launch_gated(false, args, opts, workspace, workspace_bytes, stream); });
 }
 
 int linrec_b200_gated_bwd(const linrec_gated_args* args, const linrec_opts* opts, void* workspace, size_t workspace_bytes, void* stream)
 {
-    return launch_gated(true, args, opts, workspace, workspace_bytes, stream);
+    return linrec_host::guarded([&] { return launch_gated(true, args, opts, workspace, workspace_bytes, stream); });
 }
 
 int linrec_b200_gated_step(const void* x, const void* forget, const void* input_gate, int64_t x_stride, int64_t forget_stride,
@@ -286,28 +286,30 @@ int linrec_b200_gated_step(const void* x, const void* forget, const void* input_
                            int64_t state_stride, int64_t nslots, const void* slots, int slots_are_64, int64_t nrows, int64_t nchan,
                            int dtype, void* stream)
 {
-    if (!known_dtype(dtype)) return LINREC_ERR_NOT_IMPLEMENTED;
-    if (nrows < 0 || nchan < 0 || nslots < 0 || nrows >= 0x7fffffffLL || nslots >= 0x7fffffffLL || nchan > 128LL * 65535)
-        return LINREC_ERR_INVALID_ARG;
-    if (!decay != !input_gate) return LINREC_ERR_INVALID_ARG;
-    if (nrows == 0 || nchan == 0) return LINREC_OK;
-    if (!x || !forget || !y || (!state && nslots > 0) || x_stride < nchan || forget_stride < nchan || state_stride < nchan ||
-        (decay && input_gate_stride < nchan) || (!slots && nrows > nslots))
-        return LINREC_ERR_INVALID_ARG;
-    DeviceInfo dev;
-    const int rc = linrec_host::device_facts(dev);
-    if (rc != LINREC_OK) return rc;
-    GatedStepParams p{};
-    p.x = x; p.f = forget; p.ig = input_gate; p.sx = x_stride; p.sf = forget_stride; p.si = input_gate_stride;
-    p.y = y; p.decay = decay; p.scale = decay_scale; p.state = state; p.sstate = state_stride;
-    p.slots = slots; p.slots64 = slots_are_64; p.rows = (int)nrows; p.nslots = (int)nslots; p.D = (int)nchan;
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
-    const bool four = nchan % 4 == 0 && on_boundary(x, x_stride, size, 4 * size) && on_boundary(forget, forget_stride, size, 4 * size) &&
-                      (!decay || on_boundary(input_gate, input_gate_stride, size, 4 * size)) && on_boundary(y, nchan, size, 4 * size) &&
-                      on_boundary(state, state_stride, 4, 16);
-    return dtype == LINREC_DTYPE_F32 ? launch_step<float>(p, four, dev.sm_count, s)
-         : dtype == LINREC_DTYPE_BF16 ? launch_step<__nv_bfloat16>(p, four, dev.sm_count, s) : launch_step<__half>(p, four, dev.sm_count, s);
+    return linrec_host::guarded([&]() -> int {
+        if (!known_dtype(dtype)) return LINREC_ERR_NOT_IMPLEMENTED;
+        if (nrows < 0 || nchan < 0 || nslots < 0 || nrows >= 0x7fffffffLL || nslots >= 0x7fffffffLL || nchan > 128LL * 65535)
+            return LINREC_ERR_INVALID_ARG;
+        if (!decay != !input_gate) return LINREC_ERR_INVALID_ARG;
+        if (nrows == 0 || nchan == 0) return LINREC_OK;
+        if (!x || !forget || !y || (!state && nslots > 0) || x_stride < nchan || forget_stride < nchan || state_stride < nchan ||
+            (decay && input_gate_stride < nchan) || (!slots && nrows > nslots))
+            return LINREC_ERR_INVALID_ARG;
+        DeviceInfo dev;
+        const int rc = linrec_host::device_facts(dev);
+        if (rc != LINREC_OK) return rc;
+        GatedStepParams p{};
+        p.x = x; p.f = forget; p.ig = input_gate; p.sx = x_stride; p.sf = forget_stride; p.si = input_gate_stride;
+        p.y = y; p.decay = decay; p.scale = decay_scale; p.state = state; p.sstate = state_stride;
+        p.slots = slots; p.slots64 = slots_are_64; p.rows = (int)nrows; p.nslots = (int)nslots; p.D = (int)nchan;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
+        const bool four = nchan % 4 == 0 && on_boundary(x, x_stride, size, 4 * size) && on_boundary(forget, forget_stride, size, 4 * size) &&
+                          (!decay || on_boundary(input_gate, input_gate_stride, size, 4 * size)) && on_boundary(y, nchan, size, 4 * size) &&
+                          on_boundary(state, state_stride, 4, 16);
+        return dtype == LINREC_DTYPE_F32 ? launch_step<float>(p, four, dev.sm_count, s)
+             : dtype == LINREC_DTYPE_BF16 ? launch_step<__nv_bfloat16>(p, four, dev.sm_count, s) : launch_step<__half>(p, four, dev.sm_count, s);
+    });
 }
 
 }  // extern "C"

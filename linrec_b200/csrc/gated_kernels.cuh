@@ -116,16 +116,16 @@ __device__ __forceinline__ F2 root2(F2 v)
     return f2(approx_sqrt(w.x), approx_sqrt(w.y));
 }
 // b s(i).  Fast: with d = 1 + e^-i it is b^2 / sqrt(b^2 d^2), one special function for a root and a reciprocal
-// (they bound the forward pass).  The tiny term keeps b = 0 from giving NaN: b is then taken as 1e-18.
+// (they bound the forward pass); a gate that is shut, b = 0, gives exactly nothing.
 template <bool FAST>
 __device__ __forceinline__ F2 gated_factor2(F2 b2, F2 i)
 {
     if (FAST) {
         const float2 t = f2_get(f2_mul(i, f2(-1.44269504f)));
         const F2 d = f2_add(f2(approx_exp2(t.x), approx_exp2(t.y)), f2(1.0f));
-        const F2 q = f2_add(b2, f2(1e-36f));
-        const float2 r = f2_get(f2_mul(f2_mul(q, d), d));
-        return f2_mul(q, f2(approx_rsqrt(r.x), approx_rsqrt(r.y)));
+        const float2 q = f2_get(b2), r = f2_get(f2_mul(f2_mul(b2, d), d));
+        const float2 g = f2_get(f2_mul(b2, f2(approx_rsqrt(r.x), approx_rsqrt(r.y))));
+        return f2(q.x > 0.0f ? g.x : 0.0f, q.y > 0.0f ? g.y : 0.0f);
     }
     return f2_mul(root2(b2), logistic2<false>(i));
 }

@@ -31,6 +31,18 @@ void note_cuda_error(const char* where, const char* what);
 int launch_result(const char* where);
 void count_launch();
 
+// Body of a C entry point: no C++ exception leaves it.
+template <typename Body>
+int guarded(Body body) noexcept
+{
+    try {
+        return body();
+    } catch (...) {
+        note_cuda_error("host", "out of memory or another C++ exception");
+        return LINREC_ERR_CUDA;
+    }
+}
+
 inline int ceil_div_i(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Launch with the programmatic-stream-serialization attribute: the kernels call griddepcontrol.wait before

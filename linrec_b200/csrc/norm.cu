@@ -177,7 +177,7 @@ size_t linrec_b200_group_norm_scratch_size(const linrec_group_norm_args* args, i
     return most;
 }
 
-int linrec_b200_group_norm_fwd(const linrec_group_norm_args* args, void* stream) { return launch_norm(false, args, stream); }
-int linrec_b200_group_norm_bwd(const linrec_group_norm_args* args, void* stream) { return launch_norm(true, args, stream); }
+int linrec_b200_group_norm_fwd(const linrec_group_norm_args* args, void* stream) { return linrec_host::guarded([&] { return launch_norm(false, args, stream); }); }
+int linrec_b200_group_norm_bwd(const linrec_group_norm_args* args, void* stream) { return linrec_host::guarded([&] { return launch_norm(true, args, stream); }); }
 
 }  // extern "C"

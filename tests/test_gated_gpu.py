@@ -163,6 +163,59 @@ def test_extreme_logits(decay):
         _check(t, (want[n][0], want[n][1] + 2e-15), n)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("value", ["inf", "lowest"])
+def test_masked_rows_hold_the_state(dtype, value):
+    """Logits of minus infinity, or of the type's lowest value: the decay form keeps its state to the bit and takes
+    nothing in, the forget form replaces it; of plus infinity the forget form keeps it."""
+    lb = _lb()
+    low = -float("inf") if value == "inf" else torch.finfo(dtype).min
+    g = torch.Generator().manual_seed(1)
+    x, i, h0 = torch.randn(2, 200, 72, generator=g).to(DEV, dtype), torch.randn(2, 200, 72, generator=g).to(DEV, dtype), torch.randn(2, 72, generator=g).to(DEV)
+    i[:, 5:9] = low
+    d = torch.linspace(-6.0, 3.0, 72, device=DEV)
+    for state in (h0, torch.zeros_like(h0)):
+        shut = torch.full_like(x, low)
+        y, end = lb.linrec_gated(x, shut, input_gate=i, decay=d, initial_state=state, return_state=True)
+        assert torch.equal(end, state) and torch.equal(y, state[:, None].to(dtype).expand_as(y))
+        y, end = lb.linrec_gated(x, -shut, initial_state=state, return_state=True)
+        assert torch.equal(end, state) and torch.equal(y, state[:, None].to(dtype).expand_as(y))
+        y, end = lb.linrec_gated(x, shut, initial_state=state, return_state=True)
+        assert torch.equal(y, x) and torch.equal(end, x[:, -1].float())
+        one = state.clone()
+        assert torch.equal(lb.linrec_gated_step(x[:, 0], shut[:, 0], one, input_gate=i[:, 0], decay=d), state.to(dtype))
+        assert torch.equal(one, state)
+    # a masked stretch in the middle of a sequence: the rows around it do not notice
+    f = torch.randn(2, 200, 72, generator=g).to(DEV, dtype)
+    f[:, 60:140] = low
+    keep = torch.ones(200, dtype=torch.bool, device=DEV)
+    keep[60:140] = False
+    whole, end = lb.linrec_gated(x, f, input_gate=i, decay=d, initial_state=h0, return_state=True)
+    short, end2 = lb.linrec_gated(x[:, keep], f[:, keep], input_gate=i[:, keep], decay=d, initial_state=h0, return_state=True)
+    # (tiles begin elsewhere, so products of multipliers round elsewhere)
+    assert torch.allclose(whole[:, keep].float(), short.float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-5)
+    assert torch.allclose(end, end2, rtol=1e-4, atol=1e-5)
+    # held: a run of positions is entered through the joined runs before it, fewer than 20 products and sums of terms
+    # below 10, each rounded: 20 * 10 * 2^-24 = 1.2e-5
+    assert torch.allclose(whole[:, 60:140].float(), whole[:, 59:60].float().expand(-1, 80, -1), rtol=torch.finfo(dtype).eps, atol=1.2e-5)
+
+
+def test_inference_mode():
+    lb = _lb()
+    with torch.inference_mode():
+        c = {k: v.to(DEV) for k, v in _case((3, 40, 64), True, torch.bfloat16).items()}
+        y, end = lb.linrec_gated(c["inputs"], c["forget"], input_gate=c["input_gate"], decay=c["decay"], return_state=True)
+        z = lb.linrec_gated_step(c["inputs"][:, 0], c["forget"][:, 0], end, input_gate=c["input_gate"][:, 0], decay=c["decay"])
+        assert torch.isfinite(lb.group_norm_act(z, 4)).all()
+
+
+def test_expanded_gradient():
+    """The gradient of a sum is one number seen everywhere."""
+    c = _case((2, 130, 72), True, torch.float32, states=False)
+    c["dy"] = torch.ones(2, 130, 72)
+    _compare(_run(c, lambda k, t: torch.ones((), device=DEV).expand(t.shape) if k == "dy" else t.to(DEV)), _oracle(c))
+
+
 def test_differences():
     """Gradients against central differences of the 64-bit evaluation."""
     for decay in (False, True):
