@@ -51,7 +51,7 @@ Plan plan_of(const linrec_group_norm_args& a, bool aligned, bool bwd)
         p.rp = slots / p.gb;
         p.xblocks = linrec_host::ceil_div_i(a.groups, p.gb);
         // as many CTAs as are resident at a time, so that all of them take the same number of rows
-        const long long ctas = 148 * (p.V == 1 ? (p.many ? 3 : 4) : p.many ? (bwd ? 1 : 2) : bwd ? 3 : 4);
+        const long long ctas = 148 * (p.V == 1 ? (p.many ? 3 : 4) : p.many ? (bwd ? 1 : 2) : bwd ? 2 : 4);
         const long long want = ctas / p.xblocks > 0 ? ctas / p.xblocks : 1, most = (a.nsamples + p.rp - 1) / p.rp;
         p.yblocks = p.parts = most < want ? most : want;
         return p;

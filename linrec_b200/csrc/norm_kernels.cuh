@@ -191,8 +191,10 @@ __device__ __forceinline__ NormSlot norm_slot(const NormParams& p)
     return s;
 }
 
-// NV pieces of eight elements per lane.  With one piece the next row's operands are requested before this row
-// is worked on, as they come (four registers for eight elements).
+// NV pieces of eight elements per lane.  The next row's operands are in flight while a row is worked on, as they come
+// (four registers for eight elements).  Bytes in flight bound both passes: forward four CTAs per SM with one row
+// ahead (three with two: 80 us instead of 79 at (16384, 4096) bf16 with gate, fp32 86 instead of 70), backward two CTAs
+// with two rows ahead (three with one: 160 us instead of 128).
 template <typename ST, int NV, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_kernel(const NormParams p)
 {
@@ -215,31 +217,30 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_k
     const long long step = (long long)gridDim.y * p.rp;
     long long n = (long long)blockIdx.y * p.rp + s.r;
     const float count = 1.0f / (float)p.c;
-    Eight<ST> rx[NV], rg[NV];
-    auto fetch = [&](long long row) {
+    constexpr int kAhead = 1;
+    Eight<ST> rx[kAhead][NV], rg[kAhead][NV];
+    auto fetch = [&](int set, long long row) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            rx[i].clear();
+            rx[set][i].clear();
             if (have[i] && row < p.n) {
-                rx[i].load(p.x, row * p.sx + ch[i]);
-                if (GATE) rg[i].load(p.gate, row * p.sg + ch[i]);
+                rx[set][i].load(p.x, row * p.sx + ch[i]);
+                if (GATE) rg[set][i].load(p.gate, row * p.sg + ch[i]);
             }
         }
     };
-    fetch(n);
-    // (all threads of a CTA take the same number of turns: the shuffles need whole warps)
-    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
+    auto turn = [&](int set) {
         F2 x[NV][4];
         Eight<ST> gate[NV];
         F2 sum = f2(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            rx[i].get(x[i]);
-            if (GATE) gate[i] = rg[i];
+            rx[set][i].get(x[i]);
+            if (GATE) gate[i] = rg[set][i];
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum = f2_add(sum, x[i][e]);
         }
-        fetch(n + step);
+        fetch(set, n + kAhead * step);
         const float mean = lanes_sum(f2_sum(sum), p.lanes) * count;
         F2 sq = f2(0.0f);
 #pragma unroll
@@ -266,7 +267,14 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_k
                     store_eight<ST>(p.y, n * p.C + ch[i], y);
                 }
         }
-    }
+        n += step;
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(k, n + k * step);
+    // (all threads of a CTA take the same number of turns: the shuffles need whole warps)
+    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += kAhead * step)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) turn(k);
 }
 
 // One element per access, NV per lane (rows off 16-byte boundaries, or groups that are not whole sixteens of bytes).
@@ -323,7 +331,7 @@ __device__ __forceinline__ void norm_rows_leave(const NormParams& p, const float
 }
 
 template <typename ST, int NV, bool GATE, int ACT>
-__global__ void __launch_bounds__(kNormThreads, NV == 1 ? 3 : 1) norm_rows_bwd_kernel(const NormParams p)
+__global__ void __launch_bounds__(kNormThreads, NV == 1 ? 2 : 1) norm_rows_bwd_kernel(const NormParams p)
 {
     constexpr bool kFast = sizeof(ST) == 2;
     extern __shared__ __align__(16) float2 norm_sums[];
@@ -347,30 +355,30 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 3 : 1) norm_rows_bwd_k
     const long long step = (long long)gridDim.y * p.rp;
     const float count = 1.0f / (float)p.c;
     long long n = (long long)blockIdx.y * p.rp + s.r;
-    Eight<ST> rx[NV], rg[NV], rd[NV];
-    float2 rst = make_float2(0.0f, 0.0f);
-    auto fetch = [&](long long row) {
-        if (row < p.n && s.active) rst = p.stats[row * p.G + s.g];
+    constexpr int kAhead = NV == 1 ? 2 : 1;
+    Eight<ST> rx[kAhead][NV], rg[kAhead][NV], rd[kAhead][NV];
+    float2 rst[kAhead];
+    auto fetch = [&](int set, long long row) {
+        rst[set] = row < p.n && s.active ? __ldg(p.stats + row * p.G + s.g) : make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (have[i] && row < p.n) {
-                rx[i].load(p.x, row * p.sx + ch[i]);
-                rd[i].load(p.dy, row * p.sdy + ch[i]);
-                if (GATE) rg[i].load(p.gate, row * p.sg + ch[i]);
+                rx[set][i].load(p.x, row * p.sx + ch[i]);
+                rd[set][i].load(p.dy, row * p.sdy + ch[i]);
+                if (GATE) rg[set][i].load(p.gate, row * p.sg + ch[i]);
             } else {
-                rx[i].clear(), rd[i].clear(), rg[i].clear();
+                rx[set][i].clear(), rd[set][i].clear(), rg[set][i].clear();
             }
         }
     };
-    fetch(n);
-    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += step, n += step) {
+    auto turn = [&](int set) {
         const bool row = n < p.n;
-        const float2 st = rst;
+        const float2 st = rst[set];
         F2 xhat[NV][4], k[NV][4], s1 = f2(0.0f), s2 = f2(0.0f);
         Eight<ST> cx[NV], cg[NV], cd[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) cx[i] = rx[i], cg[i] = rg[i], cd[i] = rd[i];
-        fetch(n + step);
+        for (int i = 0; i < NV; ++i) cx[i] = rx[set][i], cg[i] = rg[set][i], cd[i] = rd[set][i];
+        fetch(set, n + kAhead * step);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             F2 x[4], gt[4], dy[4], dg[4];
@@ -398,7 +406,13 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 3 : 1) norm_rows_bwd_k
                 for (int e = 0; e < 4; ++e) dx[e] = f2_mul(f2_fma(xhat[i][e], f2(-m2), f2_add(k[i][e], f2(-m1))), f2(st.y));
                 store_eight<ST>(p.dx, n * p.C + ch[i], dx);
             }
-    }
+        n += step;
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) fetch(k, n + k * step);
+    for (long long base = (long long)blockIdx.y * p.rp; base < p.n; base += kAhead * step)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) turn(k);
     if (!p.part) return;
     const int c0 = (int)blockIdx.x * p.gb * p.c, nch = min(p.gb * p.c, p.C - c0);
     float2* out = p.rp == 1 ? p.part + (long long)blockIdx.y * p.C : norm_sums + s.r * nch - c0;
