@@ -516,11 +516,87 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
     }
 }
 
+// What GatedRun says, for all positions of a tile, found by the warp that issues the copies (a search through the
+// offsets is 1600 cycles of round trips, which the other warps would all stand still for) and left beside them.
+// Used in clusters, where a column's tiles follow one another (packed (16384, 4096): 280 / 662 us without, 253 /
+// 607 with); where tickets are drawn the launch gets slower by it ((4, 4096, 4096) fp32: 128 / 240 us without).
+template <int R>
+struct GatedMarks {
+    uint32_t start[R / 32], end[R / 32], valid[R / 32];
+    int seq[R];
+    // Run by a warp: lane l has positions l, 32 + l, ...; their searches go step by step together.
+    __device__ __forceinline__ void find(const GatedParams& p, int b, long long s0, int lane)
+    {
+        constexpr int N = R / 32;
+        int q[N];
+        bool ok[N], st[N], en[N];
+        if (p.cu) {
+            int lo[N], hi[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) lo[i] = 0, hi[i] = p.nseq + 1;
+            for (int step = 32 - __clz(p.nseq + 1); step > 0; --step)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const long long s = s0 + 32 * i + lane, row = p.reverse ? p.nrows - 1 - s : s;
+                    const int mid = (lo[i] + hi[i]) >> 1;
+                    if (lo[i] < hi[i]) {
+                        if (gated_offset(p, mid) <= row) lo[i] = mid + 1;
+                        else hi[i] = mid;
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const long long s = s0 + 32 * i + lane, row = p.reverse ? p.nrows - 1 - s : s;
+                q[i] = lo[i] - 1;
+                ok[i] = s < p.nrows && q[i] >= 0 && q[i] < p.nseq;
+                const long long first = ok[i] ? gated_offset(p, q[i]) : 0, last = ok[i] ? gated_offset(p, q[i] + 1) - 1 : 0;
+                st[i] = ok[i] && row == (p.reverse ? last : first);
+                en[i] = ok[i] && row == (p.reverse ? first : last);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const long long s = s0 + 32 * i + lane;
+                ok[i] = s < p.nrows;
+                long long n = b, o = s;
+                if (p.nb == 1 && p.seqlen < p.nrows) {
+                    n = s / p.seqlen;
+                    o = s - n * p.seqlen;
+                    if (p.reverse) n = p.nseq - 1 - n;
+                }
+                q[i] = (int)n;
+                st[i] = ok[i] && o == 0;
+                en[i] = ok[i] && o == p.seqlen - 1;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t a = __ballot_sync(0xffffffffu, st[i]), c = __ballot_sync(0xffffffffu, en[i]), v = __ballot_sync(0xffffffffu, ok[i]);
+            if (lane == 0) start[i] = a, end[i] = c, valid[i] = v;
+            seq[32 * i + lane] = q[i];
+        }
+    }
+    template <int K>
+    __device__ __forceinline__ GatedRun run(int warp, int lane) const
+    {
+        constexpr uint32_t kMask = (1u << K) - 1u;
+        const int word = warp * K >> 5, shift = warp * K & 31;
+        GatedRun r;
+        r.start = start[word] >> shift & kMask;
+        r.end = end[word] >> shift & kMask;
+        r.valid = valid[word] >> shift & kMask;
+        r.cut = (r.start | ~r.valid) & kMask;
+        r.seq = (r.start | r.end) ? seq[warp * K + (lane & (K - 1))] : 0;
+        return r;
+    }
+};
+
 // The warp behind the others: draws tickets (one ahead, so that the counter's latency is hidden), issues the
 // copies, and evaluates the block's decay parameters, which the other warps find beside the operands.
 template <typename ST, bool DECAY, bool BWD, int SHAPE, int LOAD>
 __device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedMaps& maps, char* stages, uint64_t* full, uint64_t* empty,
-                                              GatedWhere* items, float (*rates)[kGatedChannels], volatile int* abort_flag, uint32_t epoch)
+                                              GatedWhere* items, GatedMarks<GatedTile<ST, DECAY, BWD, SHAPE>::R>* marks,
+                                              float (*rates)[kGatedChannels], volatile int* abort_flag, uint32_t epoch)
 {
     using T = GatedTile<ST, DECAY, BWD, SHAPE>;
     const int lane = (int)threadIdx.x & 31;
@@ -573,14 +649,21 @@ __device__ __forceinline__ void gated_produce(const GatedParams& p, const GatedM
             if (more && w.k < p.nk) {
                 const int row = p.reverse ? (int)(p.nrows - (long long)(w.k + 1) * T::R) : w.k * T::R;
                 char* to = stages + s * T::kStageBytes;
-                ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
+                if (LOAD == kLoadCluster) ptx::mbar_expect_tx(&full[s], (uint32_t)T::kStageBytes);
+                else ptx::mbar_arrive_expect_tx(&full[s], (uint32_t)T::kStageBytes);
                 ptx::tma_load_3d(to, &maps.x, &full[s], block, row, w.b);
                 ptx::tma_load_3d(to + T::kArrayBytes, &maps.f, &full[s], block, row, w.b);
                 if (DECAY) ptx::tma_load_3d(to + 2 * T::kArrayBytes, &maps.i, &full[s], block, row, w.b);
                 if (BWD) ptx::tma_load_3d(to + (T::kArrays - 1) * T::kArrayBytes, &maps.dy, &full[s], block, row, w.b);
-            } else {
+            } else if (LOAD != kLoadCluster) {
                 ptx::mbar_arrive(&full[s]);
             }
+        }
+        if (LOAD == kLoadCluster) {
+            if (more) marks[s].find(p, w.b, (long long)w.k * T::R, lane);
+            // the arrival that lets the stage be used once the copies have landed as well
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&full[s]);
         }
         if (!more) break;
     }
@@ -609,6 +692,7 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
     __shared__ uint32_t tickets[2];
     __shared__ __align__(16) GatedWhere items[T::kStages];
     __shared__ __align__(8) float rates[T::kStages][kGatedChannels];
+    __shared__ GatedMarks<T::R> marks[LOAD == kLoadCluster ? T::kStages : 1];
     __shared__ int abort_flag;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -629,7 +713,7 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
         ptx::grid_dependency_wait();
         const uint32_t epoch = LOAD == kLoadCluster ? 0u : read_epoch(p.header);
         if (warp == T::W) {
-            gated_produce<ST, DECAY, BWD, SHAPE, LOAD>(p, maps, stages, full, empty, items, rates, &abort_flag, epoch);
+            gated_produce<ST, DECAY, BWD, SHAPE, LOAD>(p, maps, stages, full, empty, items, marks, rates, &abort_flag, epoch);
             if (LOAD == kLoadCluster && p.cluster > 1) {
                 __syncwarp();
                 ptx::cluster_sync();      // nobody sends here any more
@@ -646,6 +730,10 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
             const int4 item = *reinterpret_cast<const int4*>(&items[s]);
             if (item.x < 0) break;
             const bool on = body(GatedWhere{item.x, item.y, item.z, item.w}, it, epoch, reinterpret_cast<const Word*>(stages + s * T::kStageBytes), rates[s],
+                                 [&] {
+                                     if constexpr (LOAD == kLoadCluster) return marks[s].template run<T::K>(warp, lane);
+                                     else return gated_run<T::K>(p, item.z, (long long)item.x * T::R + warp * T::K, lane);
+                                 },
                                  [&] {
                                      const uint32_t done = BWD ? it - 1u : it;
                                      if (tid == 0 && (!BWD || it > 0)) ptx::mbar_arrive(&empty[done % T::kStages]);
@@ -689,7 +777,8 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
         if (more) gated_fetch<ST, DECAY, BWD, SHAPE, LOAD>(p, next, reinterpret_cast<Word*>(stages + ((it + 1) & 1) * T::kStageBytes), warp, lane);
         ptx::cp_async_commit();
         ptx::cp_async_wait_group<1>();
-        body(w, it, epoch, reinterpret_cast<const Word*>(stages + (it & 1) * T::kStageBytes), rates[it & 1], [] {}, (volatile int*)&abort_flag);
+        body(w, it, epoch, reinterpret_cast<const Word*>(stages + (it & 1) * T::kStageBytes), rates[it & 1],
+             [&] { return gated_run<T::K>(p, w.b, (long long)w.k * T::R + warp * T::K, lane); }, [] {}, (volatile int*)&abort_flag);
         w = next;
     }
     if (tid == 0) finish_launch(p.header, epoch);
@@ -710,14 +799,14 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
     __shared__ __align__(16) std::conditional_t<LOAD == kLoadCluster, GatedExchange, GatedNoExchange> exchange;
     float carry = 0.0f;      // of a cluster's column, in the 64 threads that link
     gated_tiles<ST, DECAY, false, SHAPE, LOAD>(p, maps, exchange, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
-                                                     const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
+                                                     const typename T::Word* stage, const float* rates, auto marked, auto next, volatile int* abort_flag) {
         const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
         TileDesc* desc = p.desc + (((long long)w.job * p.units + w.b * p.dtiles + w.block()) * kGatedChannels + tid);
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
         if (LOAD != kLoadCluster && tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
-        const GatedRun run = gated_run<K>(p, w.b, s0, lane);
+        const GatedRun run = marked();
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
 
@@ -866,7 +955,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
     __shared__ __align__(16) std::conditional_t<LOAD == kLoadCluster, GatedExchange, GatedNoExchange> exchange;
     float carry = 0.0f;      // of a cluster's column, in the 64 threads that link
     gated_tiles<ST, DECAY, true, SHAPE, LOAD>(p, maps, exchange, [&](const GatedWhere& w, uint32_t it, uint32_t epoch,
-                                                    const typename T::Word* stage, const float* rates, auto next, volatile int* abort_flag) {
+                                                    const typename T::Word* stage, const float* rates, auto marked, auto next, volatile int* abort_flag) {
         const int ch = w.block() * kGatedChannels + 2 * lane;
         const int have = p.D - ch;
         const long long s0 = (long long)w.k * R + warp * K;
@@ -874,7 +963,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
         uint4 seen = make_uint4(0u, 0u, 0u, 0u);
         if (LOAD != kLoadCluster && tid < kGatedChannels && w.job > 0 && w.first()) seen = desc_load(desc - (long long)p.units * kGatedChannels, epoch);
         const float2 h0 = f2_get(load_state(p.ckpt, ((long long)w.b * p.nck + (long long)w.k * (R / kGatedCheckpoint)) * p.D + ch, w.k < p.nk ? have : 0));
-        const GatedRun run = gated_run<K>(p, w.b, s0, lane);
+        const GatedRun run = marked();
         const typename T::Word* words = stage + (p.reverse ? R - 1 - warp * K : warp * K) * 32 + lane;
         const int wstep = p.reverse ? -32 : 32;
         F2 rate = f2(0.0f);
