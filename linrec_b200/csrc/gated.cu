@@ -180,6 +180,9 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
                  (!on_boundary(in[i], stride[i], size, 16) || !p.pair || (double)stride[i] * size * (double)ax.nrows >= 1e12))
             load = linrec::kLoadWord;
     }
+    // (4-byte copies of 16-bit rows, two bytes to a channel, are slower than plain loads, eight rows of them at a time:
+    // (4, 4096, 4002) bf16 forget form 197 / 559 us and 181 / 455)
+    if (load == linrec::kLoadWord && size == 2) load = linrec::kLoadAny;
     // as many columns as the small CTAs of an SM-filling grid, or fewer, larger ones
     const int shape = p.units < (bwd ? 2 : 3) * dev.sm_count;
     auto pick = [&](int how) {

@@ -344,8 +344,8 @@ __device__ __forceinline__ void gated_carry(const GatedParams& p, const GatedWhe
 // positions:
 //   kLoadTma    one bulk-tensor copy per operand through a ring of stages, issued by a warp of its own (rows on
 //               16-byte boundaries)
-//   kLoadWord   4-byte asynchronous copies, every thread its own words, one tile ahead (4-byte boundaries)
-//   kLoadAny    plain loads by the thread, stored to the same place (any alignment)
+//   kLoadWord   32-bit elements: 4-byte asynchronous copies, every thread its own words, one tile ahead
+//   kLoadAny    16-bit elements: plain loads by the thread, stored to the same place
 //   kLoadCluster  as kLoadTma, for fewer columns than SMs: the CTAs of a cluster take consecutive tiles of ONE column
 //               and tell one another their totals through shared memory, so that a column's carry never
 //               leaves its cluster and nobody looks back through global memory
@@ -483,16 +483,8 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
             for (int j = 0; j < T::K; ++j) {
                 const bool in = s0 + j < p.nrows;
                 typename Two<ST>::Word* to = place(j);
-                if (sizeof(ST) == 4) {
-                    if (in && have > 0) ptx::cp_async_4(to, at(j));
-                    if (in && have > 1) ptx::cp_async_4(reinterpret_cast<char*>(to) + 4, at(j) + 1);
-                } else if (in && have > 1) {
-                    ptx::cp_async_4(to, at(j));
-                } else if (in && have > 0) {   // the last channel of an odd number
-                    float v[2];
-                    load_two<ST>(at(j), 0, have, v);
-                    *to = Two<ST>::pack(v);
-                }
+                if (in && have > 0) ptx::cp_async_4(to, at(j));
+                if (in && have > 1) ptx::cp_async_4(reinterpret_cast<char*>(to) + 4, at(j) + 1);
             }
         } else {
             // eight rows at a time: all of their loads, then all of their stores

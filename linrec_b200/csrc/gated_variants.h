@@ -40,7 +40,6 @@ GatedKernel gated_pick(bool bwd, int load, int shape)
     } else {
         if (load == kLoadCluster) return gated_pick<ST, DECAY, 1, kLoadCluster>(bwd);
         if (load == kLoadTma) return shape ? gated_pick<ST, DECAY, 1, kLoadTma>(bwd) : gated_pick<ST, DECAY, 0, kLoadTma>(bwd);
-        if (load == kLoadWord) return gated_pick<ST, DECAY, 0, kLoadWord>(bwd);
         return gated_pick<ST, DECAY, 0, kLoadAny>(bwd);
     }
 }

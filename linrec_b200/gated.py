@@ -25,11 +25,12 @@ import functools
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .norm import _as_float, _as_rows, _check_cuda, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
+from .norm import _as_float, _as_rows, _backward_once, _check_cuda, _empty_dense, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
 from .ops import _DTYPES, _workspace
+
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 __all__ = ["linrec_gated", "linrec_gated_step", "linrec_gated_norm", "linrec_gated_norm_step"]
 
@@ -67,7 +68,7 @@ def _check_index(name: str, t) -> None:
 def _scratch(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """The stream's workspace.  Inside a graph capture a fresh one that belongs to the graph: graphs that
     were captured on one stream may be replayed side by side on others."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     return _workspace(device, stream, nbytes)
 
@@ -127,7 +128,7 @@ def _states_like(other, shape, device, always: bool):
 
 def _forward(inputs, forget, input_gate, decay, initial, cu, scale, reverse, want_state, want_checkpoints):
     p = _Problem(inputs, forget, input_gate, decay, initial, cu, scale, reverse)
-    y = torch.empty(inputs.shape, dtype=p.dtype, device=p.device)
+    y = _empty_dense(inputs)
     p.args.y = y.data_ptr()
     final = checkpoints = None
     if want_state:
@@ -150,8 +151,7 @@ class _GatedFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return y, final
 
-    @staticmethod
-    @once_differentiable
+    @_backward_once
     def backward(ctx, dy, dfinal):
         inputs, forget, input_gate, decay, initial, cu, checkpoints = ctx.saved_tensors
         if dy is None and dfinal is None:
@@ -164,12 +164,11 @@ class _GatedFn(torch.autograd.Function):
         if dfinal is not None:
             dfinal = dfinal.contiguous()
             a.d_final_state = dfinal.data_ptr()
-        dx = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
-        df = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
+        dx, df = _empty_dense(inputs), _empty_dense(inputs)
         a.dx, a.dforget = dx.data_ptr(), df.data_ptr()
         di = ddecay = dinitial = scratch = None
         if decay is not None:
-            di = torch.empty(inputs.shape, dtype=p.dtype, device=dev)
+            di = _empty_dense(inputs)
             ddecay = torch.empty_like(decay) if p.nrows else torch.zeros_like(decay)
             scratch = torch.empty(p.sizes[1] * p.D, dtype=torch.float32, device=dev)
             a.dinput_gate, a.ddecay = di.data_ptr(), ddecay.data_ptr()
@@ -257,7 +256,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
     _check_cuda(inputs, forget, input_gate, decay, state, slots)
     if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")
-    y = torch.empty((rows, D), dtype=inputs.dtype, device=inputs.device)
+    y = _empty_dense(inputs)
     if y.numel() == 0:
         return y
     x, sx = _as_rows(inputs)

@@ -22,6 +22,7 @@ __all__ = ["group_norm_act"]
 
 _STORAGE = (torch.float32, torch.bfloat16, torch.float16)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 
 
@@ -69,9 +70,24 @@ def _wants_grad(*ts) -> bool:
     return False
 
 
+def _empty_dense(t: torch.Tensor) -> torch.Tensor:
+    """A dense tensor of the sizes and type of `t`."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _backward_once(raw):
+    """`once_differentiable(raw)` without its bookkeeping where no gradient of the gradient was asked for."""
+    refusing = once_differentiable(raw)
+
+    def backward(ctx, *grads):
+        return (refusing if torch.is_grad_enabled() else raw)(ctx, *grads)
+
+    return staticmethod(backward)
+
+
 def _on(device: torch.device, launch) -> None:
     """`launch(stream)` with `device` current."""
-    if torch.cuda.current_device() == device.index:
+    if _current_device() == device.index:
         launch(_raw_stream(device.index))
     else:
         with torch.cuda.device(device):
@@ -103,7 +119,7 @@ def _call(bwd, x, gate, weight, bias, groups, act, eps, stats, y=None, dy=None, 
 
 
 def _forward(x, gate, weight, bias, groups, act, eps, want_stats):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty_dense(x)
     stats = torch.empty(x.size(0) * groups * 2, dtype=torch.float32, device=x.device) if want_stats else None
     if y.numel():
         _call(False, x, gate, weight, bias, groups, act, eps, stats, y=y)
@@ -118,13 +134,11 @@ class _GroupNormFn(torch.autograd.Function):
         ctx.args = (groups, act, eps)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_backward_once
     def backward(ctx, dy):
         x, gate, weight, bias, stats = ctx.saved_tensors
-        dev = x.device
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dgate = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = _empty_dense(x)
+        dgate = None if gate is None else _empty_dense(x)
         make = torch.empty_like if x.numel() else torch.zeros_like
         dw = make(weight) if weight is not None and ctx.needs_input_grad[2] else None
         db = make(bias) if bias is not None and ctx.needs_input_grad[3] else None
