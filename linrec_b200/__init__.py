@@ -27,6 +27,6 @@ from .norm import group_norm_act  # noqa: E402,F401
 
 linrec = linrec_pipe
 
-__version__ = "0.2.0"
+__version__ = "0.3.0"
 __all__ = ["linrec", "linrec_ref", "linrec_tile", "linrec_pipe", "linrec_general", "linrec_gated", "linrec_gated_step",
            "group_norm_act", "linrec_gated_norm", "linrec_gated_norm_step", "check_status"]

@@ -1536,6 +1536,6 @@ const char* linrec_b200_strerror(int code)
     }
 }
 
-int linrec_b200_version(void) { return 200; }
+int linrec_b200_version(void) { return 300; }
 
 }  // extern "C"

@@ -90,9 +90,9 @@ int make_map(CUtensorMap* map, const void* ptr, int64_t stride, const GatedParam
 }
 
 // How many consecutive tiles of a column one CTA takes.  Jobs of four tiles where there are about as many
-// columns as CTAs at least (a job waits for its predecessor, handed out `units` jobs earlier: (8, 4096, 4096)
-// forward, 512 columns on 444 CTAs, 306 us as single tiles, 247 in fours, 259 in eights); fewer columns are
-// single tiles linked by decoupled look-back ((1, 32768, 2048), 32 columns: 240 us, 530 in fours).
+// columns as CTAs at least (a job waits for its predecessor, handed out `units` jobs earlier); when it was chosen (8, 4096, 4096)
+// forward, 512 columns on 444 CTAs, took 306 us as single tiles, 247 in fours, 259 in eights (now 228 in fours).
+// Fewer columns are single tiles linked by decoupled look-back ((1, 32768, 2048), 32 columns, then: 240 us, 530 in fours).
 int tiles_per_job(long long units, int nk, long long slots)
 {
     const int want = 7 * units >= 6 * slots ? 4 : 1;
@@ -181,7 +181,7 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
             load = linrec::kLoadWord;
     }
     // (4-byte copies of 16-bit rows, two bytes to a channel, are slower than plain loads, eight rows of them at a time:
-    // (4, 4096, 4002) bf16 forget form 197 / 559 us and 181 / 455)
+    // (4, 4096, 4002) bf16 forget form 197 / 559 us and 173 / 347)
     if (load == linrec::kLoadWord && size == 2) load = linrec::kLoadAny;
     // as many columns as the small CTAs of an SM-filling grid, or fewer, larger ones
     const int shape = p.units < (bwd ? 2 : 3) * dev.sm_count;

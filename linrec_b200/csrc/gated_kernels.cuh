@@ -13,13 +13,13 @@
 // rules tells ragged from dense, so the tiles are the same size whatever the lengths are.  Positions are
 // counted in scan order; a reversed scan only changes the memory row a position stands for.
 //
-// A tile is 64 channels x R positions for one CTA of eight warps: a lane owns two adjacent channels, a
-// warp K consecutive positions, kept in registers as (a, b u) pairs, so that the gates are evaluated
-// once.  Each thread folds its run into a (P, Y) pair, the eight runs meet in shared memory, and 64
-// threads link the tile to its predecessor along the axis by decoupled look-back (one 16-byte descriptor
-// per channel and tile; tickets are handed out position-major, so the predecessor is `units` tickets
-// older and a wait is only ever for a ticket that a running CTA holds).  The runs are then walked again
-// from the true state.  Reads and writes every element once.
+// A tile is 64 channels x R positions for one CTA of four or eight warps: a lane owns two adjacent channels, a
+// warp K consecutive positions, kept in registers as (a, b u) pairs.  Each thread folds its run into a (P, Y)
+// pair, the warps' runs meet in shared memory, and the tile is linked to its predecessor along the axis: by the CTA
+// itself within a job of tiles, by the cluster's shared memory, or by decoupled look-back (one 16-byte
+// descriptor per channel and job; tickets are handed out position-major, so the predecessor is `units`
+// tickets older and a wait is only ever for a ticket that a running CTA holds).  The runs are then walked
+// again from the true state.  Reads and writes every element once.
 //
 // The cut is carried as a multiplier of minus zero, which products of multipliers (all >= 0) keep, and it
 // selects rather than multiplies: 0 * NaN would let one sequence's infinities into its neighbour.
@@ -357,8 +357,9 @@ constexpr int kGatedClusterMost = 8;
 // function unit bounds, and the exchange between warps, which latency bounds) overlap each other's.  SHAPE 1:
 // eight warps and longer tiles, one CTA per SM: half as many tiles wait for one another along a column, which
 // counts when there are few columns, and it is the shape that fits 32-bit operands.
-// Measured, forward / backward us, 16-bit decay form: (8, 4096, 4096), 512 columns: 247 / 614 and 292 / 689;
-// (1, 32768, 2048), 32 columns: 269 / 735 and 240 / 598.
+// Measured when both linked tiles by look-back and jobs alone, forward / backward us, 16-bit decay form:
+// (8, 4096, 4096), 512 columns: 247 / 614 and 292 / 689; (1, 32768, 2048), 32 columns: 269 / 735 and 240 / 598.
+// The sides that are taken now measure 228 / 559 and, in clusters, 170 / 427.
 template <typename ST, bool DECAY, bool BWD, int SHAPE>
 struct GatedTile {
     static constexpr bool kFast = sizeof(ST) == 2;                     // 16-bit results: fast exponentials will do
@@ -510,8 +511,8 @@ __device__ __forceinline__ void gated_fetch(const GatedParams& p, const GatedWhe
 
 // What GatedRun says, for all positions of a tile, found by the warp that issues the copies (a search through the
 // offsets is 1600 cycles of round trips, which the other warps would all stand still for) and left beside them.
-// Used in clusters, where a column's tiles follow one another (packed (16384, 4096): 280 / 662 us without, 253 /
-// 607 with); where tickets are drawn the launch gets slower by it ((4, 4096, 4096) fp32: 128 / 240 us without).
+// Used in clusters, where a column's tiles follow one another (packed (16384, 4096): forward 286 us without,
+// 256 with); where tickets are drawn the launch gets slower by it ((4, 4096, 4096) fp32: 128 / 240 us without).
 template <int R>
 struct GatedMarks {
     uint32_t start[R / 32], end[R / 32], valid[R / 32];
@@ -777,6 +778,9 @@ __device__ __forceinline__ void gated_tiles(const GatedParams& p, const GatedMap
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
+// 6 (forget) or 8 (decay) bytes per element in 16 bits.  (8, 4096, 4096) bf16: 168 us (4.8 TB/s) and 228 us (4.7 TB/s).
+// Decay form there: issue 61 %, special functions 53 %, DRAM 55 % busy, 37 instructions per element; in the other shape
+// ((4, 4096, 4096)) 46, 44 and 44 %.  Latency between them bounds it, no unit alone.
 template <typename ST, bool DECAY, int SHAPE, int LOAD>
 __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LOAD), GatedTile<ST, DECAY, false, SHAPE>::kCtas)
     gated_fwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
@@ -927,6 +931,9 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
 // ---- backward -----------------------------------------------------------------------------------------
 // Between the two halves of a tile a thread keeps a, b and the state in front of each of its elements; x, dy
 // and the logits stay in shared memory and what else is needed is evaluated again from them.
+// 10 or 14 bytes per element in 16 bits.  (8, 4096, 4096) bf16: forget 347 us (3.9 TB/s), decay 559 us (3.4 TB/s).
+// Decay form there: issue 47 %, special functions 54 %, DRAM 40 % busy, 71 instructions per element; in the other shape
+// ((4, 4096, 4096)) 44, 43 and 31 %, 82 instructions.
 template <typename ST, bool DECAY, int SHAPE, int LOAD>
 __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOAD), GatedTile<ST, DECAY, true, SHAPE>::kCtas)
     gated_bwd_kernel(const GatedParams p, const __grid_constant__ GatedMaps maps)
@@ -1227,6 +1234,8 @@ constexpr int kStepThreads = 128;
 // the search below.
 // A slot that several rows name holds ONE sequence whose tokens are the rows in order: the first of them walks
 // through all, the others leave them to it.  Every CTA compares its rows' slots with all rows'.
+// (512, 8192) bf16 replayed in a graph: decay form with slots 17.5 us (31.8 before rows shared a CTA),
+// forget form without 8.1 us (7.2 TB/s, above the copy bandwidth: part of it comes from L2).
 template <typename ST, bool DECAY, int V, int ROWS>
 __global__ void __launch_bounds__(kStepThreads) gated_step_kernel(const GatedStepParams p)
 {

@@ -5,7 +5,7 @@
 // Backward, with dz the gradient that reaches z and k = dz w:
 //   dx = inv (k - mean(k) - xhat mean(k xhat)),   dgate = dy z act'(gate),   dw = sum dz xhat,   db = sum dz
 //
-// Two ways, both bound by memory:
+// Two ways:
 //   rows     one position per sample (what follows a recurrence) and groups of up to 1024 channels.  A group
 //            stays in the registers of the 1 to 32 lanes that hold it, the sums are shuffles; everything is
 //            read once and written once.  A thread keeps its channels from row to row, so that weights are
@@ -194,7 +194,7 @@ __device__ __forceinline__ NormSlot norm_slot(const NormParams& p)
 // NV pieces of eight elements per lane.  The next row's operands are in flight while a row is worked on, as they come
 // (four registers for eight elements).  Bytes in flight bound both passes: forward four CTAs per SM with one row
 // ahead (three with two: 80 us instead of 79 at (16384, 4096) bf16 with gate, fp32 86 instead of 70), backward two CTAs
-// with two rows ahead (three with one: 160 us instead of 128).
+// with two rows ahead (three with one: 160 us instead of 128).  So measured: 79 us (5.1 TB/s), issue slots 72 %, DRAM 54 % busy.
 template <typename ST, int NV, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_kernel(const NormParams p)
 {
@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_k
 }
 
 // One element per access, NV per lane (rows off 16-byte boundaries, or groups that are not whole sixteens of bytes).
+// (16384, 4098) bf16 with gate, 6 groups: 441 us forward, 460 backward, 0.9 and 1.5 TB/s.
 template <typename ST, int NV, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_fwd_kernel(const NormParams p)
 {
