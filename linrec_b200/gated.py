@@ -28,6 +28,7 @@ import torch
 
 from . import _capi
 from .norm import _as_float, _as_rows, _backward_once, _check_cuda, _empty_dense, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
+from .norm import _apply as _apply_norm, _check as _check_norm
 from .ops import _DTYPES, _workspace
 
 _capturing = torch._C._cuda_isCurrentStreamCapturing
@@ -293,5 +294,6 @@ def linrec_gated_norm_step(inputs: torch.Tensor, forget: torch.Tensor, gate: tor
                            activation: str | None = "silu", eps: float = 1e-5, **recurrence) -> torch.Tensor:
     """`linrec_gated_norm` for one token per row: `linrec_gated_step`, then the norm and the gate.  A padding
     row's norm is that of zeros, act of the bias times the gate."""
+    _check_norm(inputs, groups, weight, bias, gate, activation, eps)      # before the state moves
     h = linrec_gated_step(inputs, forget, state, **recurrence)
-    return group_norm_act(h, groups, weight, bias, gate=gate, activation=activation, eps=eps)
+    return _apply_norm(h, groups, weight, bias, gate, activation, eps)

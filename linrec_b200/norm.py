@@ -147,17 +147,7 @@ class _GroupNormFn(torch.autograd.Function):
         return dx, dgate, dw, db, None, None, None
 
 
-def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
-                   gate: torch.Tensor | None = None, activation: str | None = "silu", eps: float = 1e-5) -> torch.Tensor:
-    """Group norm of `x`, (samples, ..., channels): mean and (biased) variance over the dimensions between and
-    the channels of a group, `groups` groups of adjacent channels; then weight and bias per channel; then
-    the activation of the result, or the product with the activated gate where one is given.
-
-    For statistics of every position by itself give x as (positions, channels).
-    activation   "silu", "sigmoid" or None
-    weight, bias (channels,), ones and zeros by default; gate has the sizes and dtype of x
-
-    Differentiable once with respect to x, gate, weight and bias."""
+def _check(x, groups, weight, bias, gate, activation, eps) -> None:
     if x.dim() < 2:
         _fail("x needs a sample and a channel dimension")
     if x.dtype not in _STORAGE:
@@ -174,8 +164,26 @@ def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = N
     if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
         _fail("gate must have the sizes and the dtype of x")
     _check_cuda(x, gate, weight, bias)
+
+
+def _apply(x, groups, weight, bias, gate, activation, eps) -> torch.Tensor:
     weight, bias = _as_float(weight), _as_float(bias)
     args = (x, gate, weight, bias, groups, _ACTIVATIONS[activation], float(eps))
     if _wants_grad(x, gate, weight, bias):
         return _GroupNormFn.apply(*args)
     return _forward(*args, False)[0]
+
+
+def group_norm_act(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
+                   gate: torch.Tensor | None = None, activation: str | None = "silu", eps: float = 1e-5) -> torch.Tensor:
+    """Group norm of `x`, (samples, ..., channels): mean and (biased) variance over the dimensions between and
+    the channels of a group, `groups` groups of adjacent channels; then weight and bias per channel; then
+    the activation of the result, or the product with the activated gate where one is given.
+
+    For statistics of every position by itself give x as (positions, channels).
+    activation   "silu", "sigmoid" or None
+    weight, bias (channels,), ones and zeros by default; gate has the sizes and dtype of x
+
+    Differentiable once with respect to x, gate, weight and bias."""
+    _check(x, groups, weight, bias, gate, activation, eps)
+    return _apply(x, groups, weight, bias, gate, activation, eps)

@@ -89,3 +89,22 @@ def test_c_entry_options_and_sizes():
     assert _capi.lib.linrec_b200_gated_checkpoint_rows(ctypes.byref(_args(nseq=3, seqlen=600, nrows=1800))) == 30
     assert _capi.lib.linrec_b200_gated_scratch_size(ctypes.byref(a)) == 0
     assert _capi.lib.linrec_b200_gated_step(None, None, None, 8, 8, 8, None, 8.0, None, None, 8, 4, None, 0, 4, 8, 0, None) == _capi.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("why,kw", [
+    ("groups must divide", {"groups": 3}),
+    ("activation", {"activation": "relu"}),
+    ("eps", {"eps": 0.0}),
+    ("weight must have", {"weight": torch.zeros(7)}),
+    ("bias must have", {"bias": torch.zeros(7)}),
+    ("gate must have the sizes", {"gate": P[:5]}),
+    ("gate must have the sizes", {"gate": P.bfloat16()}),
+])
+def test_a_refused_norm_step_leaves_the_state(why, kw, monkeypatch):
+    from linrec_b200 import gated
+    steps = []
+    monkeypatch.setattr(gated, "linrec_gated_step", lambda x, *a, **k: steps.append(1) or x)
+    args = {"gate": None, "groups": 2, **kw}
+    with pytest.raises(RuntimeError, match=why):
+        lb.linrec_gated_norm_step(P, P, args.pop("gate"), P.clone(), args.pop("groups"), **args)
+    assert not steps
