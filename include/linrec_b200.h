@@ -329,7 +329,8 @@ LINREC_API int linrec_b200_gated_bwd(const linrec_gated_args* args, const linrec
 /* One token of each sequence: row r of x, forget(, input_gate) advances row slots[r] of `state` (nslots rows
  * of nchan floats, state_stride apart, updated in place) and gives row r of y.  Without slots row r advances
  * state row r (nrows <= nslots).  A slot outside [0, nslots) marks a padding row: its y is zero and no state
- * changes.  Rows that name the same slot are consecutive tokens of one sequence, in row order. */
+ * changes.  Rows that name the same slot are consecutive tokens of one sequence, in row order.  Neither operands
+ * nor y may overlap the state. */
 LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const void* input_gate, int64_t x_stride,
                                       int64_t forget_stride, int64_t input_gate_stride, const float* decay,
                                       float decay_scale, void* y, float* state, int64_t state_stride, int64_t nslots,

@@ -226,11 +226,26 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
 
 
 # ---- one token ---------------------------------------------------------------------------------------
+def _span(t):
+    """First byte of `t` and the one behind its last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _check_apart(state, *operands) -> None:
+    """float32 operands must lie outside the state: blocks would read what others have already advanced."""
+    for t in operands:
+        if t is not None and t.dtype == torch.float32 and t.numel() and state.numel():
+            (first, behind), (lo, hi) = _span(t), _span(state)
+            if first < hi and lo < behind:
+                _fail("operands must not share memory with the state, which is updated in place")
+
+
 def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.Tensor, *,
                       input_gate: torch.Tensor | None = None, decay: torch.Tensor | None = None,
                       decay_scale: float = 8.0, slots: torch.Tensor | None = None) -> torch.Tensor:
     """One token of the recurrence for every row of `inputs` (rows, D); `state` (slots, D), float32, is
-    updated in place and y (rows, D) returned.
+    updated in place and y (rows, D) returned.  No operand may share memory with the state.
 
     slots   (rows,) int32 or int64: the state row each row advances.  A slot outside the cache (such as -1)
             marks a padding row: zeros in y, no state touched.  Rows of the same slot are consecutive tokens
@@ -255,6 +270,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         if slots.numel() != rows:
             _fail("slots must name one state row per row of the inputs")
     _check_cuda(inputs, forget, input_gate, decay, state, slots)
+    _check_apart(state, inputs, forget, input_gate, decay)
     if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")
     y = _empty_dense(inputs)

@@ -108,3 +108,14 @@ def test_a_refused_norm_step_leaves_the_state(why, kw, monkeypatch):
     with pytest.raises(RuntimeError, match=why):
         lb.linrec_gated_norm_step(P, P, args.pop("gate"), P.clone(), args.pop("groups"), **args)
     assert not steps
+
+
+def test_step_refuses_operands_in_the_memory_of_its_state():
+    # rows are advanced by different blocks: one would read what another has already advanced
+    from linrec_b200.gated import _check_apart
+    cache = torch.zeros(20, 8)
+    for state, operand in ((cache[5:15], cache[:10]), (cache[:10], cache[:10]), (cache[:10], cache[9]), (cache[:, :4], cache[:, 4:])):
+        with pytest.raises(RuntimeError, match="share memory with the state"):
+            _check_apart(state, P, None, operand)
+    _check_apart(cache[10:], cache[:10], P, None, P[0])
+    _check_apart(cache[:0], cache, cache[:10])

@@ -502,3 +502,23 @@ def test_step_replayed():
         graph.replay()
         _check(y, tuple(v[:, t] for v in want["y"]), "y")
     _check(state, want["final"], "state")
+
+
+@pytest.mark.parametrize("which", ["inputs", "forget"])
+def test_step_refuses_operands_in_the_memory_of_its_state(which):
+    cache, x = torch.randn(20, 8, device=DEV), torch.randn(10, 8, device=DEV)
+    before = cache.clone()
+    args = {"inputs": x, "forget": x, which: cache[:10]}
+    with pytest.raises(RuntimeError, match="share memory with the state"):
+        _lb().linrec_gated_step(args["inputs"], args["forget"], cache[5:15])
+    assert torch.equal(cache, before)
+    _lb().linrec_gated_step(args["inputs"], args["forget"], cache[10:])      # side by side in one buffer
+
+
+def test_a_refused_norm_step_leaves_the_state():
+    x, state = torch.randn(10, 8, device=DEV), torch.randn(10, 8, device=DEV)
+    before = state.clone()
+    for kw in ({"groups": 3}, {"groups": 2, "weight": torch.ones(8)}, {"groups": 2, "eps": 0.0}):
+        with pytest.raises(RuntimeError):
+            _lb().linrec_gated_norm_step(x, x, None, state, **kw)
+    assert torch.equal(state, before)
