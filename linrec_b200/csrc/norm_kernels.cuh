@@ -278,7 +278,10 @@ __global__ void __launch_bounds__(kNormThreads, NV == 1 ? 4 : 2) norm_rows_fwd_k
 }
 
 // One element per access, NV per lane (rows off 16-byte boundaries, or groups that are not whole sixteens of bytes).
-// (16384, 4098) bf16 with gate, 6 groups: 441 us forward, 460 backward, 0.9 and 1.5 TB/s.
+// With many pieces per lane the operands of eight are loaded before any is worked on: behind the stores and branches of
+// the piece before them they wait for memory one by one.  (16384, 4098) with gate, 6 groups, without and with:
+// forward bf16 439 and 326 us, fp32 499 and 446; backward fp32 835 and 491, but bf16 447 and 472, and with few pieces
+// ((16384, 4004), 91 groups, bf16) 265 / 365 and 282 / 478, which therefore load piece by piece.
 template <typename ST, int NV, bool GATE, int ACT>
 __global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_fwd_kernel(const NormParams p)
 {
@@ -307,11 +310,30 @@ __global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_fwd_k
         const float inv = 1.0f / sqrtf(fmaf(lanes_sum(sq, lanes), count, p.eps));
         if (!row) continue;
         if (p.stats && s.lane == 0 && s.active) p.stats[n * p.G + s.g] = make_float2(mean, inv);
+        if constexpr (NV > 8) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (i < mine)
-                y[i * lanes] = from_f32<ST>(norm_value<kFast, GATE, ACT>(v[i], GATE ? load_one<ST>(gate, i * lanes) : 0.0f, mean, inv,
-                                                                         p.w ? __ldg(w + i * lanes) : 1.0f, p.b ? __ldg(b + i * lanes) : 0.0f));
+            for (int i0 = 0; i0 < NV; i0 += 8) {
+                float g[8], wi[8], bi[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = i0 + j;
+                    g[j] = GATE && i < mine ? load_one<ST>(gate, i * lanes) : 0.0f;
+                    wi[j] = p.w && i < mine ? __ldg(w + i * lanes) : 1.0f;
+                    bi[j] = p.b && i < mine ? __ldg(b + i * lanes) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const ST r = from_f32<ST>(norm_value<kFast, GATE, ACT>(v[i0 + j], g[j], mean, inv, wi[j], bi[j]));
+                    if (i0 + j < mine) y[(i0 + j) * lanes] = r;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i < mine)
+                    y[i * lanes] = from_f32<ST>(norm_value<kFast, GATE, ACT>(v[i], GATE ? load_one<ST>(gate, i * lanes) : 0.0f, mean, inv,
+                                                                             p.w ? __ldg(w + i * lanes) : 1.0f, p.b ? __ldg(b + i * lanes) : 0.0f));
+        }
     }
 }
 
@@ -456,24 +478,49 @@ __global__ void __launch_bounds__(kNormThreads, NV > 8 ? 3 : 4) norm_rows1_bwd_k
         ST* dx = static_cast<ST*>(p.dx) + n * p.C + ch0 + s.lane;
         ST* dgate = static_cast<ST*>(p.dgate) + n * p.C + ch0 + s.lane;
         float xhat[NV], k[NV], s1 = 0.0f, s2 = 0.0f;
+        auto take = [&](int i, float xv, float g, float d, float wi, float bi) {
+            float dz, dg;
+            norm_gradient<kFast, GATE, ACT>(xv, g, d, st, wi, bi, xhat[i], dz, dg);
+            if (p.part) {
+                float2 v = sums[i * lanes];
+                v.x = fmaf(dz, xhat[i], v.x);
+                v.y += dz;
+                sums[i * lanes] = v;
+            }
+            k[i] = dz * wi;
+            s1 += k[i];
+            s2 = fmaf(k[i], xhat[i], s2);
+            if (GATE) dgate[i * lanes] = from_f32<ST>(dg);
+        };
+        if constexpr (NV > 8 && sizeof(ST) == 4) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            xhat[i] = k[i] = 0.0f;
-            if (row && i < mine) {
-                const float wi = p.w ? __ldg(w + i * lanes) : 1.0f;
-                float dz, dg;
-                norm_gradient<kFast, GATE, ACT>(load_one<ST>(x, i * lanes), GATE ? load_one<ST>(gate, i * lanes) : 0.0f,
-                                                load_one<ST>(dy, i * lanes), st, wi, p.b ? __ldg(b + i * lanes) : 0.0f, xhat[i], dz, dg);
-                if (p.part) {
-                    float2 v = sums[i * lanes];
-                    v.x = fmaf(dz, xhat[i], v.x);
-                    v.y += dz;
-                    sums[i * lanes] = v;
+            for (int i0 = 0; i0 < NV; i0 += 8) {
+                float xv[8], g[8], d[8], wi[8], bi[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = i0 + j;
+                    const bool have = row && i < mine;
+                    xv[j] = have ? load_one<ST>(x, i * lanes) : 0.0f;
+                    g[j] = GATE && have ? load_one<ST>(gate, i * lanes) : 0.0f;
+                    d[j] = have ? load_one<ST>(dy, i * lanes) : 0.0f;
+                    wi[j] = p.w && have ? __ldg(w + i * lanes) : 1.0f;
+                    bi[j] = p.b && have ? __ldg(b + i * lanes) : 0.0f;
                 }
-                k[i] = dz * wi;
-                s1 += k[i];
-                s2 = fmaf(k[i], xhat[i], s2);
-                if (GATE) dgate[i * lanes] = from_f32<ST>(dg);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    xhat[i0 + j] = k[i0 + j] = 0.0f;
+                    if (row && i0 + j < mine) take(i0 + j, xv[j], g[j], d[j], wi[j], bi[j]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                xhat[i] = k[i] = 0.0f;
+                if (row && i < mine) {
+                    const float wi = p.w ? __ldg(w + i * lanes) : 1.0f;
+                    take(i, load_one<ST>(x, i * lanes), GATE ? load_one<ST>(gate, i * lanes) : 0.0f, load_one<ST>(dy, i * lanes), wi,
+                         p.b ? __ldg(b + i * lanes) : 0.0f);
+                }
             }
         }
         const float m1 = lanes_sum(s1, lanes) * count, m2 = lanes_sum(s2, lanes) * count;
