@@ -44,7 +44,8 @@ Plan plan_of(const linrec_group_norm_args& a, bool aligned, bool bwd)
         p.rows = true;
         const int* nv = linrec_variants::kNormPieces[p.V == 8];
         p.many = pieces > 32 * nv[0];
-        p.lanes = 1;
+        // (with many single elements per lane the kernels take a group to be a whole warp)
+        p.lanes = p.many && p.V == 1 ? 32 : 1;
         while (p.lanes < 32 && p.lanes * nv[p.many] < pieces) p.lanes *= 2;
         const int slots = linrec::kNormThreads / p.lanes;
         p.gb = (int)(a.groups < slots ? a.groups : slots);

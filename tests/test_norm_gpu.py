@@ -261,3 +261,25 @@ def test_prefill_then_decode():
                                       decay=dev["decay"], slots=slots)
         _check(y[:3], tuple(v[:, t] for v in want), f"token {t}")
     assert torch.isnan(cache[[1, 2, 4, 5, 7]]).all()
+
+
+@pytest.mark.parametrize("width", [264, 300, 384, 500, 512, 683, 1000, 1024])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_wide_groups(width, dtype):
+    """Groups of 257 to 1024 channels, one position per sample, whose lanes have many pieces each: operands on
+    16-byte boundaries, one element off them, and parameters off them; more rows than the CTAs take in one turn."""
+    for rows, groups, off in ((1000, 3, None), (1000, 3, "x"), (41, 1, "weight"), (1, 2, "x")):
+        for gate, act in ((True, "silu"), (False, "sigmoid")):
+            C = groups * width
+            c = _case((rows, C), dtype, gate, affine=gate or off == "weight", seed=width)
+            # memory that the results will get: an element that nothing writes shows
+            del [torch.full((rows, C), float("nan"), dtype=dtype, device=DEV) for _ in range(8)][:]
+
+            def place(k, t):
+                if k == off or (off == "x" and k in ("gate", "dy")):
+                    wide = torch.full((*t.shape[:-1], C + 1), float("nan"), dtype=t.dtype, device=DEV)
+                    wide[..., 1:] = t.to(DEV)
+                    return wide[..., 1:].detach()
+                return t.to(DEV)
+
+            _compare(_run(c, groups, act, place), _oracle(c, groups, act))
