@@ -110,13 +110,17 @@ __device__ __forceinline__ void decay_factors2(F2 y, F2& a, F2& b2)
         b2 = f2(b0, b1);
     }
 }
+constexpr float kSmallestNormal = 1.17549435e-38f;
 __device__ __forceinline__ F2 root2(F2 v)
 {
     const float2 w = f2_get(v);
     return f2(approx_sqrt(w.x), approx_sqrt(w.y));
 }
 // b s(i).  Fast: with d = 1 + e^-i it is b^2 / sqrt(b^2 d^2), one special function for a root and a reciprocal
-// (they bound the forward pass); a gate that is shut, b = 0, gives exactly nothing.
+// (they bound the forward pass).  A gate that is shut gives exactly nothing: so does a b^2 below the smallest normal
+// number, which the root would take for zero (its reciprocal is infinite there, and d >= 1 keeps all larger ones out of
+// that range), as the root of the other passes does.  A NaN is neither and goes through.  An input gate below e^-44 counts
+// as shut as well: b^2 d^2 overflows.
 template <bool FAST>
 __device__ __forceinline__ F2 gated_factor2(F2 b2, F2 i)
 {
@@ -125,7 +129,7 @@ __device__ __forceinline__ F2 gated_factor2(F2 b2, F2 i)
         const F2 d = f2_add(f2(approx_exp2(t.x), approx_exp2(t.y)), f2(1.0f));
         const float2 q = f2_get(b2), r = f2_get(f2_mul(f2_mul(b2, d), d));
         const float2 g = f2_get(f2_mul(b2, f2(approx_rsqrt(r.x), approx_rsqrt(r.y))));
-        return f2(q.x > 0.0f ? g.x : 0.0f, q.y > 0.0f ? g.y : 0.0f);
+        return f2(q.x < kSmallestNormal ? 0.0f : g.x, q.y < kSmallestNormal ? 0.0f : g.y);
     }
     return f2_mul(root2(b2), logistic2<false>(i));
 }

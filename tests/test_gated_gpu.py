@@ -522,3 +522,50 @@ def test_a_refused_norm_step_leaves_the_state():
         with pytest.raises(RuntimeError):
             _lb().linrec_gated_norm_step(x, x, None, state, **kw)
     assert torch.equal(state, before)
+
+
+EXTREME = [-200.0, -110.0, -89.0, -88.0, -87.5, -87.0, -86.0, -85.0, -84.0, -83.0, -82.0, -80.0, -75.0, -60.0, -45.0, -20.0, 0.0, 3.0, 17.0, 90.0, 200.0]
+
+
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_extreme_logits_in_every_type(dtype, decay):
+    """Gates that are next to nothing without being nothing, beside gates of ordinary size, in scan, gradients and step."""
+    lb = _lb()
+    T, D = 150, 64
+    # rates of the decay form: from below 2^-149 to 96, and below 1/4 in all channels (a series of its own)
+    for lo, hi, wide in ((-110.0, 12.0, 1.0), (-110.0, -4.0, 1.0), (-20.0, -5.0, 30.0)):
+        c = _case((1, T, D), decay, dtype)
+        c["forget"] = torch.tensor(EXTREME)[torch.randint(0, len(EXTREME), (1, T, D), generator=torch.Generator().manual_seed(3))].to(dtype)
+        c["inputs"][:, ::7] = 0.0
+        if decay:
+            c["decay"] = torch.linspace(lo, hi, D)
+            c["input_gate"] = wide * c["input_gate"]
+        got, want = _run(c), _oracle(c)
+        for n, t in got.items():
+            assert torch.isfinite(t).all(), n
+            # below 1.2e-38 values lose their bits; log a reaches the results through its root, 1.1e-19, times
+            # operands whose products stay below 1e4 here; an input gate below e^-44 counts as shut
+            _check(t, (want[n][0], want[n][1] + 2e-15), n)
+        state = c["initial_state"].to(DEV)
+        kw = {"input_gate": c["input_gate"][:, 0].to(DEV), "decay": c["decay"].to(DEV)} if decay else {}
+        y = lb.linrec_gated_step(c["inputs"][:, 0].to(DEV), c["forget"][:, 0].to(DEV), state, **kw)
+        _check(y, tuple(t[:, 0] + e for t, e in zip(want["y"], (0.0, 2e-15))), "step")
+        lb.check_status()
+        if not decay:
+            break
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_nan_logits_show(dtype):
+    """A NaN gate is not a shut gate: the state is NaN from there on, at the sequence's first row as well."""
+    for decay in (False, True):
+        for at in (0, 1, 40):
+            for name in ("forget", "input_gate") if decay else ("forget",):
+                c = _case((1, 70, 64), decay, dtype, states=False)
+                c[name][:, at, 3] = float("nan")
+                y = _lb().linrec_gated(*(c[k].to(DEV) for k in ("inputs", "forget")),
+                                       **({k: c[k].to(DEV) for k in ("input_gate", "decay")} if decay else {}))
+                bad = torch.zeros(70, 64, dtype=torch.bool, device=DEV)
+                bad[at:, 3] = True
+                assert torch.equal(y[0].isnan(), bad), (decay, at, name)
