@@ -21,8 +21,10 @@
 // tickets older and a wait is only ever for a ticket that a running CTA holds).  The runs are then walked
 // again from the true state.  Reads and writes every element once.
 //
-// The cut is carried as a multiplier of minus zero, which products of multipliers (all >= 0) keep, and it
-// selects rather than multiplies: 0 * NaN would let one sequence's infinities into its neighbour.
+// The cut is carried as a multiplier of minus zero, and it selects rather than multiplies: 0 * NaN would let one
+// sequence's infinities into its neighbour.  Within a run it is set from the positions of the cuts; from run to run
+// products of multipliers (all >= 0) keep it, but for NaN ones: the run they are in has a NaN sum beside them, so that
+// they reach no more than their own sequence.
 //
 // The backward pass recomputes h from fp32 checkpoints that the forward pass leaves every 64 positions
 // (never from the rounded outputs) and scans the adjoint against the direction of the forward pass:
@@ -151,6 +153,10 @@ struct GatedRun {
     uint32_t start, end, valid, cut;
     int seq;
 };
+
+// Is there a cut among a run's first j + 1 positions?  Their product is the cut then, whatever multipliers follow it: minus
+// zero times NaN would be NaN, and would let the multipliers of a sequence into the adjoint of the one before it.
+__device__ __forceinline__ bool gated_is_cut(const GatedRun& r, int j) { return r.cut & ((2u << j) - 1u); }
 
 __device__ __forceinline__ long long gated_offset(const GatedParams& p, int i)
 {
@@ -842,7 +848,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, false, SHAPE>::threads(LO
                 if (p.h0 && (run.start >> j & 1u)) u[j] = f2_fma(a[j], load_state(p.h0, (long long)__shfl_sync(0xffffffffu, run.seq, j) * p.D + ch, have), u[j]);
                 const bool cut = run.cut >> j & 1u;
                 Y = cut ? u[j] : f2_fma(a[j], Y, u[j]);
-                P = cut ? f2(kCut) : f2_mul(P, a[j]);
+                P = gated_is_cut(run, j) ? f2(kCut) : f2_mul(P, a[j]);
             }
         } else {
 #pragma unroll
@@ -1012,7 +1018,7 @@ __global__ void __launch_bounds__(GatedTile<ST, DECAY, true, SHAPE>::threads(LOA
                 if (!(run.valid >> j & 1u)) a[j] = bb[j] = add[j] = f2(0.0f);
                 if (cut) Y = p.h0 && (run.start >> j & 1u) ? of_sequence(p.h0, j) : f2(0.0f);
                 Y = f2_fma(a[j], Y, add[j]);
-                P = cut ? f2(kCut) : f2_mul(P, a[j]);
+                P = gated_is_cut(run, j) ? f2(kCut) : f2_mul(P, a[j]);
             }
 #pragma unroll
             for (int j = K - 1; j >= 0; --j, at -= wstep) q = (run.cut >> j & 1u) ? f2(0.0f) : f2_mul(a[j], f2_add(gradient(at, j, true), q));

@@ -569,3 +569,35 @@ def test_nan_logits_show(dtype):
                 bad = torch.zeros(70, 64, dtype=torch.bool, device=DEV)
                 bad[at:, 3] = True
                 assert torch.equal(y[0].isnan(), bad), (decay, at, name)
+
+
+@pytest.mark.parametrize("D", [66, 72, 1280], ids=lambda d: f"D{d}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_a_sequence_keeps_its_nan_logits(dtype, D):
+    """NaN in the logits of a sequence's first or last scanned positions leaves all other sequences' values and gradients
+    alone, bit for bit, packed and in a batch of short sequences on one axis."""
+    offsets = [0, 100, 164, 230, 500]
+    for decay in (False, True):
+        for reverse in (False, True):
+            for packed in (True, False):
+                kw = {"cu_seqlens": torch.tensor(offsets, dtype=torch.int32, device=DEV)} if packed else {}
+                lo, hi = (164, 230) if packed else (2 * 77, 3 * 77)
+                c = _case((500, D) if packed else (5, 77, D), decay, dtype, nseq=4 if packed else None)
+                clean = _run(c, reverse=reverse, **kw)
+                for at in ([0], [1], [5, 6], [-1], [-2], [20]):
+                    d = {k: v.clone() for k, v in c.items()}
+                    for n in ("forget", "input_gate") if decay else ("forget",):
+                        d[n].view(-1, D)[torch.tensor(at) + (lo if at[0] >= 0 else hi)] = float("nan")
+                    dirty = _run(d, reverse=reverse, **kw)
+                    for n in clean:
+                        if n == "ddecay":
+                            continue
+                        whole, part = clean[n].flatten(0, -2), dirty[n].flatten(0, -2)
+                        keep = torch.ones(len(whole), dtype=torch.bool, device=DEV)
+                        if len(whole) < 10:
+                            keep[2] = False
+                        else:
+                            keep[lo:hi] = False
+                        assert torch.equal(whole[keep], part[keep]), (n, at, reverse, packed)
+                        if n in ("dx", "dforget"):
+                            assert part[~keep].isnan().any(), (n, at)
