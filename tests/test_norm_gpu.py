@@ -283,3 +283,32 @@ def test_wide_groups(width, dtype):
                 return t.to(DEV)
 
             _compare(_run(c, groups, act, place), _oracle(c, groups, act))
+
+
+def test_an_outlier_in_front():
+    """Whole sequences whose first position is far from all others: the statistics hold although every thread
+    that meets the outlier counts its distances from it first."""
+    lb = _lb()
+    g = torch.Generator(device=DEV).manual_seed(3)
+    # 223 samples fill the device with one slice each: 8 channels of 600 positions per thread (16-byte accesses), or
+    # one channel of 600 (rows off 16-byte boundaries)
+    for C, groups, skip in ((2048, 32, 0), (256, 4, 1)):
+        for far in (30.0, 1000.0, 1e4):
+            base = torch.randn(223, 600, C + skip, generator=g, device=DEV)
+            x = base[..., skip:]
+            x[:, 0, ::C // groups] = far
+            y = lb.group_norm_act(x, groups, activation=None, eps=1e-5)
+            # a few samples in 64 bits
+            for n in (0, 100, 222):
+                v = x[n].double().reshape(600, groups, -1)
+                d = v - v.mean((0, 2), keepdim=True)
+                want = (d / torch.sqrt((d * d).mean((0, 2), keepdim=True) + 1e-5)).reshape(600, C)
+                # A thread adds 8 * 600 / 2 squares one after the other at most, and fewer than 32 partial sums follow.
+                # Counted about elements of the data the squares come to twice those about the mean (once, where an
+                # outlier made the thread count about its mean), so the variance is off by 2 (2400 + 32) 2^-24 of
+                # itself and its root by half of that; the mean by as many steps of the distance from those elements,
+                # which is on average below the sum of both ends' distances from zero.
+                steps = (2400 + 32) * 2.0 ** -24
+                tol = steps * (want.abs() + 2 * v.abs().mean() / v.std()) + 1e-6
+                assert (y[n].double() - want).abs().le(tol).all(), (C, far, n, ((y[n].double() - want).abs() / tol).max())
+            del base, x, y
