@@ -17,6 +17,9 @@ from one, and it takes no states and no packed sequences, which is what these op
 reference's operators take finished coefficients too (linrec/impl/cuda/ops.py:17-101).
 
 Storage types float32, bfloat16 and float16; gates, products and states are float32.
+
+Derivatives are backward ones.  Forward-mode derivatives, torch.func transforms, recording by torch.jit.trace or make_fx
+and fake tensors are refused; torch.compile runs the calls between its graphs.
 """
 from __future__ import annotations
 
@@ -27,7 +30,7 @@ import math
 import torch
 
 from . import _capi
-from .norm import _as_float, _as_rows, _backward_once, _check_cuda, _empty_dense, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
+from .norm import _as_float, _as_rows, _backward_once, _check_tensors, _empty_dense, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
 from .norm import _apply as _apply_norm, _check as _check_norm
 from .ops import _DTYPES, _workspace
 
@@ -213,7 +216,7 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
             _fail("initial_state must have one row of channels per sequence")
         if not initial_state.is_floating_point():
             _fail("initial_state must be a floating-point tensor")
-    _check_cuda(inputs, forget, input_gate, decay, initial_state, cu_seqlens)
+    _check_tensors(inputs, forget, input_gate, decay, initial_state, cu_seqlens)
     # casts outside the operator: autograd casts the gradients back
     decay, initial_state = _as_float(decay), _as_float(initial_state)
     cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
@@ -269,7 +272,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         _check_index("slots", slots)
         if slots.numel() != rows:
             _fail("slots must name one state row per row of the inputs")
-    _check_cuda(inputs, forget, input_gate, decay, state, slots)
+    _check_tensors(inputs, forget, input_gate, decay, state, slots)
     _check_apart(state, inputs, forget, input_gate, decay)
     if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")

@@ -6,6 +6,9 @@ heads are the groups, and the usual group norm of (samples, positions, channels)
     y = group_norm_act(x, groups, weight, bias, gate=g)        # (norm(x) * weight + bias) * act(g)
 
 Storage types float32, bfloat16 and float16; statistics, parameters and their gradients are float32.
+
+Derivatives are backward ones.  Forward-mode derivatives, torch.func transforms, recording by torch.jit.trace or make_fx
+and fake tensors are refused; torch.compile runs the calls between its graphs.
 """
 from __future__ import annotations
 
@@ -13,6 +16,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -24,13 +28,42 @@ _STORAGE = (torch.float32, torch.bfloat16, torch.float16)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
+# (looked up once: they are asked for at every call, and a small call is host work)
+_Tensor = torch.Tensor
+_functorch_stack = torch._C._functorch.peek_interpreter_stack
+_functorch_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+_jit_state = torch._C._get_tracing_state
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_dispatch_mode = torch._C._get_dispatch_mode
+_no_dispatch = torch._C._disabled_torch_dispatch_impl
+_RECORDERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE)
 
 
 def _fail(what: str):
     raise RuntimeError(f"linrec: {what}")
 
 
-def _check_cuda(first, *others) -> None:
+def _refuse_transforms(ts) -> None:
+    for t in ts:
+        if t is None:
+            continue
+        if _functorch_wrapped(t):
+            _fail("torch.func transforms are not supported")
+        if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+            _fail("forward-mode derivatives are not supported")
+    if _jit_state() is not None or any(_dispatch_mode(k) is not None for k in _RECORDERS):
+        _fail("calls cannot be recorded by a tracer (torch.compile runs them between its graphs)")
+
+
+def _check_tensors(first, *others) -> None:
+    """Tensors that the C library can take: real ones, all on one GPU.  It computes out of sight of PyTorch's
+    transforms and tracers, and what those would make of the calls around it is a wrong answer."""
+    ts = (first, *others)
+    if _forward_ad._current_level >= 0 or _functorch_stack() is not None or _jit_state() is not None or _dispatch_modes():
+        _refuse_transforms(ts)
+    for t in ts:
+        if type(t) is not _Tensor and t is not None and type(t).__torch_dispatch__ is not _no_dispatch:
+            _fail(f"{type(t).__name__} is not a tensor with memory of its own")
     if not first.is_cuda:
         _fail("tensors must be CUDA tensors (there is no CPU implementation)")
     device = first.device
@@ -163,7 +196,7 @@ def _check(x, groups, weight, bias, gate, activation, eps) -> None:
             _fail(f"{name} must have one floating-point value per channel")
     if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
         _fail("gate must have the sizes and the dtype of x")
-    _check_cuda(x, gate, weight, bias)
+    _check_tensors(x, gate, weight, bias)
 
 
 def _apply(x, groups, weight, bias, gate, activation, eps) -> torch.Tensor:

@@ -119,3 +119,50 @@ def test_step_refuses_operands_in_the_memory_of_its_state():
             _check_apart(state, P, None, operand)
     _check_apart(cache[10:], cache[:10], P, None, P[0])
     _check_apart(cache[:0], cache, cache[:10])
+
+
+def _entry_points():
+    d = torch.zeros(8)
+    return {
+        "scan": lambda x: lb.linrec_gated(x, P),
+        "scan, decay": lambda x: lb.linrec_gated(P, x, input_gate=P, decay=d),
+        "scan, state": lambda x: lb.linrec_gated(X, X, initial_state=x[:2]),
+        "step": lambda x: lb.linrec_gated_step(P, x, P),
+        "step, state": lambda x: lb.linrec_gated_step(P, P, x),
+        "norm": lambda x: lb.group_norm_act(x, 2),
+        "norm, gate": lambda x: lb.group_norm_act(P, 2, gate=x),
+        "norm, weight": lambda x: lb.group_norm_act(P, 2, x[0]),
+        "layer": lambda x: lb.linrec_gated_norm(x, x, x, 2),
+        "layer step": lambda x: lb.linrec_gated_norm_step(P, P, x, P, 2),
+    }
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("name", _entry_points())
+def test_what_pytorch_cannot_see_through_is_refused(name):
+    """The calls allocate a result and fill it out of PyTorch's sight: a tangent would be dropped and a recording
+    would hold an empty tensor."""
+    call = _entry_points()[name]
+    import torch.autograd.forward_ad as forward_ad
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode derivatives"):
+            call(forward_ad.make_dual(P, torch.ones_like(P)))
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            call(P)                       # no tangent, nothing to refuse
+    for transform in (lambda: torch.func.vmap(call)(P[None]), lambda: torch.func.jvp(call, (P,), (P,)),
+                      lambda: torch.func.grad(lambda x: call(x).sum())(P)):
+        with pytest.raises(RuntimeError, match="torch.func transforms"):
+            transform()
+    with pytest.raises(RuntimeError, match="recorded by a tracer"):
+        torch.jit.trace(call, (P,), check_trace=False)
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(RuntimeError, match="recorded by a tracer"):
+            make_fx(call, tracing_mode=mode)(P)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        fake = torch.empty(10, 8, device="cuda")
+        with pytest.raises(RuntimeError, match="recorded by a tracer"):
+            call(fake)
+    with pytest.raises(RuntimeError, match="FakeTensor is not a tensor with memory|CUDA tensors"):
+        call(mode.from_tensor(P))

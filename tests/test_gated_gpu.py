@@ -601,3 +601,36 @@ def test_a_sequence_keeps_its_nan_logits(dtype, D):
                         assert torch.equal(whole[keep], part[keep]), (n, at, reverse, packed)
                         if n in ("dx", "dforget"):
                             assert part[~keep].isnan().any(), (n, at)
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_under_modes_that_only_look_on_and_compiled():
+    """Counting and profiling modes, and torch.compile, which runs the calls between its graphs."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Onlooker(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    lb = _lb()
+    c = _case((2, 70, 64), True, torch.float32, states=False)
+    x, f, i, d = (c[k].to(DEV) for k in ("inputs", "forget", "input_gate", "decay"))
+
+    def layer(x):
+        y = lb.linrec_gated_norm(2.0 * x, f, i, 4, input_gate=i, decay=d)
+        state = torch.zeros(2, 64, device=DEV)
+        with torch.no_grad():
+            z = lb.linrec_gated_norm_step(x[:, 0], f[:, 0], i[:, 0], state, 4, input_gate=i[:, 0], decay=d)
+        return y + 1.0, z, state
+
+    def run(fn):
+        leaf = x.clone().requires_grad_(True)
+        out = fn(leaf)
+        return (*out, *torch.autograd.grad(out[0], leaf, c["dy"].to(DEV)))
+
+    want = run(layer)
+    with Onlooker():
+        got = run(layer)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    got = run(torch.compile(layer, backend="eager"))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
