@@ -231,16 +231,28 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
 # ---- one token ---------------------------------------------------------------------------------------
 def _span(t):
     """First byte of `t` and the one behind its last."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    first, last = t.data_ptr(), 0
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return first, first + (last + 1) * t.element_size()
+
+
+def _beside(state, t) -> bool:
+    """Are `t` and the state different columns of the rows of one buffer?"""
+    if t is None or t.dim() != 2 or t.stride(0) <= t.size(1) or t.stride(1) != 1:
+        return False
+    step, size = t.stride(0) * t.element_size(), t.element_size()
+    at = (t.data_ptr() - state.data_ptr()) % step
+    return step == state.stride(0) * 4 and at >= state.size(1) * 4 and at + t.size(1) * size <= step
 
 
 def _check_apart(state, *operands) -> None:
-    """float32 operands must lie outside the state: blocks would read what others have already advanced."""
-    for t in operands:
-        if t is not None and t.dtype == torch.float32 and t.numel() and state.numel():
-            (first, behind), (lo, hi) = _span(t), _span(state)
-            if first < hi and lo < behind:
+    """Operands of any type must lie outside the state, its first element to its last: blocks would read what others
+    have already advanced."""
+    if state.numel():
+        lo, hi = _span(state)
+        for t in operands:
+            if t is not None and t.numel() and t.data_ptr() < hi and _span(t)[1] > lo:
                 _fail("operands must not share memory with the state, which is updated in place")
 
 
@@ -248,7 +260,8 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
                       input_gate: torch.Tensor | None = None, decay: torch.Tensor | None = None,
                       decay_scale: float = 8.0, slots: torch.Tensor | None = None) -> torch.Tensor:
     """One token of the recurrence for every row of `inputs` (rows, D); `state` (slots, D), float32, is
-    updated in place and y (rows, D) returned.  No operand may share memory with the state.
+    updated in place and y (rows, D) returned.  No operand may lie in the memory from the state's first element to
+    its last, but for other columns of the same rows.
 
     slots   (rows,) int32 or int64: the state row each row advances.  A slot outside the cache (such as -1)
             marks a padding row: zeros in y, no state touched.  Rows of the same slot are consecutive tokens
@@ -273,7 +286,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         if slots.numel() != rows:
             _fail("slots must name one state row per row of the inputs")
     _check_tensors(inputs, forget, input_gate, decay, state, slots)
-    _check_apart(state, inputs, forget, input_gate, decay)
+    _check_apart(state, *[t for t in (inputs, forget, input_gate, decay, slots) if not _beside(state, t)])
     if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")
     y = _empty_dense(inputs)

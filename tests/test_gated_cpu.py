@@ -166,3 +166,35 @@ def test_what_pytorch_cannot_see_through_is_refused(name):
             call(fake)
     with pytest.raises(RuntimeError, match="FakeTensor is not a tensor with memory|CUDA tensors"):
         call(mode.from_tensor(P))
+
+
+def test_columns_beside_the_state_are_told_from_shared_memory():
+    """Both answers against the sets of bytes."""
+    from linrec_b200.gated import _beside, _check_apart
+
+    def bytes_of(t):
+        at = torch.zeros(1, dtype=torch.int64)
+        for n, s in zip(t.shape, t.stride()):
+            at = (at[:, None] + torch.arange(n) * s).flatten()
+        first = t.data_ptr() + at * t.element_size()
+        return set((first[:, None] + torch.arange(t.element_size())).flatten().tolist())
+
+    buf = torch.zeros(12, 24)
+    states = [buf[2:8, 4:12], buf[:, :8], buf[3:4, :8], buf.view(6, 48)[:, 4:12]]
+    half, index = buf.view(torch.bfloat16), buf.view(torch.int32)
+    operands = [buf[:, 12:20], buf[2:8, :4], buf[2:8, 12:], buf[:4, 8:16], buf[2:8, 11:14], buf[:2, 4:12], buf[8:, 4:12], buf[5], buf[1], buf[:, ::3],
+                buf.view(6, 48)[:, 12:20], buf.view(6, 48)[:, 40:], half[:, 24:32], half[2:8, :8], half[:, 23:25], half[8:, 8:16], half[1],
+                half[3, 8:16], index[:, 5], index[0, :9], buf.t()[12:, :], torch.zeros(12, 8), torch.zeros(12, 24)[:, :8]]
+    beside = 0
+    for state in states:
+        for t in operands:
+            shared = bytes_of(state) & bytes_of(t)
+            if _beside(state, t):
+                assert not shared
+                beside += 1
+                continue
+            if shared:
+                with pytest.raises(RuntimeError, match="share memory with the state"):
+                    _check_apart(state, t)
+    _check_apart(states[0], torch.zeros(12, 8), buf[8:], half[8:, :8], index[0, :9], None)
+    assert beside > 0

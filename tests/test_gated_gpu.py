@@ -634,3 +634,25 @@ def test_under_modes_that_only_look_on_and_compiled():
     assert all(torch.equal(a, b) for a, b in zip(want, got))
     got = run(torch.compile(layer, backend="eager"))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_step_on_columns_of_one_buffer():
+    """State and float32 operands as column blocks of the same rows; 16-bit and index views of the state's memory are
+    refused."""
+    lb = _lb()
+    D = 24
+    g = torch.Generator().manual_seed(2)
+    buf = torch.randn(10, 3 * D, generator=g).to(DEV)
+    state, x, f = buf[:, :D], buf[:, D:2 * D], buf[:, 2 * D:]
+    alone = state.clone()
+    want = lb.linrec_gated_step(x.clone(), f.clone(), alone)
+    keep = buf[:, D:].clone()
+    assert torch.equal(lb.linrec_gated_step(x, f, state), want)
+    assert torch.equal(state, alone) and torch.equal(buf[:, D:], keep)
+    state = torch.zeros(10, D, device=DEV)
+    h = torch.zeros(10, D, dtype=torch.bfloat16, device=DEV)
+    for args, kw in (((state.view(torch.bfloat16)[:, :D], h), {}), ((h, state.view(torch.float16)[:, D:].view(torch.bfloat16)), {}),
+                     ((h, h), {"slots": state.view(torch.int32)[0, :10]})):
+        with pytest.raises(RuntimeError, match="share memory with the state"):
+            lb.linrec_gated_step(*args, state, **kw)
+    assert (state == 0).all()
