@@ -342,7 +342,7 @@ LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const v
  * nchan / groups consecutive channels over all positions of a sample; mean and variance (biased) are fp32:
  *   z = (x - mean) / sqrt(var + eps) * weight + bias;   y = act(z), or z * act(gate) where gate is given
  * activation: 0 none, 1 v s(v), 2 s(v), with s the logistic function.  Results must not overlap operands.  weight and bias: nchan floats, or NULL
- * for ones and zeros.  stats: nsamples * groups pairs (mean, 1/sqrt(var + eps)), written by the forward pass
+ * for ones and zeros.  stats: nsamples * groups pairs (mean, 1/sqrt(var + eps)), 8-byte aligned, written by the forward pass
  * if given, required by the backward pass.  Results have rows at stride nchan.  dweight and dbias may be
  * NULL.  Either pass may need scratch (linrec_b200_group_norm_scratch_size for the same arguments; need not be
  * cleared, 16-byte aligned; a call's own until its kernels have run).  What follows the recurrence in a layer with

@@ -143,6 +143,10 @@ int launch_gated(bool bwd, const linrec_gated_args* args, const linrec_opts* opt
     if (bwd && (!a.dy || a.dy_stride < a.nchan || !a.dx || !a.dforget || !a.checkpoints)) return LINREC_ERR_INVALID_ARG;
     if (bwd && decay && (!a.dinput_gate || !a.ddecay || !a.scratch || a.scratch_bytes < linrec_b200_gated_scratch_size(args)))
         return LINREC_ERR_INVALID_ARG;
+    if (!linrec_host::on_elements({a.x, a.forget, a.input_gate, a.y, a.dy, a.dx, a.dforget, a.dinput_gate}, a.dtype == LINREC_DTYPE_F32 ? 4 : 2) ||
+        !linrec_host::on_elements({a.decay, a.initial_state, a.checkpoints, a.final_state, a.d_final_state, a.ddecay, a.d_initial_state, a.scratch}, 4) ||
+        !linrec_host::on_elements({a.cu_seqlens}, a.cu_is_64 ? 8 : 4))
+        return LINREC_ERR_INVALID_ARG;
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < linrec_b200_gated_workspace_size(args))
         return LINREC_ERR_WORKSPACE;
     DeviceInfo dev;
@@ -297,6 +301,9 @@ int linrec_b200_gated_step(const void* x, const void* forget, const void* input_
         if (nrows == 0 || nchan == 0) return LINREC_OK;
         if (!x || !forget || !y || (!state && nslots > 0) || x_stride < nchan || forget_stride < nchan || state_stride < nchan ||
             (decay && input_gate_stride < nchan) || (!slots && nrows > nslots))
+            return LINREC_ERR_INVALID_ARG;
+        if (!linrec_host::on_elements({x, forget, input_gate, y}, dtype == LINREC_DTYPE_F32 ? 4 : 2) || !linrec_host::on_elements({decay, state}, 4) ||
+            !linrec_host::on_elements({slots}, slots_are_64 ? 8 : 4))
             return LINREC_ERR_INVALID_ARG;
         DeviceInfo dev;
         const int rc = linrec_host::device_facts(dev);

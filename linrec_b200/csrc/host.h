@@ -4,6 +4,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
+#include <stdint.h>
+
+#include <initializer_list>
 
 #include "../../include/linrec_b200.h"
 
@@ -41,6 +44,14 @@ int guarded(Body body) noexcept
         note_cuda_error("host", "out of memory or another C++ exception");
         return LINREC_ERR_CUDA;
     }
+}
+
+// Do all of the pointers (null ones included) lie on boundaries of `size` bytes?  Kernels that meet another address fault.
+inline bool on_elements(std::initializer_list<const void*> pointers, int size)
+{
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % (unsigned)size != 0) return false;
+    return true;
 }
 
 inline int ceil_div_i(long long a, long long b) { return (int)((a + b - 1) / b); }

@@ -128,6 +128,9 @@ int launch_norm(bool bwd, const linrec_group_norm_args* args, void* stream_)
     if (!a.x || a.x_stride < a.nchan || (a.gate && a.gate_stride < a.nchan)) return LINREC_ERR_INVALID_ARG;
     if (!bwd && !a.y) return LINREC_ERR_INVALID_ARG;
     if (bwd && (!a.dy || a.dy_stride < a.nchan || !a.dx || !a.stats || (a.gate && !a.dgate))) return LINREC_ERR_INVALID_ARG;
+    if (!linrec_host::on_elements({a.x, a.gate, a.y, a.dy, a.dx, a.dgate}, a.dtype == LINREC_DTYPE_F32 ? 4 : 2) ||
+        !linrec_host::on_elements({a.weight, a.bias, a.dweight, a.dbias}, 4) || !linrec_host::on_elements({a.stats}, 8))
+        return LINREC_ERR_INVALID_ARG;
     const size_t need = linrec_b200_group_norm_scratch_size(args, bwd);
     if (need && (!a.scratch || a.scratch_bytes < need || reinterpret_cast<uintptr_t>(a.scratch) % 16 != 0)) return LINREC_ERR_WORKSPACE;
     linrec_host::DeviceInfo dev;

@@ -198,3 +198,30 @@ def test_columns_beside_the_state_are_told_from_shared_memory():
                     _check_apart(state, t)
     _check_apart(states[0], torch.zeros(12, 8), buf[8:], half[8:, :8], index[0, :9], None)
     assert beside > 0
+
+
+@pytest.mark.parametrize("dtype,kw", [
+    (_capi.DTYPE_F32, {"x": 18}), (_capi.DTYPE_F32, {"forget": 18}), (_capi.DTYPE_F32, {"y": 18}), (_capi.DTYPE_BF16, {"x": 17}),
+    (_capi.DTYPE_F16, {"y": 17}), (_capi.DTYPE_BF16, {"initial_state": 18}), (_capi.DTYPE_BF16, {"final_state": 18}), (_capi.DTYPE_BF16, {"checkpoints": 18}),
+    (_capi.DTYPE_BF16, {"cu_seqlens": 18}), (_capi.DTYPE_BF16, {"cu_seqlens": 20, "cu_is_64": 1}),
+    (_capi.DTYPE_BF16, {"decay": 18, "input_gate": 16, "input_gate_stride": 8}), (_capi.DTYPE_F32, {"decay": 16, "input_gate": 18, "input_gate_stride": 8}),
+])
+def test_c_entry_refuses_pointers_between_elements(dtype, kw):
+    # a workspace that is never reached: refused before it is looked at
+    a = _args(dtype=dtype, **kw)
+    assert _capi.lib.linrec_b200_gated_fwd(ctypes.byref(a), None, 256, 1 << 40, None) == _capi.ERR_INVALID_ARG
+    back = {"dy": 16, "dy_stride": 8, "dx": 16, "dforget": 16, "checkpoints": 16}
+    for n in back:
+        if n != "dy_stride":
+            b = _args(dtype=dtype, **{**back, n: 17})
+            assert _capi.lib.linrec_b200_gated_bwd(ctypes.byref(b), None, 256, 1 << 40, None) == _capi.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("at", range(6))
+def test_c_step_refuses_pointers_between_elements(at):
+    p = [16] * 6      # x, forget, input_gate, decay, y, state
+    p[at] += 2
+    call = lambda slots, wide: _capi.lib.linrec_b200_gated_step(p[0], p[1], p[2], 8, 8, 8, p[3], 8.0, p[4], p[5], 8, 4, slots, wide, 4, 8, _capi.DTYPE_F32, None)
+    assert call(None, 0) == _capi.ERR_INVALID_ARG
+    p[at] -= 2
+    assert call(18, 0) == call(20, 1) == _capi.ERR_INVALID_ARG

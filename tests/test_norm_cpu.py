@@ -68,3 +68,15 @@ def test_c_backward_refuses():
     # parameter gradients need scratch
     assert _capi.lib.linrec_b200_group_norm_bwd(ctypes.byref(_args(**full, dweight=16)), None) == _capi.ERR_WORKSPACE
     assert _capi.lib.linrec_b200_group_norm_bwd(None, None) == _capi.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("name", ["x", "y", "gate", "weight", "bias", "stats", "dy", "dx", "dgate", "dweight", "dbias"])
+def test_c_entries_refuse_pointers_between_elements(name):
+    good = {"gate": 16, "gate_stride": 12, "dy": 16, "dy_stride": 12, "dx": 16, "dgate": 16, "stats": 16, "scratch": 16, "scratch_bytes": 1 << 40}
+    at = 20 if name == "stats" else 18      # (pairs of floats)
+    forward = _capi.lib.linrec_b200_group_norm_fwd(ctypes.byref(_args(**{**good, name: at})), None)
+    back = _capi.lib.linrec_b200_group_norm_bwd(ctypes.byref(_args(**{**good, "dweight": 16, "dbias": 16, name: at})), None)
+    assert forward == back == _capi.ERR_INVALID_ARG
+    if name in ("x", "y", "gate", "dy", "dx", "dgate"):
+        a = _args(**{**good, name: 17}, dtype=_capi.DTYPE_BF16)
+        assert _capi.lib.linrec_b200_group_norm_fwd(ctypes.byref(a), None) == _capi.ERR_INVALID_ARG
