@@ -656,3 +656,99 @@ def test_step_on_columns_of_one_buffer():
         with pytest.raises(RuntimeError, match="share memory with the state"):
             lb.linrec_gated_step(*args, state, **kw)
     assert (state == 0).all()
+
+
+# Sizes that reach every way a tile is linked to the one before it, on a device of 148 SMs, rows on 16-byte boundaries
+# (columns: blocks of 64 channels times batch entries; `test_scan_and_gradients` has look-back).
+#   12, 20, 19 and 50 columns   clusters of eight, seven, seven and two CTAs, with turns in which some have no tile
+#   80                          clusters of one: a CTA keeps a column to itself
+#   160                         eight warps, jobs of four tiles
+#   300                         that forward in 16 bits, backward four warps
+#   450                         four warps in both directions (16 bits), jobs of four tiles and a shorter one
+COLUMNS = {12: (1, 1100, 768), 20: (2, 1100, 640), 19: (1, 2300, 1216), 50: (5, 600, 640), 80: (8, 600, 640),
+           160: (1, 700, 10240), 300: (2, 520, 9600), 450: (1, 330, 28800)}
+
+
+def _added_up(want, positions):
+    """The decay gradient is a sum over positions, `positions` of them one after the other in 32 bits; its bound
+    holds 50 roundings of every term already."""
+    if "ddecay" in want:
+        value, bound = want["ddecay"]
+        want["ddecay"] = (value, bound * (1 + (positions + 8) / 50))
+    return want
+
+
+@pytest.mark.parametrize("columns,dtype", [(n, t) for n in COLUMNS for t in DTYPES if t != torch.float16 or n in (12, 450)],
+                         ids=lambda v: str(v).replace("torch.", ""))
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+def test_every_way_of_linking_tiles(columns, dtype, decay):
+    shape = COLUMNS[columns]
+    for reverse in (False, True):
+        c = _case(shape, decay, dtype, seed=columns, states=reverse == decay)
+        got = _run(c, reverse=reverse)
+        # a thread has every fourth run of the column's positions at least
+        _compare(got, _added_up(_oracle(c, reverse=reverse), shape[-2] / 4))
+        again = _run(c, reverse=reverse)
+        assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("columns,rows", [(12, 1100), (50, 700), (80, 450), (160, 700), (450, 330)], ids=lambda n: str(n))
+@pytest.mark.parametrize("decay", [False, True], ids=["forget", "decay"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_packed_in_every_way_of_linking_tiles(columns, rows, decay, dtype):
+    for reverse, kind in ((False, torch.int32), (True, torch.int64)):
+        # empty and one-row sequences, one that starts where a tile does, one over several tiles, rows of none
+        offsets = [5, 5, 64, 65, 65, 128, 200, rows - 30, rows - 17]
+        c = _case((rows, columns * 64), decay, dtype, nseq=len(offsets) - 1, seed=columns)
+        want = _added_up(_oracle(c, offsets=offsets, reverse=reverse), rows / 4)
+        outside = torch.ones(rows, dtype=torch.bool)
+        outside[offsets[0]:offsets[-1]] = False
+        for i, n in enumerate(k for k in ("inputs", "forget", "input_gate", "dy") if k in c):
+            c[n] = c[n].clone()
+            c[n][outside] = [float("nan"), float("inf"), -float("inf"), float("nan")][i]
+        cu = torch.tensor(offsets, dtype=kind, device=DEV)
+        got = _run(c, cu_seqlens=cu, reverse=reverse)
+        _compare(got, want)
+        for n in ("y", "dx", "dforget", "dinput"):
+            if n in got:
+                assert (got[n][outside.to(DEV)] == 0).all(), n
+        again = _run(c, cu_seqlens=cu, reverse=reverse)
+        assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("columns", [12, 80, 160, 450])
+def test_linked_tiles_on_side_streams_and_replayed(columns):
+    """Two graphs captured on one stream and replayed side by side on others while the call runs eagerly on a third."""
+    lb = _lb()
+    _, T, D = COLUMNS[columns]
+    cases = [_case((1, T, D), True, torch.bfloat16, seed=s) for s in (1, 2)]
+    want = [_run(c) for c in cases]
+    stream, graphs = torch.cuda.Stream(), []
+    for c in cases:
+        dev = {k: v.to(DEV) for k, v in c.items()}
+        leaves = [dev[k].requires_grad_(True) for k in NAMES]
+        torch.cuda.synchronize()
+
+        def step():
+            y, final = lb.linrec_gated(leaves[0], leaves[1], input_gate=leaves[2], decay=leaves[3], initial_state=leaves[4], return_state=True)
+            return [y, final, *torch.autograd.grad([y, final], leaves, [dev["dy"], dev["dfinal"]])]
+
+        with torch.cuda.stream(stream):
+            step()
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                outs = step()
+        graphs.append((graph, outs, dev, leaves))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        for (graph, *_), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = _run(cases[0])
+    torch.cuda.synchronize()
+    for w, (_, outs, *_) in zip(want, graphs):
+        assert all(torch.equal(w[n], t) for n, t in zip(("y", "final", *NAMES.values()), outs))
+    assert all(torch.equal(want[0][n], eager[n]) for n in eager)
+    lb.check_status()
