@@ -42,6 +42,7 @@ extern "C" {
 #define LINREC_ERR_TOO_LONG        (-6)  /* tile-only call and the row does not fit one tile    */
 #define LINREC_ERR_UNALIGNED       (-7)  /* bulk-copy path forced on pointers/strides it cannot take */
 #define LINREC_ERR_SCRATCH_LIMIT   (-8)  /* problem needs more scratch than the built-in buffer has  */
+#define LINREC_ERR_OVERLAP         (-9)  /* operands share memory with what a call updates in place */
 
 /* ---- element storage types (arithmetic is fp32, except for LINREC_DTYPE_F64) ----------------- */
 #define LINREC_DTYPE_F32   0
@@ -330,7 +331,8 @@ LINREC_API int linrec_b200_gated_bwd(const linrec_gated_args* args, const linrec
  * of nchan floats, state_stride apart, updated in place) and gives row r of y.  Without slots row r advances
  * state row r (nrows <= nslots).  A slot outside [0, nslots) marks a padding row: its y is zero and no state
  * changes.  Rows that name the same slot are consecutive tokens of one sequence, in row order.  Neither operands
- * nor y may overlap the state. */
+ * nor y may lie in the memory from the state's first element to its last (LINREC_ERR_OVERLAP), but for other columns of
+ * rows at the same distance. */
 LINREC_API int linrec_b200_gated_step(const void* x, const void* forget, const void* input_gate, int64_t x_stride,
                                       int64_t forget_stride, int64_t input_gate_stride, const float* decay,
                                       float decay_scale, void* y, float* state, int64_t state_stride, int64_t nslots,

@@ -23,6 +23,7 @@ ERR_TIMEOUT = -5
 ERR_TOO_LONG = -6
 ERR_UNALIGNED = -7
 ERR_SCRATCH_LIMIT = -8
+ERR_OVERLAP = -9
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_F64 = 0, 1, 2, 3
 KIND_REF, KIND_TILE, KIND_PIPE = 0, 1, 2

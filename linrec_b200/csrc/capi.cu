@@ -1532,6 +1532,7 @@ const char* linrec_b200_strerror(int code)
         case LINREC_ERR_TOO_LONG: return "row does not fit one tile";
         case LINREC_ERR_UNALIGNED: return "this copy path needs 16-byte aligned rows (bulk copies along the last axis: whole 128-byte lines)";
         case LINREC_ERR_SCRATCH_LIMIT: return "problem needs more scratch than the 1 MiB built into the library (use linrec_b200_fwd with a workspace)";
+        case LINREC_ERR_OVERLAP: return "operands or results overlap the state, which is updated in place";
         default: return "unknown status";
     }
 }

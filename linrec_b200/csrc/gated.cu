@@ -59,6 +59,22 @@ int parse(const linrec_opts* o, int& wait_ms)
     return LINREC_OK;
 }
 
+// Rows of `width` bytes, `step` apart.  Do two sets share memory, or does one lie among the other's rows in any other way than
+// in columns of its own?
+struct Rows {
+    const void* p;
+    int64_t n, step, width;
+};
+bool rows_meet(const Rows& a, const Rows& b)
+{
+    if (!a.p || !b.p || a.n == 0 || b.n == 0) return false;
+    const intptr_t a0 = reinterpret_cast<intptr_t>(a.p), b0 = reinterpret_cast<intptr_t>(b.p);
+    if (a0 + (a.n - 1) * a.step + a.width <= b0 || b0 + (b.n - 1) * b.step + b.width <= a0) return false;
+    if (a.step != b.step) return true;
+    const int64_t at = ((a0 - b0) % b.step + b.step) % b.step;      // of a's columns, from b's on
+    return at < b.width || at + a.width > b.step;
+}
+
 bool on_boundary(const void* p, int64_t stride, int size, int bytes)
 {
     return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * size % bytes == 0;
@@ -302,6 +318,13 @@ int linrec_b200_gated_step(const void* x, const void* forget, const void* input_
         if (!x || !forget || !y || (!state && nslots > 0) || x_stride < nchan || forget_stride < nchan || state_stride < nchan ||
             (decay && input_gate_stride < nchan) || (!slots && nrows > nslots))
             return LINREC_ERR_INVALID_ARG;
+        // blocks would read what others have already advanced
+        const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
+        const Rows of_state{state, nslots, state_stride * 4, nchan * 4};
+        for (const Rows& r : {Rows{x, nrows, x_stride * size, nchan * size}, Rows{forget, nrows, forget_stride * size, nchan * size},
+                              Rows{input_gate, nrows, input_gate_stride * size, nchan * size}, Rows{y, nrows, nchan * size, nchan * size},
+                              Rows{decay, 1, nchan * 4, nchan * 4}, Rows{slots, 1, nrows * (slots_are_64 ? 8 : 4), nrows * (slots_are_64 ? 8 : 4)}})
+            if (rows_meet(r, of_state)) return LINREC_ERR_OVERLAP;
         if (!linrec_host::on_elements({x, forget, input_gate, y}, dtype == LINREC_DTYPE_F32 ? 4 : 2) || !linrec_host::on_elements({decay, state}, 4) ||
             !linrec_host::on_elements({slots}, slots_are_64 ? 8 : 4))
             return LINREC_ERR_INVALID_ARG;
@@ -313,7 +336,6 @@ int linrec_b200_gated_step(const void* x, const void* forget, const void* input_
         p.y = y; p.decay = decay; p.scale = decay_scale; p.state = state; p.sstate = state_stride;
         p.slots = slots; p.slots64 = slots_are_64; p.rows = (int)nrows; p.nslots = (int)nslots; p.D = (int)nchan;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const int size = dtype == LINREC_DTYPE_F32 ? 4 : 2;
         const bool four = nchan % 4 == 0 && on_boundary(x, x_stride, size, 4 * size) && on_boundary(forget, forget_stride, size, 4 * size) &&
                           (!decay || on_boundary(input_gate, input_gate_stride, size, 4 * size)) && on_boundary(y, nchan, size, 4 * size) &&
                           on_boundary(state, state_stride, 4, 16);

@@ -42,19 +42,20 @@ __all__ = ["linrec_gated", "linrec_gated_step", "linrec_gated_norm", "linrec_gat
 # ---- arguments ---------------------------------------------------------------------------------------
 def _check_operands(inputs, forget, input_gate, decay, decay_scale) -> None:
     """What the scan and the step have in common."""
-    if inputs.dtype not in _STORAGE:
-        _fail(f"dtype {inputs.dtype} is not supported (float32, bfloat16, float16)")
+    shape, dtype = inputs.shape, inputs.dtype
+    if dtype not in _STORAGE:
+        _fail(f"dtype {dtype} is not supported (float32, bfloat16, float16)")
     for name, t in (("forget", forget), ("input_gate", input_gate)):
         if t is None:
             continue
-        if t.shape != inputs.shape:
+        if t.shape != shape:
             _fail(f"{name} must have the sizes of the inputs")
-        if t.dtype != inputs.dtype:
+        if t.dtype != dtype:
             _fail(f"{name} must have the dtype of the inputs")
     if (input_gate is None) != (decay is None):
         _fail("input_gate and decay come together (decay form) or not at all (forget form)")
     if decay is not None:
-        if decay.shape != inputs.shape[-1:]:
+        if decay.shape != shape[-1:]:
             _fail("decay must have one value per channel")
         if not decay.is_floating_point():
             _fail("decay must be a floating-point tensor")
@@ -92,7 +93,7 @@ class _Problem:
     def __init__(self, inputs, forget, input_gate, decay, initial, cu, scale, reverse):
         shape = inputs.shape
         self.D = D = shape[-1]
-        self.nrows = inputs.numel() // D if D else 0
+        self.nrows = math.prod(shape[:-1]) if D else 0
         self.seqlen = shape[-2]
         if cu is not None:
             self.nseq = cu.numel() - 1
@@ -200,19 +201,20 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
     return_state                 also return the state behind each sequence's last scanned row, float32
 
     Differentiable once with respect to inputs, forget, input_gate, decay and initial_state."""
-    if inputs.dim() < 2:
+    shape = inputs.shape
+    if len(shape) < 2:
         _fail("inputs need a sequence and a channel dimension")
     _check_operands(inputs, forget, input_gate, decay, decay_scale)
-    lead = inputs.shape[:-2]
+    lead = shape[:-2]
     if cu_seqlens is not None:
         _check_index("cu_seqlens", cu_seqlens)
-        if inputs.dim() != 2:
+        if len(shape) != 2:
             _fail("packed inputs have two dimensions (rows, channels)")
         if cu_seqlens.numel() < 1:
             _fail("cu_seqlens holds one offset more than there are sequences")
         lead = (cu_seqlens.numel() - 1,)
     if initial_state is not None:
-        if tuple(initial_state.shape) != (*lead, inputs.size(-1)):
+        if initial_state.shape != (*lead, shape[-1]):
             _fail("initial_state must have one row of channels per sequence")
         if not initial_state.is_floating_point():
             _fail("initial_state must be a floating-point tensor")
@@ -221,7 +223,7 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
     decay, initial_state = _as_float(decay), _as_float(initial_state)
     cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
     args = (inputs, forget, input_gate, decay, initial_state, cu_seqlens, float(decay_scale), bool(reverse), bool(return_state))
-    if _wants_grad(*args[:5]):
+    if _wants_grad(inputs, forget, input_gate, decay, initial_state):
         y, final = _GatedFn.apply(*args)
     else:
         y, final, _ = _forward(*args, False)
@@ -231,28 +233,16 @@ def linrec_gated(inputs: torch.Tensor, forget: torch.Tensor, *, input_gate: torc
 # ---- one token ---------------------------------------------------------------------------------------
 def _span(t):
     """First byte of `t` and the one behind its last."""
-    first, last = t.data_ptr(), 0
-    for n, s in zip(t.shape, t.stride()):
-        last += (n - 1) * s
-    return first, first + (last + 1) * t.element_size()
-
-
-def _beside(state, t) -> bool:
-    """Are `t` and the state different columns of the rows of one buffer?"""
-    if t is None or t.dim() != 2 or t.stride(0) <= t.size(1) or t.stride(1) != 1:
-        return False
-    step, size = t.stride(0) * t.element_size(), t.element_size()
-    at = (t.data_ptr() - state.data_ptr()) % step
-    return step == state.stride(0) * 4 and at >= state.size(1) * 4 and at + t.size(1) * size <= step
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
 def _check_apart(state, *operands) -> None:
-    """Operands of any type must lie outside the state, its first element to its last: blocks would read what others
-    have already advanced."""
-    if state.numel():
-        lo, hi = _span(state)
-        for t in operands:
-            if t is not None and t.numel() and t.data_ptr() < hi and _span(t)[1] > lo:
+    """Names the refusal of operands in the memory between the state's first and last element."""
+    for t in operands:
+        if t is not None and t.numel() and state.numel():
+            (first, behind), (lo, hi) = _span(t), _span(state)
+            if first < hi and lo < behind:
                 _fail("operands must not share memory with the state, which is updated in place")
 
 
@@ -276,7 +266,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         _fail("state must have two dimensions, one row of channels per slot")
     if state.dtype != torch.float32:
         _fail("state must be float32")
-    if state.numel() and ((D > 1 and state.stride(1) != 1) or (state.size(0) > 1 and state.stride(0) < D)):
+    if not state.is_contiguous() and state.numel() and ((D > 1 and state.stride(1) != 1) or (state.size(0) > 1 and state.stride(0) < D)):
         _fail("state rows must be dense and must not overlap: they are updated in place")
     if slots is None:
         if state.size(0) != rows:
@@ -286,7 +276,6 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
         if slots.numel() != rows:
             _fail("slots must name one state row per row of the inputs")
     _check_tensors(inputs, forget, input_gate, decay, state, slots)
-    _check_apart(state, *[t for t in (inputs, forget, input_gate, decay, slots) if not _beside(state, t)])
     if _wants_grad(inputs, forget, input_gate, decay, state):
         _fail("linrec_gated_step updates its state in place and has no backward pass; use linrec_gated")
     y = _empty_dense(inputs)
@@ -299,7 +288,14 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
     slots = None if slots is None else slots.contiguous()
     args = (x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), decay_scale, y.data_ptr(), state.data_ptr(), max(state.stride(0), D),
             state.size(0), _ptr(slots), slots is not None and slots.dtype == torch.int64, rows, D, _DTYPES[inputs.dtype])
-    _on(inputs.device, lambda stream: _capi.raise_for(_capi.lib.linrec_b200_gated_step(*args, stream), "linrec_b200_gated_step"))
+
+    def launch(stream):
+        rc = _capi.lib.linrec_b200_gated_step(*args, stream)
+        if rc == _capi.ERR_OVERLAP:
+            _check_apart(state, inputs, forget, input_gate, decay, slots)
+        _capi.raise_for(rc, "linrec_b200_gated_step")
+
+    _on(inputs.device, launch)
     torch.autograd.graph.increment_version(state)
     return y
 

@@ -32,7 +32,7 @@ _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 _Tensor = torch.Tensor
 _functorch_stack = torch._C._functorch.peek_interpreter_stack
 _functorch_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
-_jit_state = torch._C._get_tracing_state
+_jit_tracing = torch._C._is_tracing
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _dispatch_mode = torch._C._get_dispatch_mode
 _no_dispatch = torch._C._disabled_torch_dispatch_impl
@@ -51,26 +51,32 @@ def _refuse_transforms(ts) -> None:
             _fail("torch.func transforms are not supported")
         if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
             _fail("forward-mode derivatives are not supported")
-    if _jit_state() is not None or any(_dispatch_mode(k) is not None for k in _RECORDERS):
+    if _jit_tracing() or any(_dispatch_mode(k) is not None for k in _RECORDERS):
         _fail("calls cannot be recorded by a tracer (torch.compile runs them between its graphs)")
+
+
+def _check_memory(t) -> None:
+    if type(t).__torch_dispatch__ is not _no_dispatch:
+        _fail(f"{type(t).__name__} is not a tensor with memory of its own")
 
 
 def _check_tensors(first, *others) -> None:
     """Tensors that the C library can take: real ones, all on one GPU.  It computes out of sight of PyTorch's
     transforms and tracers, and what those would make of the calls around it is a wrong answer."""
-    ts = (first, *others)
-    if _forward_ad._current_level >= 0 or _functorch_stack() is not None or _jit_state() is not None or _dispatch_modes():
-        _refuse_transforms(ts)
-    for t in ts:
-        if type(t) is not _Tensor and t is not None and type(t).__torch_dispatch__ is not _no_dispatch:
-            _fail(f"{type(t).__name__} is not a tensor with memory of its own")
+    if _forward_ad._current_level >= 0 or _dispatch_modes() or _jit_tracing() or _functorch_stack() is not None:
+        _refuse_transforms((first, *others))
+    if type(first) is not _Tensor:
+        _check_memory(first)
     if not first.is_cuda:
         _fail("tensors must be CUDA tensors (there is no CPU implementation)")
     device = first.device
     for t in others:
-        if t is not None and t.device != device:
-            _fail("tensors must be CUDA tensors (there is no CPU implementation)" if not t.is_cuda else
-                  "tensors must be on the same device")
+        if t is not None:
+            if type(t) is not _Tensor:
+                _check_memory(t)
+            if t.device != device:
+                _fail("tensors must be CUDA tensors (there is no CPU implementation)" if not t.is_cuda else
+                      "tensors must be on the same device")
 
 
 def _as_rows(t: torch.Tensor):
@@ -181,20 +187,22 @@ class _GroupNormFn(torch.autograd.Function):
 
 
 def _check(x, groups, weight, bias, gate, activation, eps) -> None:
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         _fail("x needs a sample and a channel dimension")
     if x.dtype not in _STORAGE:
         _fail(f"dtype {x.dtype} is not supported (float32, bfloat16, float16)")
-    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or x.size(-1) % groups:
+    if isinstance(groups, bool) or not isinstance(groups, int) or groups < 1 or shape[-1] % groups:
         _fail("groups must divide the channels")
     if activation not in _ACTIVATIONS:
         _fail(f"activation {activation!r} is not one of {list(_ACTIVATIONS)}")
     if not 0.0 < float(eps) < float("inf"):
         _fail("eps must be positive and finite")
+    channels = shape[-1:]
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and (t.shape != x.shape[-1:] or not t.is_floating_point()):
+        if t is not None and (t.shape != channels or not t.is_floating_point()):
             _fail(f"{name} must have one floating-point value per channel")
-    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+    if gate is not None and (gate.shape != shape or gate.dtype != x.dtype):
         _fail("gate must have the sizes and the dtype of x")
     _check_tensors(x, gate, weight, bias)
 

@@ -169,9 +169,8 @@ def test_what_pytorch_cannot_see_through_is_refused(name):
 
 
 def test_columns_beside_the_state_are_told_from_shared_memory():
-    """Both answers against the sets of bytes."""
-    from linrec_b200.gated import _beside, _check_apart
-
+    """The C entry's answer for every operand in turn, against sets of bytes.  A result that lies between elements,
+    which is looked at later, keeps the accepted calls from going further."""
     def bytes_of(t):
         at = torch.zeros(1, dtype=torch.int64)
         for n, s in zip(t.shape, t.stride()):
@@ -179,25 +178,36 @@ def test_columns_beside_the_state_are_told_from_shared_memory():
         first = t.data_ptr() + at * t.element_size()
         return set((first[:, None] + torch.arange(t.element_size())).flatten().tolist())
 
+    code = {torch.float32: _capi.DTYPE_F32, torch.bfloat16: _capi.DTYPE_BF16}
+    lone = torch.zeros(64)
+    apart = lone.data_ptr()
+
+    def step(state, dtype, rows, D, x=(apart, 8), forget=(apart, 8), gate=(apart, 8), y=apart + 129, decay=apart, slots=None):
+        return _capi.lib.linrec_b200_gated_step(x[0], forget[0], gate[0], x[1], forget[1], gate[1], decay, 8.0, y, state.data_ptr(), state.stride(0),
+                                                state.size(0), slots, 0, rows, D, dtype, None)
+
     buf = torch.zeros(12, 24)
-    states = [buf[2:8, 4:12], buf[:, :8], buf[3:4, :8], buf.view(6, 48)[:, 4:12]]
     half, index = buf.view(torch.bfloat16), buf.view(torch.int32)
-    operands = [buf[:, 12:20], buf[2:8, :4], buf[2:8, 12:], buf[:4, 8:16], buf[2:8, 11:14], buf[:2, 4:12], buf[8:, 4:12], buf[5], buf[1], buf[:, ::3],
-                buf.view(6, 48)[:, 12:20], buf.view(6, 48)[:, 40:], half[:, 24:32], half[2:8, :8], half[:, 23:25], half[8:, 8:16], half[1],
-                half[3, 8:16], index[:, 5], index[0, :9], buf.t()[12:, :], torch.zeros(12, 8), torch.zeros(12, 24)[:, :8]]
-    beside = 0
+    states = [buf[2:8, 4:12], buf[:, :8], buf[3:4, :8], buf.view(6, 48)[:, 4:12]]
+    operands = [buf[:, 12:20], buf[2:8, 12:20], buf[:4, 8:16], buf[2:8, 11:19], buf[:2, 4:12], buf[8:, 4:12], buf.view(6, 48)[:, 12:20],
+                buf.view(6, 48)[:, 40:], half[:, 24:32], half[2:8, :8], half[:, 23:31], half[8:, 8:16], half[3:4, 8:16], buf.view(36, 8)[:9]]
+    answers = set()
     for state in states:
+        slots = torch.zeros(64, dtype=torch.int32).data_ptr()
         for t in operands:
-            shared = bytes_of(state) & bytes_of(t)
-            if _beside(state, t):
-                assert not shared
-                beside += 1
-                continue
-            if shared:
-                with pytest.raises(RuntimeError, match="share memory with the state"):
-                    _check_apart(state, t)
-    _check_apart(states[0], torch.zeros(12, 8), buf[8:], half[8:, :8], index[0, :9], None)
-    assert beside > 0
+            shared = bool(bytes_of(state) & bytes_of(t))
+            for name in ("x", "forget", "gate"):
+                rc = step(state, code[t.dtype], t.size(0), 8, slots=slots, **{name: (t.data_ptr(), t.stride(0))})
+                assert rc in ((_capi.ERR_OVERLAP,) if shared else (_capi.ERR_OVERLAP, _capi.ERR_INVALID_ARG))
+                # columns of their own in rows at the state's distance, and memory on either side of it, are no overlap
+                if t.stride(0) * t.element_size() == state.stride(0) * 4 and not shared:
+                    assert rc == _capi.ERR_INVALID_ARG
+                answers.add((shared, rc))
+        if state.size(0) > 1:
+            inside = state.data_ptr() + state.stride(0) * 4
+            assert step(state, 0, 2, 8, slots=inside) == step(state, 0, 2, 8, decay=inside, slots=slots) == _capi.ERR_OVERLAP
+            assert step(state, 0, 2, 8, y=inside, slots=slots) == _capi.ERR_OVERLAP
+    assert (True, _capi.ERR_OVERLAP) in answers and (False, _capi.ERR_INVALID_ARG) in answers
 
 
 @pytest.mark.parametrize("dtype,kw", [
@@ -219,7 +229,7 @@ def test_c_entry_refuses_pointers_between_elements(dtype, kw):
 
 @pytest.mark.parametrize("at", range(6))
 def test_c_step_refuses_pointers_between_elements(at):
-    p = [16] * 6      # x, forget, input_gate, decay, y, state
+    p = [(i + 1) << 20 for i in range(6)]      # x, forget, input_gate, decay, y, state
     p[at] += 2
     call = lambda slots, wide: _capi.lib.linrec_b200_gated_step(p[0], p[1], p[2], 8, 8, 8, p[3], 8.0, p[4], p[5], 8, 4, slots, wide, 4, 8, _capi.DTYPE_F32, None)
     assert call(None, 0) == _capi.ERR_INVALID_ARG
