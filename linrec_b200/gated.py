@@ -30,7 +30,8 @@ import math
 import torch
 
 from . import _capi
-from .norm import _as_float, _as_rows, _backward_once, _check_tensors, _empty_dense, _fail, _on, _ptr, _STORAGE, _wants_grad, group_norm_act
+from .norm import (_HUGEST, _STORAGE, _TINIEST, _as_float, _as_rows, _backward_once, _check_tensors, _empty_dense, _fail, _on, _ptr,
+                   _wants_grad, group_norm_act)
 from .norm import _apply as _apply_norm, _check as _check_norm
 from .ops import _DTYPES, _workspace
 
@@ -59,8 +60,8 @@ def _check_operands(inputs, forget, input_gate, decay, decay_scale) -> None:
             _fail("decay must have one value per channel")
         if not decay.is_floating_point():
             _fail("decay must be a floating-point tensor")
-        if not 0.0 < decay_scale < math.inf:
-            _fail("decay_scale must be positive and finite")
+        if not _TINIEST < decay_scale < _HUGEST:
+            _fail("decay_scale must be positive and finite in float32")
 
 
 def _check_index(name: str, t) -> None:
@@ -286,7 +287,7 @@ def linrec_gated_step(inputs: torch.Tensor, forget: torch.Tensor, state: torch.T
     i, si = (None, 0) if input_gate is None else _as_rows(input_gate)
     decay = _as_float(decay)
     slots = None if slots is None else slots.contiguous()
-    args = (x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), decay_scale, y.data_ptr(), state.data_ptr(), max(state.stride(0), D),
+    args = (x.data_ptr(), f.data_ptr(), _ptr(i), sx, sf, si, _ptr(decay), float(decay_scale), y.data_ptr(), state.data_ptr(), max(state.stride(0), D),
             state.size(0), _ptr(slots), slots is not None and slots.dtype == torch.int64, rows, D, _DTYPES[inputs.dtype])
 
     def launch(stream):

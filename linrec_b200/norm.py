@@ -27,6 +27,7 @@ __all__ = ["group_norm_act"]
 _STORAGE = (torch.float32, torch.bfloat16, torch.float16)
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_TINIEST, _HUGEST = 2.0 ** -150, 2.0 ** 128 - 2.0 ** 103      # what lies between them is neither zero nor infinite in float32
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 # (looked up once: they are asked for at every call, and a small call is host work)
 _Tensor = torch.Tensor
@@ -196,8 +197,8 @@ def _check(x, groups, weight, bias, gate, activation, eps) -> None:
         _fail("groups must divide the channels")
     if activation not in _ACTIVATIONS:
         _fail(f"activation {activation!r} is not one of {list(_ACTIVATIONS)}")
-    if not 0.0 < float(eps) < float("inf"):
-        _fail("eps must be positive and finite")
+    if not _TINIEST < float(eps) < _HUGEST:
+        _fail("eps must be positive and finite in float32")
     channels = shape[-1:]
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and (t.shape != channels or not t.is_floating_point()):

@@ -235,3 +235,18 @@ def test_c_step_refuses_pointers_between_elements(at):
     assert call(None, 0) == _capi.ERR_INVALID_ARG
     p[at] -= 2
     assert call(18, 0) == call(20, 1) == _capi.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("value", [1e39, 2.0 ** 128 - 2.0 ** 103, 1e-46, 2.0 ** -150])
+def test_scalars_that_float32_cannot_hold(value):
+    """They would reach the kernels as infinity or zero; the largest and smallest that it holds are taken."""
+    d = torch.zeros(8)
+    assert ctypes.c_float(value).value in (0.0, float("inf"))
+    for call, why in ((lambda v: lb.linrec_gated(X, X, input_gate=X, decay=d, decay_scale=v), "decay_scale"),
+                      (lambda v: lb.linrec_gated_step(P, P, P, input_gate=P, decay=d, decay_scale=v), "decay_scale"),
+                      (lambda v: lb.group_norm_act(P, 2, eps=v), "eps")):
+        with pytest.raises(RuntimeError, match=why):
+            call(value)
+        for good in (2.0 ** 128 - 2.0 ** 104, 2.0 ** -149, torch.tensor(8.0)):
+            with pytest.raises(RuntimeError, match="CUDA tensors"):
+                call(good)

@@ -752,3 +752,16 @@ def test_linked_tiles_on_side_streams_and_replayed(columns):
         assert all(torch.equal(w[n], t) for n, t in zip(("y", "final", *NAMES.values()), outs))
     assert all(torch.equal(want[0][n], eager[n]) for n in eager)
     lb.check_status()
+
+
+def test_scale_as_a_tensor():
+    """A scale that is no Python number means the same to the step as to the scan."""
+    lb = _lb()
+    c = {k: v.to(DEV) for k, v in _case((3, 1, 64), True, torch.float32).items()}
+    x, f, i = (c[k] for k in ("inputs", "forget", "input_gate"))
+    want, end = lb.linrec_gated(x, f, input_gate=i, decay=c["decay"], decay_scale=4.0, initial_state=c["initial_state"], return_state=True)
+    for scale in (4.0, 4, torch.tensor(4.0), np.float32(4.0)):
+        state = c["initial_state"].clone()
+        y = lb.linrec_gated_step(x[:, 0], f[:, 0], state, input_gate=i[:, 0], decay=c["decay"], decay_scale=scale)
+        # one position: the same products, each rounded once, whichever kernel forms them (bound of the oracle below 1e-6)
+        assert torch.allclose(y, want[:, 0], rtol=1e-5, atol=1e-6) and torch.allclose(state, end, rtol=1e-5, atol=1e-6)
