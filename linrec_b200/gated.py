@@ -60,7 +60,7 @@ def _check_operands(inputs, forget, input_gate, decay, decay_scale) -> None:
             _fail("decay must have one value per channel")
         if not decay.is_floating_point():
             _fail("decay must be a floating-point tensor")
-        if not _TINIEST < decay_scale < _HUGEST:
+        if not _TINIEST < float(decay_scale) < _HUGEST:
             _fail("decay_scale must be positive and finite in float32")
 
 
