@@ -641,8 +641,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_planes_stats_kernel(cons
         const float count = (float)V * (float)((k.l1 - first + k.Y - 1) / k.Y);
         float about = load_one<ST>(p.x, (row0 + first) * p.sx + ch), m, squares;
         // A second time, about the thread's mean, where the first element lies so far from the others that the squares are
-        // a small difference of large sums (more than a 32nd of them is what an element within five standard deviations
-        // leaves).  (223, 600, 2048) fp32, 32 groups, every sample's first position at 1000: results were off by 1.1 %, now by
+        // less than a 32nd of the sum they are a difference of (within five standard deviations they are more).  (223, 600, 2048) fp32, 32 groups, every sample's first position at 1000: results were off by 1.1 %, now by
         // 2e-6; no time where it does not occur ((8, 8192, 2048) bf16 177 us with and without).
         for (bool again = false;; again = true) {
             float s, q;
